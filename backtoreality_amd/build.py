@@ -43,6 +43,10 @@ HIPCC_FLAGS = [
     # kernels too (929 sites), and the guard below had nothing to say about them.  Memory
     # operations are merged by another pass and are unaffected.
     "-fno-vectorize",
+    # ... and no packed f32 instruction at all: the instruction selector makes them from ordinary
+    # float2 / scalar code by itself where the target feature is on (the host pass of hipcc says that
+    # it does not know the feature; harmless).
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 # sources whose code depends on BTR_FMAD (they evaluate sq3() / dot3()): the index-producing ones
 MODE_SOURCES = ("ball_query.hip", "ball_query_bucket.hip", "ball_query_grid.hip",
