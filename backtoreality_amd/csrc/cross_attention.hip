@@ -1,0 +1,914 @@
+// cross_attention.hip -- attention of a batch of queries onto keys / values of another length:
+//
+//   S = scale q k^T over the keys that are not padding,  P = softmax(S),  out = P v       per head
+//   backward: D = rowsum(dout * out),  dS = P * (dout v^T - D),
+//             dv = P^T dout,  dq = scale dS k,  dk = scale dS^T q
+//
+// for float32, bfloat16 and float16, head widths up to 128, any lengths, per-batch key counts and
+// / or a padding mask, and query heads that share key / value heads (h = g * hk).
+// (reference: the attention of detection/GroupFree3D/models/transformer.py:36-76 with the
+// key_padding_mask of models/multi_head_attention.py; csrc/attention.hip is the f32, unpadded core
+// with dropout that the whole-layer call uses.)
+//
+// Rows.  The g query heads of one key head are rows of ONE product: row r of (batch, key head) is
+// query r / g, head r % g of the group.  A single new query with 8 heads a group is then 8 rows of
+// a tile instead of 8 one-row tiles, the keys are read once for all of them, and dk / dv sum over
+// the group inside a workgroup: no atomics anywhere, equal results from run to run.
+//
+// Orientation.  Every product is arranged so that the lane that holds a score also holds it where
+// the next product wants it.  Forward and dq compute S^T = K Q^T (32x32 tiles): a lane then has 16
+// keys of ONE row, so maximum and sum are reductions over its own registers plus one exchange with
+// the other half of the wave, the rescaling factor of a row is the lane's own, and the 16 values
+// are, unmoved, the B operand of O^T += V^T P^T -- in a permuted key order that the A operand
+// follows (a sum over keys does not care).  dk / dv compute S = Q K^T: a lane has 16 rows of one key
+// and the same holds.  V^T, K^T, Q^T, dO^T fragments come from the row-major tiles by gfx950's LDS
+// transpose read (16-bit) or 4-byte reads (f32).
+//
+// Numbers: scores, maxima, sums, O, dq, dk, dv accumulate in f32.  For 16-bit inputs P and dS are
+// rounded to the input type where they enter the matrix instructions (relative error half an
+// ulp per term; P <= 1).  f32 runs on the f32 matrix instructions, nothing is rounded below 32 bits.
+#include <algorithm>
+
+#include "decoder_ops.hpp"
+
+#pragma clang fp contract(fast)
+
+namespace btr {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct XaArgs {
+  int b, lq, lk, h, hk, g, d, rows;              // rows = lq * g
+  const void *q, *k, *v, *dout;
+  long long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;   // element strides
+  const int *lengths;                            // (b) or NULL
+  const unsigned char *mask;                     // (b, lk), nonzero = padding, or NULL
+  long long mask_sb;
+  void *out;                                     // (b, lq, h, d)
+  float *lse;      // (b * hk, rows): log2 of the row's sum of exp2(scale_log2 * s); +inf: no key
+  float *delta;    // (b * hk, rows): D
+  void *dq, *dk, *dv;                            // contiguous, shaped like q, k, v
+  float scale, scale_log2;
+  int tiles, nsplit, chunk;                      // workgroup tiles, shares of the long axis, its length
+  float *part, *part2;                           // partial results of the shares
+};
+
+typedef __attribute__((address_space(3))) s16x4_t *lds_s16x4;
+
+// ------------------------------------------------------------------------------- tiles in LDS
+// Row-major [row][DP]; PITCH bytes a row.  16-bit: 64 mod 128 bytes and the 16-byte units of a row
+// XOR-ed with (row / 4) % 4, so that both ways of reading -- sixteen rows at one column, and 4 x 16
+// blocks for the transpose read -- touch every bank once.  f32: one 16-byte unit of padding.
+template <typename T, int DP>
+struct Tile {
+  static constexpr int V = Elem<T>::kVec;
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int PITCH = F32 ? DP * 4 + 16 : (DP * 2) % 128 == 64 ? DP * 2 : DP * 2 + 64;
+  static constexpr int UNITS = DP / V;           // 16-byte units of a row
+  __device__ static __forceinline__ int unit_off(int row, int unit) {
+    return row * PITCH + (F32 ? unit : unit ^ ((row >> 2) & 3)) * 16;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16_t mma(typename Elem<T>::Vec a, typename Elem<T>::Vec b, f32x16_t c);
+template <>
+__device__ __forceinline__ f32x16_t mma<__bf16>(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16_t mma<_Float16>(f16x8_t a, f16x8_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+template <>   // f32: the 16 bytes are four reduction steps of two
+__device__ __forceinline__ f32x16_t mma<float>(f32x4_t a, f32x4_t b, f32x16_t c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
+// row of a 32x32 result tile that register v of lane half hh holds (its column is lane & 31)
+__device__ __forceinline__ constexpr int acc_row(int v, int hh) {
+  return (v & 3) + 8 * (v >> 2) + 4 * hh;
+}
+
+// first product: tile rows [row0, row0 + 32) x the register operand f (one row per lane & 31)
+template <typename T, int DP>
+__device__ __forceinline__ f32x16_t tile_times_rows(const char *tile, int row0, int l31, int hh,
+                                                    const typename Elem<T>::Vec *f) {
+  typedef Tile<T, DP> TL;
+  f32x16_t acc = {};
+#pragma unroll
+  for (int j = 0; j < TL::UNITS / 2; ++j) {
+    const auto a = *reinterpret_cast<const typename Elem<T>::Vec *>(
+        tile + row0 * TL::PITCH + TL::unit_off(l31, 2 * j + hh));
+    acc = mma<T>(a, f[j], acc);
+  }
+  return acc;
+}
+
+// second product: acc[nt] (32 columns of the tile x 32) += tile[row0 .. row0 + 32)^T w, w as the
+// first product left it (register v: tile row acc_row(v, hh))
+template <typename T, int DP>
+__device__ __forceinline__ void tile_t_times(const char *tile, int row0, int lane,
+                                             const f32x16_t &w, f32x16_t *acc) {
+  typedef Tile<T, DP> TL;
+  const int l31 = lane & 31, hh = lane >> 5;
+  const char *t = tile + row0 * TL::PITCH;
+  if constexpr (TL::F32) {
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+      const float *row = reinterpret_cast<const float *>(t + acc_row(s, hh) * TL::PITCH);
+#pragma unroll
+      for (int nt = 0; nt < DP / 32; ++nt)
+        acc[nt] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * nt + l31], w[s], acc[nt], 0, 0, 0);
+    }
+  } else {
+    // lane p of a group of 16 addresses row p / 4, columns 4 (p % 4) .. + 3 of a [4][16] block and
+    // receives column p, rows 0 .. 3
+    const int p = lane & 15, half = (lane >> 4) & 1;
+    const int unit = 2 * half + ((p & 3) >> 1), sub = (p & 1) * 8;
+    const char *lo = t + (4 * hh + (p >> 2)) * TL::PITCH + (unit ^ hh) * 16 + sub;
+    const char *hi = t + (8 + 4 * hh + (p >> 2)) * TL::PITCH + (unit ^ (hh + 2)) * 16 + sub;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      typename Elem<T>::Vec bv;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bv[j] = (T)w[8 * s + j];
+#pragma unroll
+      for (int nt = 0; nt < DP / 32; ++nt) {
+        union {
+          s16x4_t s4[2];
+          typename Elem<T>::Vec v;
+        } u;
+        u.s4[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4)(lo + 16 * s * TL::PITCH + 64 * nt));
+        u.s4[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4)(hi + 16 * s * TL::PITCH + 64 * nt));
+        acc[nt] = mma<T>(u.v, bv, acc[nt]);
+      }
+    }
+  }
+}
+
+// value of the lane 32 away
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// NR rows of a tile, global -> registers (a tile ahead) -> LDS
+template <typename T, int DP, int NR, int THREADS>
+struct Stage {
+  typedef Tile<T, DP> TL;
+  static constexpr int N = (NR * TL::UNITS + THREADS - 1) / THREADS;
+  static constexpr bool EXACT = NR * TL::UNITS % THREADS == 0;
+  typename Elem<T>::Vec r[N];
+  // addr(row) -> pointer of the row (called for rows < limit only)
+  template <typename F>
+  __device__ __forceinline__ void fetch(F addr, int row0, int limit, int d, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + THREADS * i, row = e / TL::UNITS, col = (e % TL::UNITS) * TL::V;
+      r[i] = typename Elem<T>::Vec{};
+      if ((EXACT || row < NR) && row0 + row < limit && col < d)
+        r[i] = load_row(addr(row0 + row), col, d);
+    }
+  }
+  // rows whose bit in `live` is clear become zero whatever they hold (a padded row may hold NaN)
+  __device__ __forceinline__ void store(char *tile, const unsigned long long *live, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + THREADS * i, row = e / TL::UNITS, unit = e % TL::UNITS;
+      if (!EXACT && row >= NR) continue;
+      typename Elem<T>::Vec v = r[i];
+      if (live && !((live[row >> 6] >> (row & 63)) & 1)) v = typename Elem<T>::Vec{};
+      *reinterpret_cast<typename Elem<T>::Vec *>(tile + TL::unit_off(row, unit)) = v;
+    }
+  }
+};
+
+// which keys of a tile take part, one bit each
+template <int NR>
+struct Live {
+  static constexpr int W = (NR + 63) / 64;
+  unsigned char m[W];
+  __device__ __forceinline__ void fetch(const unsigned char *mask, int key0, int kend, int lane) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int key = key0 + 64 * i + lane;
+      m[i] = mask && key < kend ? mask[key] : 0;
+    }
+  }
+  __device__ __forceinline__ void words(int key0, int kend, int lane, unsigned long long *w) const {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = __ballot(key0 + 64 * i + lane < kend && m[i] == 0);
+  }
+};
+
+// workgroup -> (tile, batch x key head, share): consecutive workgroups land on the eight XCDs in
+// turn, so each XCD is given a contiguous eighth of the list, in which the tiles that read the
+// same keys follow each other and share its L2
+__device__ __forceinline__ void place(const XaArgs &a, int &tile, int &bh, int &split) {
+  const int n = gridDim.x, id = blockIdx.x, per = n / 8;
+  const int w = id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+  tile = w % a.tiles;
+  const int t = w / a.tiles;
+  split = t % a.nsplit;
+  bh = t / a.nsplit;
+}
+
+template <typename T>
+struct Rows {   // row r of (batch, key head) -> element offset of its query / its output
+  const XaArgs &a;
+  int b, kh;
+  __device__ __forceinline__ const T *q(int r) const {
+    const int l = r / a.g, hd = kh * a.g + r - l * a.g;
+    return (const T *)a.q + b * a.q_sb + l * a.q_sl + hd * a.q_sh;
+  }
+  __device__ __forceinline__ long long o(int r) const {   // out, dout, dq: contiguous
+    const int l = r / a.g, hd = kh * a.g + r - l * a.g;
+    return (((long long)b * a.lq + l) * a.h + hd) * a.d;
+  }
+};
+
+__device__ __forceinline__ int key_count(const XaArgs &a, int b) {
+  int n = a.lk;
+  if (a.lengths) n = min(n, max(a.lengths[b], 0));
+  return n;
+}
+
+// four consecutive columns of a row
+template <typename T>
+__device__ __forceinline__ void store4(T *row, int c, int d, const float (&v)[4]) {
+  typedef T U4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (c + 4 <= d) {
+    U4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (T)v[j];
+    *reinterpret_cast<U4 *>(row + c) = o;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < d) row[c + j] = (T)v[j];
+  }
+}
+
+// Sums of the waves that split the keys (WK > 1): wave w's acc[nt] times its factor f, added in
+// wave order; the result of row `row` (of 32) at out(row, column)
+constexpr int kMergePitch = 4;   // floats between rows beyond DP: rows land on different banks
+
+// -------------------------------------------------------------------------------- forward
+// WR waves along the rows (32 each) x WK along the keys, KT key subtiles of 32 per wave and tile.
+//   WR 4, WK 1: >= 33 rows; the four waves share every K / V tile.
+//   WR 1, WK 4: few rows (single queries): the waves take a quarter of every tile and merge.
+// NBUF 2: tiles double-buffered, one barrier a tile.
+template <typename T, int DP, int WR, int WK, int KT, int NBUF>
+__global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int BKV = 32 * WK * KT, NT = DP / 32, TB = BKV * TL::PITCH;
+  constexpr int MERGE = WK > 1 ? WK * 32 * (DP + kMergePitch) * 4 : 0;
+  constexpr int BYTES = 2 * TB * NBUF > MERGE ? 2 * TB * NBUF : MERGE;
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  __shared__ float mx[WK > 1 ? WK * 32 : 1], sm[WK > 1 ? WK * 32 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
+  const int wr = w % WR, wk = w / WR;
+  int tile, bh, split;
+  place(a, tile, bh, split);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
+  const T *kp = (const T *)a.k + b * a.k_sb + kh * a.k_sh;
+  const T *vp = (const T *)a.v + b * a.v_sb + kh * a.v_sh;
+  const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const Rows<T> rows{a, b, kh};
+  const int r = tile * 32 * WR + 32 * wr + l31;
+
+  Vec qf[TL::UNITS / 2];
+#pragma unroll
+  for (int j = 0; j < TL::UNITS / 2; ++j) {
+    qf[j] = Vec{};
+    if (r < a.rows) qf[j] = load_row(rows.q(r), (2 * j + hh) * TL::V, a.d);
+  }
+  f32x16_t o[NT] = {};
+  float m = -INFINITY, l = 0.f;
+
+  Stage<T, DP, BKV, 256> sk, sv;
+  Live<BKV> lv;
+  auto krow = [&](int key) { return kp + key * a.k_sl; };
+  auto vrow = [&](int key) { return vp + key * a.v_sl; };
+  if (kbeg < kend) {
+    sk.fetch(krow, kbeg, kend, a.d, tid);
+    sv.fetch(vrow, kbeg, kend, a.d, tid);
+    lv.fetch(mask, kbeg, kend, lane);
+  }
+  int buf = 0;
+  for (int k0 = kbeg; k0 < kend; k0 += BKV) {
+    char *kt = smem + buf * 2 * TB, *vt = kt + TB;
+    unsigned long long live[Live<BKV>::W];
+    lv.words(k0, kend, lane, live);
+    if (NBUF == 1) lds_barrier();                // the previous tile's reads are done
+    sk.store(kt, mask ? live : nullptr, tid);
+    sv.store(vt, mask ? live : nullptr, tid);
+    if (k0 + BKV < kend) {                       // next tile's loads fly under this one's math
+      sk.fetch(krow, k0 + BKV, kend, a.d, tid);
+      sv.fetch(vrow, k0 + BKV, kend, a.d, tid);
+      lv.fetch(mask, k0 + BKV, kend, lane);
+    }
+    lds_barrier();
+    if (NBUF == 2) buf ^= 1;
+    f32x16_t s[KT];
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const int sub = wk * KT + t;
+      const unsigned bits = (unsigned)(live[sub >> 1] >> (32 * (sub & 1)));
+      s[t] = tile_times_rows<T, DP>(kt, 32 * sub, l31, hh, qf);
+      if (bits != 0xffffffffu) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (!((bits >> acc_row(v, hh)) & 1)) s[t][v] = -INFINITY;
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) top = fmaxf(top, s[t][v]);
+    }
+    top = fmaxf(top, other_half(top));
+    if (__ballot(top > m)) {                     // some row's maximum moved
+      const float mn = fmaxf(m, top);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.scale_log2);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[nt][v] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : m * a.scale_log2;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        s[t][v] = __builtin_amdgcn_exp2f(fmaf(s[t][v], a.scale_log2, -base));
+        l += s[t][v];
+      }
+      tile_t_times<T, DP>(vt, 32 * (wk * KT + t), lane, s[t], o);
+    }
+  }
+  l += other_half(l);
+
+  float *po = nullptr, *pm = nullptr;
+  const long long prow = ((long long)split * a.b * a.hk + bh) * a.rows;   // + row
+  if (a.nsplit > 1) {
+    po = a.part;
+    pm = a.part2;
+  }
+  // (maximum in units of log2, sum) of the rows
+  if constexpr (WK == 1) {
+    if (r >= a.rows) return;
+    const float mb = m * a.scale_log2;           // (-inf stays -inf)
+    if (po) {
+      float *dst = po + (prow + r) * a.d;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int gq = 0; gq < 4; ++gq) {
+          const float v4[4] = {o[nt][4 * gq], o[nt][4 * gq + 1], o[nt][4 * gq + 2],
+                               o[nt][4 * gq + 3]};
+          store4(dst, 32 * nt + 8 * gq + 4 * hh, a.d, v4);
+        }
+      if (hh == 0) {
+        pm[2 * (prow + r)] = mb;
+        pm[2 * (prow + r) + 1] = l;
+      }
+    } else {
+      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // (NaN stays NaN)
+      T *dst = (T *)a.out + rows.o(r);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int gq = 0; gq < 4; ++gq) {
+          const float v4[4] = {o[nt][4 * gq] * inv, o[nt][4 * gq + 1] * inv,
+                               o[nt][4 * gq + 2] * inv, o[nt][4 * gq + 3] * inv};
+          store4(dst, 32 * nt + 8 * gq + 4 * hh, a.d, v4);
+        }
+      if (hh == 0 && a.lse)
+        a.lse[(long long)bh * a.rows + r] = l == 0.f ? INFINITY : mb + __builtin_amdgcn_logf(l);
+    }
+  } else {
+    constexpr int LDO = DP + kMergePitch;
+    float *om = reinterpret_cast<float *>(smem);
+    __syncthreads();                             // every wave is done with the tiles
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq)
+        *reinterpret_cast<f32x4_t *>(om + (wk * 32 + l31) * LDO + 32 * nt + 8 * gq + 4 * hh) =
+            f32x4_t{o[nt][4 * gq], o[nt][4 * gq + 1], o[nt][4 * gq + 2], o[nt][4 * gq + 3]};
+    if (hh == 0) {
+      mx[wk * 32 + l31] = m * a.scale_log2;
+      sm[wk * 32 + l31] = l;
+    }
+    __syncthreads();
+    const int row = tid >> 3, sub = tid & 7, rr = tile * 32 + row;
+    if (rr >= a.rows) return;
+    float M = -INFINITY, L = 0.f, f[WK];
+#pragma unroll
+    for (int k = 0; k < WK; ++k) M = fmaxf(M, mx[k * 32 + row]);
+#pragma unroll
+    for (int k = 0; k < WK; ++k) {
+      f[k] = mx[k * 32 + row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[k * 32 + row] - M);
+      L = fmaf(sm[k * 32 + row], f[k], L);
+    }
+    const float inv = po ? 1.f : L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+    for (int c = 4 * sub; c < a.d; c += 32) {
+      f32x4_t t = {};
+#pragma unroll
+      for (int k = 0; k < WK; ++k)
+        t += *reinterpret_cast<const f32x4_t *>(om + (k * 32 + row) * LDO + c) * f[k];
+      const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
+      if (po)
+        store4(po + (prow + rr) * a.d, c, a.d, v4);
+      else
+        store4((T *)a.out + rows.o(rr), c, a.d, v4);
+    }
+    if (sub == 0) {
+      if (po) {
+        pm[2 * (prow + rr)] = M;
+        pm[2 * (prow + rr) + 1] = L;
+      } else if (a.lse) {
+        a.lse[(long long)bh * a.rows + rr] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+      }
+    }
+  }
+}
+
+// joins the shares: 32 threads a row, fixed order
+template <typename T>
+__global__ __launch_bounds__(256) void cross_attention_join_kernel(XaArgs a) {
+  const long long nrow = (long long)a.b * a.hk * a.rows;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= nrow) return;
+  const int bh = (int)(row / a.rows), r = (int)(row - (long long)bh * a.rows);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  float M = -INFINITY, L = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, a.part2[2 * (s * nrow + row)]);
+  // a share's weight: without a finite score its sum itself, which is 0, or NaN if its scores were
+  auto weight = [&](int s) {
+    const float m = a.part2[2 * (s * nrow + row)];
+    return m == -INFINITY ? a.part2[2 * (s * nrow + row) + 1] : __builtin_amdgcn_exp2f(m - M);
+  };
+  for (int s = 0; s < a.nsplit; ++s)
+    L = fmaf(a.part2[2 * (s * nrow + row) + 1], weight(s), L);
+  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  const Rows<T> rows{a, b, kh};
+  T *dst = (T *)a.out + rows.o(r);
+  for (int c = threadIdx.x & 31; c < a.d; c += 32) {
+    float t = 0.f;
+    for (int s = 0; s < a.nsplit; ++s)
+      t = fmaf(a.part[(s * nrow + row) * a.d + c], weight(s), t);
+    dst[c] = (T)(t * inv);
+  }
+  if ((threadIdx.x & 31) == 0 && a.lse)
+    a.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+}
+
+// -------------------------------------------------------------------------------- backward, dq
+// As the forward: per tile S^T = K Q^T, dP^T = V dO^T, dS^T in place, dq^T += K^T dS^T.  D = rowsum
+// (dO * O) comes first, from the same fragments, and is left for the dk / dv kernel.
+template <typename T, int DP, int WR, int WK, int KT>
+__global__ __launch_bounds__(256) void cross_attention_bwd_q_kernel(XaArgs a) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int BKV = 32 * WK * KT, NT = DP / 32, TB = BKV * TL::PITCH;
+  constexpr int MERGE = WK > 1 ? WK * 32 * (DP + kMergePitch) * 4 : 0;
+  constexpr int BYTES = 2 * TB > MERGE ? 2 * TB : MERGE;
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
+  const int wr = w % WR, wk = w / WR;
+  int tile, bh, split;
+  place(a, tile, bh, split);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
+  const T *kp = (const T *)a.k + b * a.k_sb + kh * a.k_sh;
+  const T *vp = (const T *)a.v + b * a.v_sb + kh * a.v_sh;
+  const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const Rows<T> rows{a, b, kh};
+  const int r = tile * 32 * WR + 32 * wr + l31;
+
+  Vec qf[TL::UNITS / 2], gf[TL::UNITS / 2];
+  float delta = 0.f, lse = INFINITY;
+#pragma unroll
+  for (int j = 0; j < TL::UNITS / 2; ++j) {
+    qf[j] = gf[j] = Vec{};
+    if (r < a.rows) {
+      const int c = (2 * j + hh) * TL::V;
+      qf[j] = load_row(rows.q(r), c, a.d);
+      gf[j] = load_row((const T *)a.dout + rows.o(r), c, a.d);
+      const Vec of = load_row((const T *)a.out + rows.o(r), c, a.d);
+#pragma unroll
+      for (int i = 0; i < TL::V; ++i) delta = fmaf((float)gf[j][i], (float)of[i], delta);
+    }
+  }
+  delta += other_half(delta);
+  if (r < a.rows) {
+    lse = a.lse[(long long)bh * a.rows + r];
+    if (split == 0 && wk == 0 && hh == 0) a.delta[(long long)bh * a.rows + r] = delta;
+  }
+  f32x16_t dq[NT] = {};
+
+  Stage<T, DP, BKV, 256> sk, sv;
+  Live<BKV> lv;
+  auto krow = [&](int key) { return kp + key * a.k_sl; };
+  auto vrow = [&](int key) { return vp + key * a.v_sl; };
+  if (kbeg < kend) {
+    sk.fetch(krow, kbeg, kend, a.d, tid);
+    sv.fetch(vrow, kbeg, kend, a.d, tid);
+    lv.fetch(mask, kbeg, kend, lane);
+  }
+  char *kt = smem, *vt = smem + TB;
+  for (int k0 = kbeg; k0 < kend; k0 += BKV) {
+    unsigned long long live[Live<BKV>::W];
+    lv.words(k0, kend, lane, live);
+    lds_barrier();
+    sk.store(kt, mask ? live : nullptr, tid);
+    sv.store(vt, mask ? live : nullptr, tid);
+    if (k0 + BKV < kend) {
+      sk.fetch(krow, k0 + BKV, kend, a.d, tid);
+      sv.fetch(vrow, k0 + BKV, kend, a.d, tid);
+      lv.fetch(mask, k0 + BKV, kend, lane);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const int sub = wk * KT + t;
+      const unsigned bits = (unsigned)(live[sub >> 1] >> (32 * (sub & 1)));
+      f32x16_t s = tile_times_rows<T, DP>(kt, 32 * sub, l31, hh, qf);
+      const f32x16_t dp = tile_times_rows<T, DP>(vt, 32 * sub, l31, hh, gf);
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], a.scale_log2, -lse)) * (dp[v] - delta);
+      if (bits != 0xffffffffu) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (!((bits >> acc_row(v, hh)) & 1)) s[v] = 0.f;
+      }
+      tile_t_times<T, DP>(kt, 32 * sub, lane, s, dq);
+    }
+  }
+  const long long prow = ((long long)split * a.b * a.hk + bh) * a.rows;
+  if constexpr (WK == 1) {
+    if (r >= a.rows) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const float v4[4] = {dq[nt][4 * gq] * a.scale, dq[nt][4 * gq + 1] * a.scale,
+                             dq[nt][4 * gq + 2] * a.scale, dq[nt][4 * gq + 3] * a.scale};
+        const int c = 32 * nt + 8 * gq + 4 * hh;
+        if (a.nsplit > 1)
+          store4(a.part + (prow + r) * a.d, c, a.d, v4);
+        else
+          store4((T *)a.dq + rows.o(r), c, a.d, v4);
+      }
+  } else {
+    constexpr int LDO = DP + kMergePitch;
+    float *om = reinterpret_cast<float *>(smem);
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq)
+        *reinterpret_cast<f32x4_t *>(om + (wk * 32 + l31) * LDO + 32 * nt + 8 * gq + 4 * hh) =
+            f32x4_t{dq[nt][4 * gq], dq[nt][4 * gq + 1], dq[nt][4 * gq + 2], dq[nt][4 * gq + 3]};
+    __syncthreads();
+    const int row = tid >> 3, sub = tid & 7, rr = tile * 32 + row;
+    if (rr >= a.rows) return;
+    for (int c = 4 * sub; c < a.d; c += 32) {
+      f32x4_t t = {};
+#pragma unroll
+      for (int k = 0; k < WK; ++k)
+        t += *reinterpret_cast<const f32x4_t *>(om + (k * 32 + row) * LDO + c);
+      const float v4[4] = {t[0] * a.scale, t[1] * a.scale, t[2] * a.scale, t[3] * a.scale};
+      if (a.nsplit > 1)
+        store4(a.part + (prow + rr) * a.d, c, a.d, v4);
+      else
+        store4((T *)a.dq + rows.o(rr), c, a.d, v4);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- backward, dk, dv
+// Four waves x 32 keys; the rows pass by in tiles of 32.  S = Q K^T, dP = dO V^T with K and V rows
+// in registers, then dv^T += dO^T P and dk^T += Q^T dS.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void cross_attention_bwd_kv_kernel(XaArgs a) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int BR = 32, NT = DP / 32, TB = BR * TL::PITCH;
+  __shared__ __attribute__((aligned(16))) char smem[4 * TB];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][BR];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
+  int tile, bh, split;
+  place(a, tile, bh, split);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int nk = key_count(a, b);
+  const int rbeg = split * a.chunk;
+  int rend = min(a.rows, rbeg + a.chunk);
+  if (tile * 128 >= nk) rend = rbeg;             // padding only: zeros
+  const int key = tile * 128 + 32 * w + l31;
+  const bool live = key < nk && !(a.mask && a.mask[b * a.mask_sb + key]);
+  const Rows<T> rows{a, b, kh};
+
+  Vec kf[TL::UNITS / 2], vf[TL::UNITS / 2];
+#pragma unroll
+  for (int j = 0; j < TL::UNITS / 2; ++j) {
+    kf[j] = vf[j] = Vec{};
+    if (live) {
+      const int c = (2 * j + hh) * TL::V;
+      kf[j] = load_row((const T *)a.k + b * a.k_sb + kh * a.k_sh + key * a.k_sl, c, a.d);
+      vf[j] = load_row((const T *)a.v + b * a.v_sb + kh * a.v_sh + key * a.v_sl, c, a.d);
+    }
+  }
+  f32x16_t dk[NT] = {}, dv[NT] = {};
+  Stage<T, DP, BR, 256> sq, sg;
+  float st = 0.f;
+  auto qrow = [&](int r) { return rows.q(r); };
+  auto grow = [&](int r) { return (const T *)a.dout + rows.o(r); };
+  auto fetch = [&](int r0) {
+    sq.fetch(qrow, r0, rend, a.d, tid);
+    sg.fetch(grow, r0, rend, a.d, tid);
+    if (tid < 2 * BR) {                          // lse (+inf beyond the rows: P = 0), then D
+      const int r = r0 + (tid & (BR - 1));
+      const float *src = tid < BR ? a.lse : a.delta;
+      st = r < rend ? src[(long long)bh * a.rows + r] : tid < BR ? INFINITY : 0.f;
+    }
+  };
+  if (rbeg < rend) fetch(rbeg);
+  int buf = 0;
+  for (int r0 = rbeg; r0 < rend; r0 += BR) {
+    char *qt = smem + buf * 2 * TB, *gt = qt + TB;
+    float *lse = stat[buf][0], *dl = stat[buf][1];
+    sq.store(qt, nullptr, tid);
+    sg.store(gt, nullptr, tid);
+    if (tid < 2 * BR) (tid < BR ? lse : dl)[tid & (BR - 1)] = st;
+    if (r0 + BR < rend) fetch(r0 + BR);
+    lds_barrier();
+    buf ^= 1;
+    f32x16_t p = tile_times_rows<T, DP>(qt, 0, l31, hh, kf);
+    f32x16_t ds = tile_times_rows<T, DP>(gt, 0, l31, hh, vf);
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(lse + 8 * gq + 4 * hh);
+      const f32x4_t d4 = *reinterpret_cast<const f32x4_t *>(dl + 8 * gq + 4 * hh);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int v = 4 * gq + i;
+        p[v] = live ? __builtin_amdgcn_exp2f(fmaf(p[v], a.scale_log2, -l4[i])) : 0.f;
+        ds[v] = live ? p[v] * (ds[v] - d4[i]) : 0.f;
+      }
+    }
+    tile_t_times<T, DP>(gt, 0, lane, p, dv);
+    tile_t_times<T, DP>(qt, 0, lane, ds, dk);
+  }
+  if (key >= a.lk) return;
+  const long long krow = (((long long)b * a.lk + key) * a.hk + kh) * a.d;
+  const long long ptotal = (long long)a.b * a.lk * a.hk * a.d;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const int c = 32 * nt + 8 * gq + 4 * hh;
+      const float k4[4] = {dk[nt][4 * gq] * a.scale, dk[nt][4 * gq + 1] * a.scale,
+                           dk[nt][4 * gq + 2] * a.scale, dk[nt][4 * gq + 3] * a.scale};
+      const float v4[4] = {dv[nt][4 * gq], dv[nt][4 * gq + 1], dv[nt][4 * gq + 2],
+                           dv[nt][4 * gq + 3]};
+      if (a.nsplit > 1) {
+        store4(a.part + split * ptotal + krow, c, a.d, k4);
+        store4(a.part2 + split * ptotal + krow, c, a.d, v4);
+      } else {
+        store4((T *)a.dk + krow, c, a.d, k4);
+        store4((T *)a.dv + krow, c, a.d, v4);
+      }
+    }
+}
+
+// out[i] = sum over the shares, in order; blockIdx.y picks one of two tensors.  ROWS: the share is
+// laid out (batch, key head, row, d), the tensor (batch, query, head, d)
+template <typename T, bool ROWS>
+__global__ __launch_bounds__(256) void cross_attention_sum_kernel(XaArgs a, long long n, T *out0,
+                                                                  T *out1) {
+  const float *p = blockIdx.y ? a.part2 : a.part;
+  T *out = blockIdx.y ? out1 : out0;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
+       i += (long long)gridDim.x * 256) {
+    float t = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) t += p[s * n + i];
+    long long dst = i;
+    if (ROWS) {
+      const long long row = i / a.d;
+      const int bh = (int)(row / a.rows), r = (int)(row - (long long)bh * a.rows);
+      const Rows<T> rows{a, bh / a.hk, bh % a.hk};
+      dst = rows.o(r) + (i - row * a.d);
+    }
+    out[dst] = (T)t;
+  }
+}
+
+// ------------------------------------------------------------------------------------ host
+constexpr int kFewRows = 32;     // one tile of rows: the waves split the keys instead
+
+struct Shares {
+  int tiles, n, chunk;
+};
+
+// Shares of the long axis: one where the tiles alone give every CU two workgroups; else enough for
+// about four per CU, none shorter than `least`.
+Shares shares(int tiles, long long bh, int length, int step, int least) {
+  const long long base = std::max<long long>(1, tiles * bh);
+  long long n = 1;
+  if (base < 512) n = std::min<long long>((1024 + base - 1) / base, length / least);
+  n = std::max<long long>(1, n);
+  int chunk = cdiv(length, n);
+  chunk = std::max(step, cdiv(chunk, step) * step);
+  return {tiles, std::max(1, cdiv(length, chunk)), chunk};
+}
+bool few(int rows) { return rows <= kFewRows; }
+Shares row_shares(int b, int lk, int hk, int rows) {   // forward, dq: over the keys
+  return shares(cdiv(rows, few(rows) ? 32 : 128), (long long)b * hk, lk, 128, 256);
+}
+Shares key_shares(int b, int lk, int hk, int rows) {   // dk, dv: over the rows
+  return shares(cdiv(lk, 128), (long long)b * hk, rows, 32, 128);
+}
+
+template <typename T, int DP>
+void launch_fwd(const XaArgs &a, hipStream_t hs) {
+  const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
+  if (few(a.rows))
+    hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 1, 4, 1, 1>), grid, dim3(256), 0, hs, a);
+  else
+    hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 4, 1, 2, 1>), grid, dim3(256), 0, hs, a);
+}
+template <typename T, int DP>
+void launch_bwd_q(const XaArgs &a, hipStream_t hs) {
+  const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
+  if (few(a.rows))
+    hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 1, 4, 1>), grid, dim3(256), 0, hs, a);
+  else
+    hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 4, 1, 2>), grid, dim3(256), 0, hs, a);
+}
+template <typename T, int DP>
+void launch_bwd_kv(const XaArgs &a, hipStream_t hs) {
+  const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
+  hipLaunchKernelGGL((cross_attention_bwd_kv_kernel<T, DP>), grid, dim3(256), 0, hs, a);
+}
+
+#define BTR_XA_WIDTH(FN, ...)                  \
+  do {                                         \
+    if (a.d <= 32) FN<T, 32>(__VA_ARGS__);     \
+    else if (a.d <= 64) FN<T, 64>(__VA_ARGS__);\
+    else if (a.d <= 96) FN<T, 96>(__VA_ARGS__);\
+    else FN<T, 128>(__VA_ARGS__);              \
+  } while (0)
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+int check(const char *what, const btr_cross_attention_t *p, XaArgs &a) {
+  BTR_REQUIRE(p, "%s: null description", what);
+  BTR_REQUIRE(p->dtype >= BTR_F32 && p->dtype <= BTR_F16, "%s: unknown element type %d", what,
+              p->dtype);
+  BTR_REQUIRE(p->b >= 0 && p->lq >= 0 && p->lk >= 0 && p->h >= 1 && p->hk >= 1 &&
+                  p->h % p->hk == 0,
+              "%s: batch %d, queries %d, keys %d, heads %d on %d key heads", what, p->b, p->lq,
+              p->lk, p->h, p->hk);
+  BTR_REQUIRE(p->d >= 1 && p->d <= 128, "%s: head width %d (1 .. 128)", what, p->d);
+  BTR_REQUIRE(p->scale > 0.f && p->scale < INFINITY, "%s: scale %g", what, p->scale);
+  a = XaArgs{};
+  a.b = p->b; a.lq = p->lq; a.lk = p->lk; a.h = p->h; a.hk = p->hk; a.g = p->h / p->hk; a.d = p->d;
+  const long long rows = (long long)p->lq * a.g;
+  // a workgroup list and a row index of 32 bits
+  BTR_REQUIRE(rows <= (1 << 30) && p->lk <= (1 << 30) &&
+                  (rows / 32 + p->lk / 128 + 2) * (long long)p->b * p->hk <= (1 << 30),
+              "%s: too many rows (%lld) or keys (%d)", what, rows, p->lk);
+  a.rows = (int)rows;
+  a.q = p->q; a.k = p->k; a.v = p->v;
+  a.q_sb = p->q_sb; a.q_sl = p->q_sl; a.q_sh = p->q_sh;
+  a.k_sb = p->k_sb; a.k_sl = p->k_sl; a.k_sh = p->k_sh;
+  a.v_sb = p->v_sb; a.v_sl = p->v_sl; a.v_sh = p->v_sh;
+  a.lengths = p->lengths;
+  a.mask = p->mask;
+  a.mask_sb = p->mask_sb;
+  a.scale = p->scale;
+  a.scale_log2 = p->scale * kLog2e;
+  const bool some = p->b > 0 && p->lq > 0, keys = p->b > 0 && p->lk > 0;
+  BTR_REQUIRE((!some || p->q) && (!keys || (p->k && p->v)), "%s: null pointer", what);
+  return BTR_OK;
+}
+
+size_t fwd_bytes(const XaArgs &a) {
+  const Shares s = row_shares(a.b, a.lk, a.hk, a.rows);
+  if (s.n == 1) return 0;
+  const size_t n = (size_t)s.n * a.b * a.hk * a.rows;
+  return align256(n * a.d * 4) + align256(n * 8);
+}
+size_t bwd_bytes(const XaArgs &a) {   // D, then the shares of dq or of dk, dv
+  const size_t delta = align256((size_t)a.b * a.hk * a.rows * 4);
+  const Shares q = row_shares(a.b, a.lk, a.hk, a.rows), k = key_shares(a.b, a.lk, a.hk, a.rows);
+  size_t nq = 0, nk = 0;
+  if (q.n > 1) nq = align256((size_t)q.n * a.b * a.hk * a.rows * a.d * 4);
+  if (k.n > 1) nk = 2 * align256((size_t)k.n * a.b * a.lk * a.hk * a.d * 4);
+  return delta + std::max(nq, nk);
+}
+
+}  // namespace
+}  // namespace btr
+
+using namespace btr;
+
+extern "C" size_t btr_cross_attention_fwd_workspace_bytes(const btr_cross_attention_t *p) {
+  XaArgs a;
+  if (check("cross_attention", p, a) != BTR_OK) return 0;
+  return fwd_bytes(a);
+}
+
+extern "C" size_t btr_cross_attention_bwd_workspace_bytes(const btr_cross_attention_t *p) {
+  XaArgs a;
+  if (check("cross_attention", p, a) != BTR_OK) return 0;
+  return bwd_bytes(a);
+}
+
+extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out, float *lse,
+                                       void *workspace, size_t workspace_bytes,
+                                       btr_stream_t stream) {
+  XaArgs a;
+  const int rc = check("cross_attention_fwd", p, a);
+  if (rc != BTR_OK) return rc;
+  if (a.b == 0 || a.rows == 0) return BTR_OK;
+  BTR_REQUIRE(out, "cross_attention_fwd: null pointer");
+  const size_t need = fwd_bytes(a);
+  BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
+              "cross_attention_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  a.out = out;
+  a.lse = lse;
+  const Shares s = row_shares(a.b, a.lk, a.hk, a.rows);
+  a.tiles = s.tiles; a.nsplit = s.n; a.chunk = s.chunk;
+  const long long nrow = (long long)a.b * a.hk * a.rows;
+  if (s.n > 1) {
+    a.part = (float *)workspace;
+    a.part2 = (float *)((char *)workspace + align256((size_t)s.n * nrow * a.d * 4));
+  }
+  hipStream_t hs = as_stream(stream);
+  BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_fwd, a, hs));
+  if (s.n > 1)
+    BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_join_kernel<T>),
+                                                    dim3((unsigned)((nrow + 7) / 8)), dim3(256), 0,
+                                                    hs, a));
+  return check_launch("cross_attention_fwd");
+}
+
+extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const void *out,
+                                       const float *lse, const void *dout, void *dq, void *dk,
+                                       void *dv, void *workspace, size_t workspace_bytes,
+                                       btr_stream_t stream) {
+  XaArgs a;
+  const int rc = check("cross_attention_bwd", p, a);
+  if (rc != BTR_OK) return rc;
+  if (a.b == 0) return BTR_OK;
+  BTR_REQUIRE((a.rows == 0 || (out && lse && dout && dq)) && (a.lk == 0 || (dk && dv)),
+              "cross_attention_bwd: null pointer");
+  const size_t need = bwd_bytes(a);
+  BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
+              "cross_attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  a.out = const_cast<void *>(out);
+  a.lse = const_cast<float *>(lse);
+  a.dout = dout;
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  a.delta = (float *)workspace;
+  float *ws = (float *)((char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4));
+  hipStream_t hs = as_stream(stream);
+  if (a.rows > 0) {
+    const Shares s = row_shares(a.b, a.lk, a.hk, a.rows);
+    XaArgs q = a;
+    q.tiles = s.tiles; q.nsplit = s.n; q.chunk = s.chunk; q.part = ws;
+    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_q, q, hs));
+    if (s.n > 1) {
+      const long long n = (long long)a.b * a.hk * a.rows * a.d;
+      const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
+      BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_sum_kernel<T, true>),
+                                                      dim3(grid), dim3(256), 0, hs, q, n, (T *)dq,
+                                                      (T *)nullptr));
+    }
+  }
+  if (a.lk > 0) {
+    const Shares s = key_shares(a.b, a.lk, a.hk, a.rows);
+    XaArgs k = a;
+    const long long n = (long long)a.b * a.lk * a.hk * a.d;
+    k.tiles = s.tiles; k.nsplit = s.n; k.chunk = s.chunk; k.part = ws;
+    k.part2 = (float *)((char *)ws + align256((size_t)s.n * n * 4));
+    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_kv, k, hs));
+    if (s.n > 1) {
+      const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
+      BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_sum_kernel<T, false>),
+                                                      dim3(grid, 2), dim3(256), 0, hs, k, n,
+                                                      (T *)dk, (T *)dv));
+    }
+  }
+  return check_launch("cross_attention_bwd");
+}

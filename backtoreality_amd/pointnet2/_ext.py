@@ -131,6 +131,21 @@ _SIGNATURES = {
     "btr_attention_bwd": (_ci, [_ci] * 5 + [_vp, _ll, _ll, _vp, _vp, _ll, _ll, _vp, _vp, _vp, _vp,
                                             _vp, _ll, _ll, _vp, _vp, _ll, _ll, _cf, _cf,
                                             ctypes.c_ulonglong, _vp, _vp]),
+    # decoder operators for float32 / bfloat16 / float16 (groupfree/decoder_ops.py)
+    "btr_layer_norm_fwd": (_ci, [_ci, _ll, _ci, _vp, _ll, _vp, _ll, _vp, _vp, _cf, _vp, _vp, _vp]),
+    "btr_layer_norm_bwd_workspace_bytes": (_sz, [_ll, _ci]),
+    "btr_layer_norm_bwd": (_ci, [_ci, _ll, _ci, _vp, _ll, _vp, _ll, _vp, _ll] + [_vp] * 6 +
+                           [_sz, _vp]),
+    "btr_linear_fwd_workspace_bytes": (_sz, [_ci] * 3),
+    "btr_linear_fwd": (_ci, [_ci] * 4 + [_vp, _ll, _vp, _ll, _vp, _ci, _vp, _ll, _vp, _vp, _vp, _sz,
+                                         _vp]),
+    "btr_linear_bwd_workspace_bytes": (_sz, [_ci] * 4),
+    "btr_linear_bwd": (_ci, [_ci] * 4 + [_vp, _ll, _vp, _ll, _ci, _vp, _vp, _ll] + [_vp] * 4 +
+                       [_sz, _vp]),
+    "btr_cross_attention_fwd_workspace_bytes": (_sz, [_vp]),
+    "btr_cross_attention_fwd": (_ci, [_vp] * 4 + [_sz, _vp]),
+    "btr_cross_attention_bwd_workspace_bytes": (_sz, [_vp]),
+    "btr_cross_attention_bwd": (_ci, [_vp] * 8 + [_sz, _vp]),
     # whole-layer entry points (csrc/sa_layer.hip): description + plan by address
     "btr_sa_layer_plan": (_ci, [_vp, _vp]),
     "btr_sa_layer_ppfl": (_ci, [_vp, _vp]),
@@ -324,6 +339,15 @@ class DecoderPlan(ctypes.Structure):
         "bwd_scratch_bytes", "g_sa_in_w", "g_sa_in_b", "g_sa_out_w", "g_sa_out_b", "g_ca_in_w",
         "g_ca_in_b", "g_ca_out_w", "g_ca_out_b", "g_lin1_w", "g_lin1_b", "g_lin2_w",
         "g_lin2_b")] + [("g_ln", _sz3), ("grads_floats", _sz)]
+
+
+class CrossAttention(ctypes.Structure):
+    """btr_cross_attention_t: one cross-attention call (sizes, pointers, element strides)."""
+    _fields_ = [(n, _ci) for n in ("dtype", "b", "lq", "lk", "h", "hk", "d")] + \
+        [("q", _vp), ("k", _vp), ("v", _vp)] + \
+        [(n, _ll) for n in ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl",
+                            "v_sh")] + \
+        [("lengths", _vp), ("mask", _vp), ("mask_sb", _ll), ("scale", _cf)]
 
 
 GF_MAX_DECODER_LAYERS = 12   # BTR_GF_MAX_DECODER_LAYERS

@@ -1107,6 +1107,76 @@ int btr_grad_sumsq_multi(int chunks, int tensor0, const btr_adam_item_t *items,
 int btr_grad_norm_final(int chunks, const float *partial, float clip, float *out,
                         btr_stream_t stream);
 
+/* ---- decoder operators for float32, bfloat16 and float16 ----------------------------------------
+ * The three operators a transformer decoder layer is made of (reference:
+ * detection/GroupFree3D/models/transformer.py:36-76), each with its backward, for the calls the
+ * float32 whole-layer entry points above do not cover: 16-bit types, padded keys, key / value heads
+ * shared by several query heads, any width, odd strides.  Strides are in elements, the last axis is
+ * contiguous, rows may start at any element (16-byte alignment is not needed).  Workspaces are the
+ * caller's: nothing is kept between calls, nothing is allocated, every call may be captured. */
+#define BTR_F32 0
+#define BTR_BF16 1
+#define BTR_F16 2
+
+/* y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over each row of s = x [+ residual].
+ * weight / bias (width) in the type of x, each may be NULL (1 and 0); y (rows, width) contiguous;
+ * stats (rows, 2) receives mean and 1 / sqrt(var + eps) for the backward, or NULL. */
+int btr_layer_norm_fwd(int dtype, long long rows, int width, const void *x, long long ldx,
+                       const void *residual, long long ldr, const void *weight, const void *bias,
+                       float eps, void *y, float *stats, btr_stream_t stream);
+/* dx (rows, width) contiguous: the gradient of x and of residual alike; dweight / dbias (width), each
+ * may be NULL (zeros when rows == 0) */
+size_t btr_layer_norm_bwd_workspace_bytes(long long rows, int width);
+int btr_layer_norm_bwd(int dtype, long long rows, int width, const void *x, long long ldx,
+                       const void *residual, long long ldr, const void *dy, long long lddy,
+                       const void *weight, const float *stats, void *dx, void *dweight,
+                       void *dbias, void *workspace, size_t workspace_bytes, btr_stream_t stream);
+
+/* z = x weight^T + bias, y = act(z) [+ residual]: x (m, k), weight (n, k), bias (n) or NULL, residual
+ * (m, n) or NULL, y (m, n) contiguous.  act: BTR_ACT_*; GELU is the erf form.  z (m, n) contiguous
+ * in the type of x: what the backward of an activation needs, or NULL.  n, k >= 1. */
+#define BTR_ACT_NONE 0
+#define BTR_ACT_RELU 1
+#define BTR_ACT_GELU 2
+size_t btr_linear_fwd_workspace_bytes(int m, int n, int k);
+int btr_linear_fwd(int dtype, int m, int n, int k, const void *x, long long ldx, const void *weight,
+                   long long ldw, const void *bias, int act, const void *residual, long long ldr,
+                   void *y, void *z, void *workspace, size_t workspace_bytes, btr_stream_t stream);
+/* dx (m, k), dweight (n, k), dbias (n), contiguous, each may be NULL; the gradient of the residual
+ * is dy itself.  z as the forward left it (ReLU without a residual: y serves as well), unused and
+ * may be NULL without activation. */
+size_t btr_linear_bwd_workspace_bytes(int dtype, int m, int n, int k);
+int btr_linear_bwd(int dtype, int m, int n, int k, const void *x, long long ldx, const void *weight,
+                   long long ldw, int act, const void *z, const void *dy, long long lddy, void *dx,
+                   void *dweight, void *dbias, void *workspace, size_t workspace_bytes,
+                   btr_stream_t stream);
+
+/* out = softmax(scale q k^T) v per head, q (b, lq, h, d), k / v (b, lk, hk, d) with strides
+ * (batch, length, head); h % hk == 0, query head i reads key head i / (h / hk); d <= 128, scale > 0.
+ * Keys j >= lengths[b] (int32, or NULL: all lk; values outside [0, lk] are clamped) and keys with
+ * mask[b * mask_sb + j] != 0 (one byte each, or NULL) take no part, whatever their rows hold; a
+ * query without keys gets zeros.  out (b, lq, h, d) contiguous; lse: b * h * lq floats for the
+ * backward, in an order of its own, or NULL. */
+typedef struct {
+  int dtype, b, lq, lk, h, hk, d;
+  const void *q, *k, *v;
+  long long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
+  const int *lengths;
+  const unsigned char *mask;
+  long long mask_sb;
+  float scale;
+} btr_cross_attention_t;
+
+size_t btr_cross_attention_fwd_workspace_bytes(const btr_cross_attention_t *p);
+int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out, float *lse, void *workspace,
+                            size_t workspace_bytes, btr_stream_t stream);
+/* dout (b, lq, h, d) contiguous; dq / dk / dv contiguous, shaped like q / k / v, fully written
+ * (padding: zeros) */
+size_t btr_cross_attention_bwd_workspace_bytes(const btr_cross_attention_t *p);
+int btr_cross_attention_bwd(const btr_cross_attention_t *p, const void *out, const float *lse,
+                            const void *dout, void *dq, void *dk, void *dv, void *workspace,
+                            size_t workspace_bytes, btr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

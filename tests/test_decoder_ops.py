@@ -1,0 +1,91 @@
+"""Refusals of groupfree/decoder_ops.py and of its C entries: host checks, so no GPU is needed."""
+import ctypes
+
+import pytest
+import torch
+
+from backtoreality_amd.groupfree import decoder_ops as ops
+from backtoreality_amd.pointnet2 import _ext
+
+lib = _ext._lib
+PTR = 4096   # a non-null address for entries that refuse before they read anything
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="CPU not supported"):
+        ops.layer_norm(x)
+    with pytest.raises(RuntimeError, match="CPU not supported"):
+        ops.linear(x, torch.zeros(3, 8))
+    q = torch.zeros(1, 2, 2, 8)
+    with pytest.raises(RuntimeError, match="CPU not supported"):
+        ops.cross_attention(q, q, q)
+
+
+def _error():
+    return lib.btr_last_error().decode()
+
+
+def test_layer_norm_entry_refuses():
+    ok = dict(dtype=1, rows=4, width=8, x=PTR, ldx=8, r=None, ldr=0, y=PTR)
+
+    def fwd(**kw):
+        a = dict(ok, **kw)
+        return lib.btr_layer_norm_fwd(a["dtype"], a["rows"], a["width"], a["x"], a["ldx"], a["r"],
+                                      a["ldr"], None, None, 1e-5, a["y"], None, None)
+    for bad in (dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(width=0), dict(x=None),
+                dict(ldx=7), dict(r=PTR, ldr=7), dict(y=None)):
+        assert fwd(**bad) == -1 and "layer_norm_fwd" in _error(), bad
+    assert fwd(rows=0, x=None, y=None) == 0
+    assert lib.btr_layer_norm_bwd(0, 4, 8, PTR, 8, None, 0, PTR, 8, None, PTR, PTR, PTR, PTR, None, 0,
+                                  None) == -1 and "workspace" in _error()
+    assert lib.btr_layer_norm_bwd(0, 4, 8, PTR, 8, None, 0, PTR, 7, None, PTR, PTR, None, None, None,
+                                  0, None) == -1
+    assert lib.btr_layer_norm_bwd_workspace_bytes(0, 8) == 0
+
+
+def test_linear_entry_refuses():
+    def fwd(dtype=0, m=4, n=8, k=16, x=PTR, ldx=16, w=PTR, ldw=16, act=0, r=None, ldr=0, y=PTR):
+        return lib.btr_linear_fwd(dtype, m, n, k, x, ldx, w, ldw, None, act, r, ldr, y, None, None, 0,
+                                  None)
+    for bad in (dict(dtype=9), dict(m=-1), dict(n=0), dict(k=0), dict(x=None), dict(w=None),
+                dict(y=None), dict(ldx=15), dict(ldw=15), dict(r=PTR, ldr=7), dict(act=3)):
+        assert fwd(**bad) == -1 and "linear_fwd" in _error(), bad
+    assert fwd(m=1, n=64, k=100000, ldx=100000, ldw=100000) == -1 and "workspace" in _error()
+    assert fwd(m=0, x=None, w=None, y=None) == 0
+
+    def bwd(ldg=8, act=0, z=None, dy=PTR, ws=PTR, nbytes=1 << 20):
+        return lib.btr_linear_bwd(0, 4, 8, 16, PTR, 16, PTR, 16, act, z, dy, ldg, PTR, PTR, PTR, ws,
+                                  nbytes, None)
+    for bad in (dict(ldg=7), dict(act=2), dict(dy=None), dict(ws=None), dict(nbytes=16)):
+        assert bwd(**bad) == -1 and "linear_bwd" in _error(), bad
+
+
+def test_cross_attention_entry_refuses():
+    def desc(**kw):
+        p = _ext.CrossAttention(dtype=1, b=2, lq=3, lk=70, h=4, hk=2, d=64, q=PTR, k=PTR, v=PTR,
+                                scale=0.125)
+        for name, value in kw.items():
+            setattr(p, name, value)
+        return p
+
+    def fwd(p, out=PTR, ws=PTR, nbytes=1 << 30):
+        return lib.btr_cross_attention_fwd(ctypes.addressof(p), out, None, ws, nbytes, None)
+    for bad in (dict(dtype=7), dict(b=-1), dict(lq=-1), dict(lk=-1), dict(h=0), dict(hk=0), dict(hk=3),
+                dict(d=0), dict(d=129), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
+                dict(scale=float("nan")), dict(q=None), dict(k=None), dict(v=None), dict(lq=2 ** 30)):
+        p = desc(**bad)
+        assert fwd(p) == -1 and "cross_attention_fwd" in _error(), bad
+        assert lib.btr_cross_attention_bwd_workspace_bytes(ctypes.addressof(p)) == 0
+    assert lib.btr_cross_attention_fwd(None, PTR, None, PTR, 1 << 30, None) == -1
+    assert fwd(desc(), out=None) == -1
+    long = desc(lq=1, lk=100000)                         # split over the keys: needs a workspace
+    need = lib.btr_cross_attention_fwd_workspace_bytes(ctypes.addressof(long))
+    assert need > 0 and fwd(long, nbytes=need - 1) == -1 and "workspace" in _error()
+    assert fwd(long, ws=None, nbytes=need) == -1
+    assert fwd(desc(b=0, q=None, k=None, v=None), out=None) == 0
+    p = desc()
+    assert lib.btr_cross_attention_bwd(ctypes.addressof(p), PTR, PTR, PTR, PTR, None, PTR, PTR,
+                                       1 << 30, None) == -1
+    assert lib.btr_cross_attention_bwd(ctypes.addressof(p), PTR, PTR, PTR, PTR, PTR, PTR, PTR, 0,
+                                       None) == -1 and "workspace" in _error()
