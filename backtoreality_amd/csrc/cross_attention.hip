@@ -28,6 +28,7 @@
 // rounded to the input type where they enter the matrix instructions (relative error half an
 // ulp per term; P <= 1).  f32 runs on the f32 matrix instructions, nothing is rounded below 32 bits.
 #include <algorithm>
+#include <cstdint>
 
 #include "decoder_ops.hpp"
 
@@ -36,6 +37,7 @@
 namespace btr {
 namespace {
 
+constexpr int kMaxShares = 1024;    // of a row's keys
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct XaArgs {
@@ -55,6 +57,7 @@ struct XaArgs {
 };
 
 typedef __attribute__((address_space(3))) s16x4_t *lds_s16x4;
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------------------- tiles in LDS
 // Row-major [row][DP]; PITCH bytes a row.  16-bit: 64 mod 128 bytes and the 16-byte units of a row
@@ -252,9 +255,94 @@ __device__ __forceinline__ void store4(T *row, int c, int d, const float (&v)[4]
   }
 }
 
-// Sums of the waves that split the keys (WK > 1): wave w's acc[nt] times its factor f, added in
-// wave order; the result of row `row` (of 32) at out(row, column)
 constexpr int kMergePitch = 4;   // floats between rows beyond DP: rows land on different banks
+
+// writes row r from the transposed accumulators (lane: row, 4 consecutive columns a register quad):
+// the result and its log-sum-exp, or the share's unnormalised sums with (maximum in log2 units, sum)
+template <typename T, int DP>
+__device__ __forceinline__ void finish_row(const XaArgs &a, const Rows<T> &rows, int bh, int split,
+                                           int r, int hh, float m, float l,
+                                           const f32x16_t (&o)[DP / 32]) {
+  const float mb = m * a.scale_log2;             // (-inf stays -inf)
+  const bool share = a.nsplit > 1;
+  const long long row = ((long long)split * a.b * a.hk + bh) * a.rows + r;
+  const float inv = share ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // (NaN stays NaN)
+#pragma unroll
+  for (int nt = 0; nt < DP / 32; ++nt)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const float v4[4] = {o[nt][4 * gq] * inv, o[nt][4 * gq + 1] * inv, o[nt][4 * gq + 2] * inv,
+                           o[nt][4 * gq + 3] * inv};
+      const int c = 32 * nt + 8 * gq + 4 * hh;
+      if (share)
+        store4(a.part + row * a.d, c, a.d, v4);
+      else
+        store4((T *)a.out + rows.o(r), c, a.d, v4);
+    }
+  if (hh == 0) {
+    if (share) {
+      a.part2[2 * row] = mb;
+      a.part2[2 * row + 1] = l;
+    } else if (a.lse) {
+      a.lse[(long long)bh * a.rows + r] = l == 0.f ? INFINITY : mb + __builtin_amdgcn_logf(l);
+    }
+  }
+}
+
+// the same for 32 rows whose keys WK waves of the workgroup of 256 have shared: through LDS (om: WK
+// x 32 x (DP + 4) floats, the tiles' storage), added in wave order
+template <typename T, int DP, int WK>
+__device__ __forceinline__ void merge_rows(const XaArgs &a, const Rows<T> &rows, int bh, int split,
+                                           int tile, int wk, int tid, float m, float l,
+                                           const f32x16_t (&o)[DP / 32], float *om, float *mx,
+                                           float *sm) {
+  constexpr int LDO = DP + kMergePitch;
+  const int lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
+  __syncthreads();                               // every wave is done with the tiles
+#pragma unroll
+  for (int nt = 0; nt < DP / 32; ++nt)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq)
+      *reinterpret_cast<f32x4_t *>(om + (wk * 32 + l31) * LDO + 32 * nt + 8 * gq + 4 * hh) =
+          f32x4_t{o[nt][4 * gq], o[nt][4 * gq + 1], o[nt][4 * gq + 2], o[nt][4 * gq + 3]};
+  if (hh == 0) {
+    mx[wk * 32 + l31] = m * a.scale_log2;
+    sm[wk * 32 + l31] = l;
+  }
+  __syncthreads();
+  const int row = tid >> 3, sub = tid & 7, rr = tile * 32 + row;
+  if (rr >= a.rows) return;
+  const bool share = a.nsplit > 1;
+  const long long prow = ((long long)split * a.b * a.hk + bh) * a.rows + rr;
+  float M = -INFINITY, L = 0.f, f[WK];
+#pragma unroll
+  for (int k = 0; k < WK; ++k) M = fmaxf(M, mx[k * 32 + row]);
+#pragma unroll
+  for (int k = 0; k < WK; ++k) {
+    f[k] = mx[k * 32 + row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[k * 32 + row] - M);
+    L = fmaf(sm[k * 32 + row], f[k], L);
+  }
+  const float inv = share ? 1.f : L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  for (int c = 4 * sub; c < a.d; c += 32) {
+    f32x4_t t = {};
+#pragma unroll
+    for (int k = 0; k < WK; ++k)
+      t += *reinterpret_cast<const f32x4_t *>(om + (k * 32 + row) * LDO + c) * f[k];
+    const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
+    if (share)
+      store4(a.part + prow * a.d, c, a.d, v4);
+    else
+      store4((T *)a.out + rows.o(rr), c, a.d, v4);
+  }
+  if (sub == 0) {
+    if (share) {
+      a.part2[2 * prow] = M;
+      a.part2[2 * prow + 1] = L;
+    } else if (a.lse) {
+      a.lse[(long long)bh * a.rows + rr] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+    }
+  }
+}
 
 // -------------------------------------------------------------------------------- forward
 // WR waves along the rows (32 each) x WK along the keys, KT key subtiles of 32 per wave and tile.
@@ -354,120 +442,59 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
   }
   l += other_half(l);
 
-  float *po = nullptr, *pm = nullptr;
-  const long long prow = ((long long)split * a.b * a.hk + bh) * a.rows;   // + row
-  if (a.nsplit > 1) {
-    po = a.part;
-    pm = a.part2;
-  }
-  // (maximum in units of log2, sum) of the rows
   if constexpr (WK == 1) {
-    if (r >= a.rows) return;
-    const float mb = m * a.scale_log2;           // (-inf stays -inf)
-    if (po) {
-      float *dst = po + (prow + r) * a.d;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int gq = 0; gq < 4; ++gq) {
-          const float v4[4] = {o[nt][4 * gq], o[nt][4 * gq + 1], o[nt][4 * gq + 2],
-                               o[nt][4 * gq + 3]};
-          store4(dst, 32 * nt + 8 * gq + 4 * hh, a.d, v4);
-        }
-      if (hh == 0) {
-        pm[2 * (prow + r)] = mb;
-        pm[2 * (prow + r) + 1] = l;
-      }
-    } else {
-      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // (NaN stays NaN)
-      T *dst = (T *)a.out + rows.o(r);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int gq = 0; gq < 4; ++gq) {
-          const float v4[4] = {o[nt][4 * gq] * inv, o[nt][4 * gq + 1] * inv,
-                               o[nt][4 * gq + 2] * inv, o[nt][4 * gq + 3] * inv};
-          store4(dst, 32 * nt + 8 * gq + 4 * hh, a.d, v4);
-        }
-      if (hh == 0 && a.lse)
-        a.lse[(long long)bh * a.rows + r] = l == 0.f ? INFINITY : mb + __builtin_amdgcn_logf(l);
-    }
+    if (r < a.rows) finish_row<T, DP>(a, rows, bh, split, r, hh, m, l, o);
   } else {
-    constexpr int LDO = DP + kMergePitch;
-    float *om = reinterpret_cast<float *>(smem);
-    __syncthreads();                             // every wave is done with the tiles
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int gq = 0; gq < 4; ++gq)
-        *reinterpret_cast<f32x4_t *>(om + (wk * 32 + l31) * LDO + 32 * nt + 8 * gq + 4 * hh) =
-            f32x4_t{o[nt][4 * gq], o[nt][4 * gq + 1], o[nt][4 * gq + 2], o[nt][4 * gq + 3]};
-    if (hh == 0) {
-      mx[wk * 32 + l31] = m * a.scale_log2;
-      sm[wk * 32 + l31] = l;
-    }
-    __syncthreads();
-    const int row = tid >> 3, sub = tid & 7, rr = tile * 32 + row;
-    if (rr >= a.rows) return;
-    float M = -INFINITY, L = 0.f, f[WK];
-#pragma unroll
-    for (int k = 0; k < WK; ++k) M = fmaxf(M, mx[k * 32 + row]);
-#pragma unroll
-    for (int k = 0; k < WK; ++k) {
-      f[k] = mx[k * 32 + row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[k * 32 + row] - M);
-      L = fmaf(sm[k * 32 + row], f[k], L);
-    }
-    const float inv = po ? 1.f : L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
-    for (int c = 4 * sub; c < a.d; c += 32) {
-      f32x4_t t = {};
-#pragma unroll
-      for (int k = 0; k < WK; ++k)
-        t += *reinterpret_cast<const f32x4_t *>(om + (k * 32 + row) * LDO + c) * f[k];
-      const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
-      if (po)
-        store4(po + (prow + rr) * a.d, c, a.d, v4);
-      else
-        store4((T *)a.out + rows.o(rr), c, a.d, v4);
-    }
-    if (sub == 0) {
-      if (po) {
-        pm[2 * (prow + rr)] = M;
-        pm[2 * (prow + rr) + 1] = L;
-      } else if (a.lse) {
-        a.lse[(long long)bh * a.rows + rr] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
-      }
-    }
+    merge_rows<T, DP, WK>(a, rows, bh, split, tile, wk, tid, m, l, o, (float *)smem, mx, sm);
   }
 }
 
-// joins the shares: 32 threads a row, fixed order
+// Joins the shares of one row (a workgroup each): the weights once into LDS, then eight groups of 32
+// threads add every eighth share, and the groups' sums are added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void cross_attention_join_kernel(XaArgs a) {
-  const long long nrow = (long long)a.b * a.hk * a.rows;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= nrow) return;
+  __shared__ float wt[kMaxShares], red[8][128 + 4];
+  const long long nrow = (long long)a.b * a.hk * a.rows, row = blockIdx.x;
   const int bh = (int)(row / a.rows), r = (int)(row - (long long)bh * a.rows);
-  const int b = bh / a.hk, kh = bh - b * a.hk;
-  float M = -INFINITY, L = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, a.part2[2 * (s * nrow + row)]);
-  // a share's weight: without a finite score its sum itself, which is 0, or NaN if its scores were
-  auto weight = [&](int s) {
-    const float m = a.part2[2 * (s * nrow + row)];
-    return m == -INFINITY ? a.part2[2 * (s * nrow + row) + 1] : __builtin_amdgcn_exp2f(m - M);
-  };
-  for (int s = 0; s < a.nsplit; ++s)
-    L = fmaf(a.part2[2 * (s * nrow + row) + 1], weight(s), L);
-  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
-  const Rows<T> rows{a, b, kh};
-  T *dst = (T *)a.out + rows.o(r);
-  for (int c = threadIdx.x & 31; c < a.d; c += 32) {
-    float t = 0.f;
-    for (int s = 0; s < a.nsplit; ++s)
-      t = fmaf(a.part[(s * nrow + row) * a.d + c], weight(s), t);
-    dst[c] = (T)(t * inv);
+  const int tid = threadIdx.x, g = tid >> 5, c = 4 * (tid & 31);
+  float M = -INFINITY;
+  for (int s = tid; s < a.nsplit; s += 256) {
+    wt[s] = a.part2[2 * (s * nrow + row)];
+    M = fmaxf(M, wt[s]);
   }
-  if ((threadIdx.x & 31) == 0 && a.lse)
-    a.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+  for (int i = 32; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor(M, i));
+  if ((tid & 63) == 0) red[0][tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  // a share's weight: without a finite score its sum itself, which is 0, or NaN if its scores were
+  for (int s = tid; s < a.nsplit; s += 256) {
+    const float m = wt[s];
+    wt[s] = m == -INFINITY ? a.part2[2 * (s * nrow + row) + 1] : __builtin_amdgcn_exp2f(m - M);
+  }
+  __syncthreads();
+  f32x4_t t = {};
+  float L = 0.f;
+  for (int s = g; s < a.nsplit; s += 8) {
+    const f32x4_t p = load_row(a.part + (s * nrow + row) * a.d, c, a.d);
+    t += p * wt[s];
+    L = fmaf(a.part2[2 * (s * nrow + row) + 1], wt[s], L);
+  }
+  *reinterpret_cast<f32x4_t *>(&red[g][c]) = t;
+  if ((tid & 31) == 0) red[g][128] = L;
+  __syncthreads();
+  if (g) return;
+  L = 0.f;
+  t = f32x4_t{};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    t += *reinterpret_cast<const f32x4_t *>(&red[k][c]);
+    L += red[k][128];
+  }
+  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  const Rows<T> rows{a, bh / a.hk, bh % a.hk};
+  const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
+  store4((T *)a.out + rows.o(r), c, a.d, v4);
+  if (tid == 0 && a.lse) a.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
 // -------------------------------------------------------------------------------- backward, dq
@@ -712,6 +739,323 @@ __global__ __launch_bounds__(256) void cross_attention_sum_kernel(XaArgs a, long
   }
 }
 
+// =========================================================== 16-bit, aligned: tiles by LDS DMA
+// Heads of up to 64 or 128 columns, a multiple of 8, rows on 16-byte boundaries: the tiles go from
+// memory to LDS without passing through registers, a tile ahead of its use, which frees the 32
+// staging registers a lane (two waves per SIMD fit: 332 -> 1xx registers at D = 128) and the LDS
+// write instructions.  The DMA fills 64 consecutive 16-byte units per wave instruction, so rows
+// cannot be padded; instead lane -> unit is permuted: unit u of row r lies at u ^ swz(r), where the
+// 16 rows of a row read fall on 16 different units of the 64 banks and so do the four rows x 32
+// bytes of a transpose read.  Rows past the last key, masked keys and columns past d are loaded
+// from beyond the buffer's bound, which reads as zero.
+template <int D>
+struct Dma {
+  static constexpr int UNITS = D / 8, PITCH = D * 2;
+  static_assert(D == 64 || D == 128, "a row is a power of two of units");
+  __device__ static __forceinline__ int swz(int row) {
+    return D == 128 ? ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)
+                    : (row & 2) | ((row >> 2) & 1) | ((row >> 1) & 4);
+  }
+  // fragment j of tile row l31 (+ 32 per subtile as an immediate): base ^ (j << 5)
+  __device__ static __forceinline__ int row_base(int l31, int hh) {
+    return l31 * PITCH + ((hh ^ swz(l31)) << 4);
+  }
+  // transpose read of columns 32 nt .. + 31: base ^ (nt << 6); the eight rows further on: the
+  // swizzle's highest bit flips, + 8 rows
+  __device__ static __forceinline__ int tr_base(int lane) {
+    const int p = lane & 15, half = (lane >> 4) & 1, hh = lane >> 5, row = 4 * hh + (p >> 2);
+    return row * PITCH + (((2 * half + ((p & 3) >> 1)) ^ swz(row)) << 4) + (p & 1) * 8;
+  }
+  static constexpr int kTrHi = UNITS / 2 << 4;   // the bit that flips
+};
+
+// rows x columns of a (row stride sl) matrix that a DMA may touch; anything else reads as zero
+struct DmaSrc {
+  const char *base;
+  long long sl;                                  // bytes
+  int d;                                         // bytes
+};
+constexpr int kFar = 0x7ffffff0;                 // an offset beyond every bound
+
+// ROWS rows from row0 (those below `limit` and live) into `tile`, by THREADS threads
+template <int D, int ROWS, int THREADS>
+__device__ __forceinline__ void dma_tile(const DmaSrc &s, int row0, int limit,
+                                         const unsigned long long *live, char *tile, int tid) {
+  typedef Dma<D> DM;
+  constexpr int N = ROWS * DM::UNITS / THREADS;
+  static_assert(ROWS * DM::UNITS % THREADS == 0, "whole instructions");
+  const int n = min(ROWS, limit - row0);
+  // raw buffer descriptor: 48-bit base, bytes, 32-bit data
+  const unsigned long long at = (unsigned long long)(s.base + row0 * s.sl);
+  const int bytes = n > 0 ? (n - 1) * (int)s.sl + s.d : 0;
+  const i32x4_t rsrc = {__builtin_amdgcn_readfirstlane((int)at),
+                        __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
+                        __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+  const unsigned lds = (unsigned)(unsigned long long)(
+      __attribute__((address_space(3))) char *)tile + (tid & ~63) * 16;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * THREADS + tid, row = e / DM::UNITS, u = (e % DM::UNITS) ^ DM::swz(row);
+    int off = row * (int)s.sl + u * 16;
+    if (u * 16 >= s.d) off = kFar;
+    if (live && !((live[row >> 6] >> (row & 63)) & 1)) off = kFar;
+    // (in assembly: the compiler would wait for every DMA in flight before any transpose read; the
+    // kernels wait for a tile themselves, dma_wait, before the barrier in front of its first read)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds + i * THREADS * 16)), "v"(off), "s"(rsrc)
+                 : "memory");
+  }
+}
+// The DMA instructions are the compiler's to count only through this: what it has loaded itself must
+// have arrived before the first of them, or it waits for everything in flight at the first use.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// KT subtiles of 32 rows x the register operand.  The fragments are asked for in two batches ahead
+// of the products: read one by one just before its product, each would cost an LDS round trip.
+template <typename T, int D, int KT>
+__device__ __forceinline__ void dma_rows(const char *tile, int base, const typename Elem<T>::Vec *f,
+                                         f32x16_t (&acc)[KT]) {
+  constexpr int J = D / 16, HALF = J / 2;
+  typename Elem<T>::Vec x[J][KT];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int j = h * HALF; j < (h + 1) * HALF; ++j)
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+        x[j][t] = *reinterpret_cast<const typename Elem<T>::Vec *>(
+            tile + t * 32 * Dma<D>::PITCH + (base ^ (j << 5)));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int t = 0; t < KT; ++t) acc[t] = f32x16_t{};
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int t = 0; t < KT; ++t) acc[t] = mma<T>(x[j][t], f[j], acc[t]);
+}
+// acc[nt] += tile[32 rows]^T w: the next 16 rows' fragments are in flight during a step's products
+template <typename T, int D>
+struct DmaT {
+  static constexpr int NT = D / 32;
+  s16x4_t x[2][NT][2];
+  __device__ __forceinline__ void load(const char *tile, int base, int s) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      x[s & 1][nt][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4)(tile + (base ^ (nt << 6)) + 16 * s * Dma<D>::PITCH));
+      x[s & 1][nt][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(
+          tile + (base ^ (nt << 6) ^ Dma<D>::kTrHi) + (16 * s + 8) * Dma<D>::PITCH));
+    }
+  }
+  __device__ __forceinline__ void step(const f32x16_t &w, int s, f32x16_t *acc) {
+    typename Elem<T>::Vec bv;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bv[j] = (T)w[8 * (s & 1) + j];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      union {
+        s16x4_t s4[2];
+        typename Elem<T>::Vec v;
+      } u;
+      u.s4[0] = x[s & 1][nt][0];
+      u.s4[1] = x[s & 1][nt][1];
+      acc[nt] = mma<T>(u.v, bv, acc[nt]);
+    }
+  }
+};
+// ... over KT subtiles; the first step's fragments have been loaded
+template <typename T, int D, int KT>
+__device__ __forceinline__ void dma_t(DmaT<T, D> &v, const char *tile, int base,
+                                      const f32x16_t (&w)[KT], f32x16_t *acc) {
+#pragma unroll
+  for (int s = 0; s < 2 * KT; ++s) {
+    if (s + 1 < 2 * KT) {
+      v.load(tile, base, s + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    v.step(w[s >> 1], s, acc);
+  }
+}
+
+// online softmax of one tile of KT x 32 scores a lane holds: maximum, rescaling, exponentials, sum
+template <int KT, int NT>
+__device__ __forceinline__ void online(f32x16_t (&s)[KT], float &m, float &l, f32x16_t (&o)[NT],
+                                       float c) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) top = fmaxf(top, s[t][v]);
+  top = fmaxf(top, other_half(top));
+  if (__ballot(top > m)) {                       // some row's maximum moved
+    const float mn = fmaxf(m, top);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[nt][v] *= f;
+  }
+  const float base = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      s[t][v] = __builtin_amdgcn_exp2f(fmaf(s[t][v], c, -base));
+      l += s[t][v];
+    }
+}
+template <int KT>
+__device__ __forceinline__ void drop_dead(f32x16_t (&s)[KT], unsigned long long live, int hh) {
+  if (~live == 0 || (KT == 1 && (unsigned)live == 0xffffffffu)) return;
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    const unsigned bits = (unsigned)(live >> (32 * t)) >> (4 * hh);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[t][v] = bits & (1u << acc_row(v, 0)) ? s[t][v] : -INFINITY;
+  }
+}
+
+// forward: WR waves x 32 rows share tiles of 64 keys, double-buffered, one barrier a tile
+template <typename T, int D, int WR>
+__global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaArgs a) {
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int NT = D / 32, TB = 64 * Dma<D>::PITCH;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TB];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
+  int tile, bh, split;
+  place(a, tile, bh, split);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
+  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, a.d * 2};
+  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, a.d * 2};
+  const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const Rows<T> rows{a, b, kh};
+  const int r = (tile * WR + w) * 32 + l31;
+  Vec qf[D / 16];
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    qf[j] = Vec{};
+    if (r < a.rows && 16 * j + 8 * hh < a.d)
+      qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + 16 * j + 8 * hh);
+  }
+  f32x16_t o[NT] = {};
+  float m = -INFINITY, l = 0.f;
+  const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
+
+  Live<64> lv;
+  unsigned long long live[1] = {0}, next[1] = {0};
+  auto issue = [&](int k0, int buf) {
+    dma_tile<D, 64, 64 * WR>(ks, k0, kend, mask ? next : nullptr, smem + buf * 2 * TB, tid);
+    dma_tile<D, 64, 64 * WR>(vs, k0, kend, mask ? next : nullptr, smem + buf * 2 * TB + TB, tid);
+  };
+  lv.fetch(mask, kbeg, kend, lane);
+  loads_done();
+  if (kbeg < kend) {
+    lv.words(kbeg, kend, lane, next);
+    issue(kbeg, 0);
+    if (mask) lv.fetch(mask, kbeg + 64, kend, lane);
+  }
+  int buf = 0;
+  for (int k0 = kbeg; k0 < kend; k0 += 64) {
+    live[0] = next[0];
+    dma_wait();
+    lds_barrier();
+    if (k0 + 64 < kend) {
+      lv.words(k0 + 64, kend, lane, next);
+      issue(k0 + 64, buf ^ 1);
+      if (mask) lv.fetch(mask, k0 + 128, kend, lane);
+    }
+    const char *kt = smem + buf * 2 * TB, *vt = kt + TB;
+    buf ^= 1;
+    f32x16_t s[2];
+    dma_rows<T, D, 2>(kt, rb, qf, s);
+    drop_dead<2>(s, live[0], hh);
+    DmaT<T, D> v;
+    v.load(vt, tb, 0);
+    online<2, NT>(s, m, l, o, a.scale_log2);
+    dma_t<T, D, 2>(v, vt, tb, s, o);
+  }
+  l += other_half(l);
+  if (r < a.rows) finish_row<T, D>(a, rows, bh, split, r, hh, m, l, o);
+}
+
+// few rows (32): every wave streams its own tiles of 32 keys -- wave w those of index w, w + 4, ..
+// -- through its own double buffer, without a barrier until the four merge.  Bound by HBM: 64 KB a
+// CU in flight.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs a) {
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int NT = D / 32, TB = 32 * Dma<D>::PITCH, MERGE = 4 * 32 * (D + kMergePitch) * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[16 * TB > MERGE ? 16 * TB : MERGE];
+  __shared__ float mx[4 * 32], sm[4 * 32];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
+  int tile, bh, split;
+  place(a, tile, bh, split);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
+  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, a.d * 2};
+  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, a.d * 2};
+  const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const Rows<T> rows{a, b, kh};
+  const int r = tile * 32 + l31;
+  Vec qf[D / 16];
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    qf[j] = Vec{};
+    if (r < a.rows && 16 * j + 8 * hh < a.d)
+      qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + 16 * j + 8 * hh);
+  }
+  f32x16_t o[NT] = {};
+  float m = -INFINITY, l = 0.f;
+  const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
+  const int wave = __builtin_amdgcn_readfirstlane(w);
+  char *own = smem + wave * 4 * TB;
+
+  Live<32> lv;
+  unsigned long long live[1] = {0}, next[1] = {0};
+  auto issue = [&](int k0, int buf) {
+    dma_tile<D, 32, 64>(ks, k0, kend, mask ? next : nullptr, own + buf * 2 * TB, lane);
+    dma_tile<D, 32, 64>(vs, k0, kend, mask ? next : nullptr, own + buf * 2 * TB + TB, lane);
+  };
+  const int first = kbeg + 32 * wave;
+  lv.fetch(mask, first, min(kend, first + 32), lane);
+  loads_done();
+  if (first < kend) {
+    lv.words(first, min(kend, first + 32), lane, next);
+    issue(first, 0);
+    if (mask) lv.fetch(mask, first + 128, min(kend, first + 160), lane);
+  }
+  int buf = 0;
+  for (int k0 = first; k0 < kend; k0 += 128) {
+    live[0] = next[0];
+    if (k0 + 128 < kend) {
+      lv.words(k0 + 128, min(kend, k0 + 160), lane, next);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the reads of the buffer it refills
+      issue(k0 + 128, buf ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * 32 * Dma<D>::UNITS / 64) : "memory");
+      if (mask) lv.fetch(mask, k0 + 256, min(kend, k0 + 288), lane);
+    } else {
+      dma_wait();
+    }
+    const char *kt = own + buf * 2 * TB, *vt = kt + TB;
+    buf ^= 1;
+    f32x16_t s[1];
+    dma_rows<T, D, 1>(kt, rb, qf, s);
+    drop_dead<1>(s, live[0], hh);
+    DmaT<T, D> v;
+    v.load(vt, tb, 0);
+    online<1, NT>(s, m, l, o, a.scale_log2);
+    dma_t<T, D, 1>(v, vt, tb, s, o);
+  }
+  l += other_half(l);
+  merge_rows<T, D, 4>(a, rows, bh, split, tile, w, tid, m, l, o, (float *)smem, mx, sm);
+}
+
 // ------------------------------------------------------------------------------------ host
 constexpr int kFewRows = 32;     // one tile of rows: the waves split the keys instead
 
@@ -731,16 +1075,44 @@ Shares shares(int tiles, long long bh, int length, int step, int least) {
   return {tiles, std::max(1, cdiv(length, chunk)), chunk};
 }
 bool few(int rows) { return rows <= kFewRows; }
-Shares row_shares(int b, int lk, int hk, int rows) {   // forward, dq: over the keys
-  return shares(cdiv(rows, few(rows) ? 32 : 128), (long long)b * hk, lk, 128, 256);
+// rows of a workgroup of the DMA kernels: 256 where those still give every CU two workgroups (the
+// keys are read half as often), else 128
+int dma_rows_per(const XaArgs &a) {
+  return (long long)cdiv(a.rows, 256) * a.b * a.hk >= 512 ? 256 : 128;
+}
+Shares row_shares(const XaArgs &a, bool dma) {   // forward, dq: over the keys
+  return shares(cdiv(a.rows, few(a.rows) ? 32 : dma ? dma_rows_per(a) : 128), (long long)a.b * a.hk,
+                a.lk, 128, 256);
+}
+// Can tiles of K and V go through LDS DMA?  Whole 16-byte units on 16-byte boundaries, rows apart
+// by at least a row, a tile's offsets within 31 bits.
+bool dma_ok(const XaArgs &a, int dtype) {
+  auto ok = [&](const void *p, long long sb, long long sl, long long sh) {
+    return ((uintptr_t)p & 15) == 0 && ((sb | sl | sh) & 7) == 0 && sl >= a.d &&
+           sl <= (1 << 22);
+  };
+  return dtype != BTR_F32 && a.d % 8 == 0 && (a.d <= 64 || a.d > 96) &&
+         ok(a.k, a.k_sb, a.k_sl, a.k_sh) && ok(a.v, a.v_sb, a.v_sl, a.v_sh);
 }
 Shares key_shares(int b, int lk, int hk, int rows) {   // dk, dv: over the rows
   return shares(cdiv(lk, 128), (long long)b * hk, rows, 32, 128);
 }
 
 template <typename T, int DP>
-void launch_fwd(const XaArgs &a, hipStream_t hs) {
+void launch_fwd(const XaArgs &a, bool dma, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
+  if constexpr (sizeof(T) == 2 && DP != 96) {
+    constexpr int D = DP < 64 ? 64 : DP;
+    if (dma) {
+      if (few(a.rows))
+        hipLaunchKernelGGL((cross_attention_fwd_stream_kernel<T, D>), grid, dim3(256), 0, hs, a);
+      else if (dma_rows_per(a) == 256)
+        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, D, 8>), grid, dim3(512), 0, hs, a);
+      else
+        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, D, 4>), grid, dim3(256), 0, hs, a);
+      return;
+    }
+  }
   if (few(a.rows))
     hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 1, 4, 1, 1>), grid, dim3(256), 0, hs, a);
   else
@@ -802,15 +1174,15 @@ int check(const char *what, const btr_cross_attention_t *p, XaArgs &a) {
   return BTR_OK;
 }
 
-size_t fwd_bytes(const XaArgs &a) {
-  const Shares s = row_shares(a.b, a.lk, a.hk, a.rows);
+size_t fwd_bytes(const XaArgs &a, int dtype) {
+  const Shares s = row_shares(a, dma_ok(a, dtype));
   if (s.n == 1) return 0;
   const size_t n = (size_t)s.n * a.b * a.hk * a.rows;
   return align256(n * a.d * 4) + align256(n * 8);
 }
 size_t bwd_bytes(const XaArgs &a) {   // D, then the shares of dq or of dk, dv
   const size_t delta = align256((size_t)a.b * a.hk * a.rows * 4);
-  const Shares q = row_shares(a.b, a.lk, a.hk, a.rows), k = key_shares(a.b, a.lk, a.hk, a.rows);
+  const Shares q = row_shares(a, false), k = key_shares(a.b, a.lk, a.hk, a.rows);
   size_t nq = 0, nk = 0;
   if (q.n > 1) nq = align256((size_t)q.n * a.b * a.hk * a.rows * a.d * 4);
   if (k.n > 1) nk = 2 * align256((size_t)k.n * a.b * a.lk * a.hk * a.d * 4);
@@ -825,7 +1197,7 @@ using namespace btr;
 extern "C" size_t btr_cross_attention_fwd_workspace_bytes(const btr_cross_attention_t *p) {
   XaArgs a;
   if (check("cross_attention", p, a) != BTR_OK) return 0;
-  return fwd_bytes(a);
+  return fwd_bytes(a, p->dtype);
 }
 
 extern "C" size_t btr_cross_attention_bwd_workspace_bytes(const btr_cross_attention_t *p) {
@@ -842,12 +1214,13 @@ extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out
   if (rc != BTR_OK) return rc;
   if (a.b == 0 || a.rows == 0) return BTR_OK;
   BTR_REQUIRE(out, "cross_attention_fwd: null pointer");
-  const size_t need = fwd_bytes(a);
+  const size_t need = fwd_bytes(a, p->dtype);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "cross_attention_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.out = out;
   a.lse = lse;
-  const Shares s = row_shares(a.b, a.lk, a.hk, a.rows);
+  const bool dma = dma_ok(a, p->dtype);
+  const Shares s = row_shares(a, dma);
   a.tiles = s.tiles; a.nsplit = s.n; a.chunk = s.chunk;
   const long long nrow = (long long)a.b * a.hk * a.rows;
   if (s.n > 1) {
@@ -855,11 +1228,10 @@ extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out
     a.part2 = (float *)((char *)workspace + align256((size_t)s.n * nrow * a.d * 4));
   }
   hipStream_t hs = as_stream(stream);
-  BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_fwd, a, hs));
+  BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_fwd, a, dma, hs));
   if (s.n > 1)
     BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_join_kernel<T>),
-                                                    dim3((unsigned)((nrow + 7) / 8)), dim3(256), 0,
-                                                    hs, a));
+                                                    dim3((unsigned)nrow), dim3(256), 0, hs, a));
   return check_launch("cross_attention_fwd");
 }
 
@@ -884,7 +1256,7 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
   float *ws = (float *)((char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4));
   hipStream_t hs = as_stream(stream);
   if (a.rows > 0) {
-    const Shares s = row_shares(a.b, a.lk, a.hk, a.rows);
+    const Shares s = row_shares(a, false);
     XaArgs q = a;
     q.tiles = s.tiles; q.nsplit = s.n; q.chunk = s.chunk; q.part = ws;
     BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_q, q, hs));

@@ -45,10 +45,12 @@ __device__ __forceinline__ typename Elem<T>::Vec load_row(const T *row, int e0, 
   typename Elem<T>::Vec v = {};
   if (e0 + V <= n) {
     v = *reinterpret_cast<const typename Elem<T>::VecU *>(row + e0);
-  } else if (e0 < n) {
+  } else if (e0 < n) {   // (the row's last element in place of what is beyond: the loads fly together)
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e0 + j < n) v[j] = row[e0 + j];
+    for (int j = 0; j < V; ++j) {
+      const T t = row[min(e0 + j, n - 1)];
+      v[j] = e0 + j < n ? t : (T)0.f;
+    }
   }
   return v;
 }
