@@ -777,6 +777,33 @@ struct DmaSrc {
 };
 constexpr int kFar = 0x7ffffff0;                 // an offset beyond every bound
 
+__device__ __forceinline__ i32x4_t dma_rsrc(const char *base, int bytes) {
+  // raw buffer descriptor: 48-bit base, bytes, 32-bit data
+  const unsigned long long at = (unsigned long long)base;
+  return i32x4_t{__builtin_amdgcn_readfirstlane((int)at),
+                 __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
+                 __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+// 64 lanes x 16 (4) bytes at their offsets -> 64 consecutive units from lds (the same in all lanes).
+// In assembly: the compiler would wait for every DMA in flight before any transpose read; the
+// kernels wait for a tile themselves, dma_wait, before the barrier in front of its first read.
+__device__ __forceinline__ unsigned lds_at(const char *lds) {
+  return __builtin_amdgcn_readfirstlane(
+      (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)lds);
+}
+__device__ __forceinline__ void dma16(i32x4_t rsrc, int off, const char *lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_at(lds)), "v"(off), "s"(rsrc)
+               : "memory");
+}
+__device__ __forceinline__ void dma4(i32x4_t rsrc, int off, const char *lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds_at(lds)), "v"(off), "s"(rsrc)
+               : "memory");
+}
+
 // ROWS rows from row0 (those below `limit` and live) into `tile`, by THREADS threads
 template <int D, int ROWS, int THREADS>
 __device__ __forceinline__ void dma_tile(const DmaSrc &s, int row0, int limit,
@@ -785,26 +812,14 @@ __device__ __forceinline__ void dma_tile(const DmaSrc &s, int row0, int limit,
   constexpr int N = ROWS * DM::UNITS / THREADS;
   static_assert(ROWS * DM::UNITS % THREADS == 0, "whole instructions");
   const int n = min(ROWS, limit - row0);
-  // raw buffer descriptor: 48-bit base, bytes, 32-bit data
-  const unsigned long long at = (unsigned long long)(s.base + row0 * s.sl);
-  const int bytes = n > 0 ? (n - 1) * (int)s.sl + s.d : 0;
-  const i32x4_t rsrc = {__builtin_amdgcn_readfirstlane((int)at),
-                        __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
-                        __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
-  const unsigned lds = (unsigned)(unsigned long long)(
-      __attribute__((address_space(3))) char *)tile + (tid & ~63) * 16;
+  const i32x4_t rsrc = dma_rsrc(s.base + row0 * s.sl, n > 0 ? (n - 1) * (int)s.sl + s.d : 0);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int e = i * THREADS + tid, row = e / DM::UNITS, u = (e % DM::UNITS) ^ DM::swz(row);
     int off = row * (int)s.sl + u * 16;
     if (u * 16 >= s.d) off = kFar;
     if (live && !((live[row >> 6] >> (row & 63)) & 1)) off = kFar;
-    // (in assembly: the compiler would wait for every DMA in flight before any transpose read; the
-    // kernels wait for a tile themselves, dma_wait, before the barrier in front of its first read)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(__builtin_amdgcn_readfirstlane(lds + i * THREADS * 16)), "v"(off), "s"(rsrc)
-                 : "memory");
+    dma16(rsrc, off, tile + (i * THREADS + (tid & ~63)) * 16);
   }
 }
 // The DMA instructions are the compiler's to count only through this: what it has loaded itself must
@@ -1056,6 +1071,229 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
   merge_rows<T, D, 4>(a, rows, bh, split, tile, w, tid, m, l, o, (float *)smem, mx, sm);
 }
 
+// dq: WR waves x 32 rows share tiles of 64 keys as in the forward
+template <typename T, int D, int WR>
+__global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(XaArgs a) {
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int NT = D / 32, TB = 64 * Dma<D>::PITCH;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TB];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
+  int tile, bh, split;
+  place(a, tile, bh, split);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
+  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, a.d * 2};
+  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, a.d * 2};
+  const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const Rows<T> rows{a, b, kh};
+  const int r = (tile * WR + w) * 32 + l31;
+  Vec qf[D / 16], gf[D / 16];
+  float delta = 0.f, lse = INFINITY;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    qf[j] = gf[j] = Vec{};
+    if (r < a.rows && 16 * j + 8 * hh < a.d) {
+      const int c = 16 * j + 8 * hh;
+      qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + c);
+      gf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>((const T *)a.dout + rows.o(r) + c);
+      const Vec of =
+          *reinterpret_cast<const typename Elem<T>::VecU *>((const T *)a.out + rows.o(r) + c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta = fmaf((float)gf[j][i], (float)of[i], delta);
+    }
+  }
+  delta += other_half(delta);
+  if (r < a.rows) {
+    lse = a.lse[(long long)bh * a.rows + r];
+    if (split == 0 && hh == 0) a.delta[(long long)bh * a.rows + r] = delta;
+  }
+  f32x16_t dq[NT] = {};
+  const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
+
+  Live<64> lv;
+  unsigned long long live[1] = {0}, next[1] = {0};
+  auto issue = [&](int k0, int buf) {
+    dma_tile<D, 64, 64 * WR>(ks, k0, kend, mask ? next : nullptr, smem + buf * 2 * TB, tid);
+    dma_tile<D, 64, 64 * WR>(vs, k0, kend, mask ? next : nullptr, smem + buf * 2 * TB + TB, tid);
+  };
+  lv.fetch(mask, kbeg, kend, lane);
+  loads_done();
+  if (kbeg < kend) {
+    lv.words(kbeg, kend, lane, next);
+    issue(kbeg, 0);
+    if (mask) lv.fetch(mask, kbeg + 64, kend, lane);
+  }
+  int buf = 0;
+  for (int k0 = kbeg; k0 < kend; k0 += 64) {
+    live[0] = next[0];
+    dma_wait();
+    lds_barrier();
+    if (k0 + 64 < kend) {
+      lv.words(k0 + 64, kend, lane, next);
+      issue(k0 + 64, buf ^ 1);
+      if (mask) lv.fetch(mask, k0 + 128, kend, lane);
+    }
+    const char *kt = smem + buf * 2 * TB, *vt = kt + TB;
+    buf ^= 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const char *kt2 = kt + 32 * t * Dma<D>::PITCH;
+      f32x16_t s[1], dp[1];
+      dma_rows<T, D, 1>(kt2, rb, qf, s);
+      dma_rows<T, D, 1>(vt + 32 * t * Dma<D>::PITCH, rb, gf, dp);
+      DmaT<T, D> kx;
+      kx.load(kt2, tb, 0);
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        s[0][v] = __builtin_amdgcn_exp2f(fmaf(s[0][v], a.scale_log2, -lse)) * (dp[0][v] - delta);
+      const unsigned bits = (unsigned)(live[0] >> (32 * t));
+      if (bits != 0xffffffffu) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          s[0][v] = (bits >> (4 * hh)) & (1u << acc_row(v, 0)) ? s[0][v] : 0.f;
+      }
+      dma_t<T, D, 1>(kx, kt2, tb, s, dq);
+    }
+  }
+  if (r >= a.rows) return;
+  const long long prow = ((long long)split * a.b * a.hk + bh) * a.rows + r;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const float v4[4] = {dq[nt][4 * gq] * a.scale, dq[nt][4 * gq + 1] * a.scale,
+                           dq[nt][4 * gq + 2] * a.scale, dq[nt][4 * gq + 3] * a.scale};
+      const int c = 32 * nt + 8 * gq + 4 * hh;
+      if (a.nsplit > 1)
+        store4(a.part + prow * a.d, c, a.d, v4);
+      else
+        store4((T *)a.dq + rows.o(r), c, a.d, v4);
+    }
+}
+
+// dk, dv: WK waves x 32 keys, tiles of 64 rows.  A lane owns one key, its column of both results
+// depends on no other key: what a padded key's lane computes is dropped at the end, nothing is
+// selected on the way.  Rows past the end read as zeros (P = 1, but dout, dP - D and q are 0).
+// Needs 64 % g == 0: a lane's row of a tile is then the same head and offset in every tile.
+template <typename T, int D, int WK>
+__global__ __launch_bounds__(64 * WK, D == 64 ? 2 : 1) void cross_attention_bwd_kv_dma_kernel(XaArgs a) {
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int NT = D / 32, TB = 64 * Dma<D>::PITCH, THREADS = 64 * WK;
+  constexpr int N = 64 * Dma<D>::UNITS / THREADS;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TB];
+  __shared__ __attribute__((aligned(1024))) float stat[2][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
+  int tile, bh, split;
+  place(a, tile, bh, split);
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int nk = key_count(a, b);
+  const int rbeg = split * a.chunk;
+  int rend = min(a.rows, rbeg + a.chunk);
+  if (tile * 32 * WK >= nk) rend = rbeg;         // padding only: zeros
+  const int key = (tile * WK + w) * 32 + l31;
+  const bool live = key < nk && !(a.mask && a.mask[b * a.mask_sb + key]);
+  Vec kf[D / 16], vf[D / 16];
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    kf[j] = vf[j] = Vec{};
+    if (live && 16 * j + 8 * hh < a.d) {
+      const int c = 16 * j + 8 * hh;
+      kf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(
+          (const T *)a.k + b * a.k_sb + kh * a.k_sh + key * a.k_sl + c);
+      vf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(
+          (const T *)a.v + b * a.v_sb + kh * a.v_sh + key * a.v_sl + c);
+    }
+  }
+  f32x16_t dk[NT] = {}, dv[NT] = {};
+  const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
+
+  // this thread's units of a tile: row and byte offset from the tile's first query
+  int row[N], qo[N], go[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * THREADS + tid, u = (e % Dma<D>::UNITS) ^ Dma<D>::swz(e / Dma<D>::UNITS);
+    row[i] = e / Dma<D>::UNITS;
+    const int l = row[i] / a.g, hd = row[i] - l * a.g;
+    qo[i] = 2 * (l * (int)a.q_sl + hd * (int)a.q_sh + 8 * u);
+    go[i] = 2 * ((l * a.h + hd) * a.d + 8 * u);
+    if (8 * u >= a.d) row[i] = 1 << 30;          // a column past the head's width
+  }
+  const char *qb = (const char *)((const T *)a.q + b * a.q_sb + (long long)kh * a.g * a.q_sh);
+  const char *gb = (const char *)((const T *)a.dout + ((long long)b * a.lq * a.h + kh * a.g) * a.d);
+  auto issue = [&](int r0, int buf) {
+    char *qt = smem + buf * 2 * TB, *gt = qt + TB;
+    const int l0 = r0 / a.g;                     // (whole: 64 % g == 0)
+    const i32x4_t qr = dma_rsrc(qb + 2 * (l0 * a.q_sl), kFar);
+    const i32x4_t gr = dma_rsrc(gb + 2 * ((long long)l0 * a.h * a.d), kFar);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      dma16(qr, r0 + row[i] < rend ? qo[i] : kFar, qt + (i * THREADS + (tid & ~63)) * 16);
+      dma16(gr, r0 + row[i] < rend ? go[i] : kFar, gt + (i * THREADS + (tid & ~63)) * 16);
+    }
+    if (w < 2) {                                 // lse, D of the rows
+      const float *src = (w ? a.delta : a.lse) + (long long)bh * a.rows + r0;
+      dma4(dma_rsrc((const char *)src, (rend - r0) * 4), lane * 4, (char *)stat[buf][w ? 1 : 0]);
+    }
+  };
+  loads_done();
+  if (rbeg < rend) issue(rbeg, 0);
+  int buf = 0;
+  for (int r0 = rbeg; r0 < rend; r0 += 64) {
+    dma_wait();
+    lds_barrier();
+    if (r0 + 64 < rend) issue(r0 + 64, buf ^ 1);
+    const char *qt = smem + buf * 2 * TB, *gt = qt + TB;
+    const float *lse = stat[buf][0], *dl = stat[buf][1];
+    buf ^= 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const char *q2 = qt + 32 * t * Dma<D>::PITCH, *g2 = gt + 32 * t * Dma<D>::PITCH;
+      f32x16_t p[1], ds[1];
+      dma_rows<T, D, 1>(q2, rb, kf, p);
+      dma_rows<T, D, 1>(g2, rb, vf, ds);
+      DmaT<T, D> gx;
+      gx.load(g2, tb, 0);
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(lse + 32 * t + 8 * gq + 4 * hh);
+        const f32x4_t d4 = *reinterpret_cast<const f32x4_t *>(dl + 32 * t + 8 * gq + 4 * hh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int v = 4 * gq + i;
+          p[0][v] = __builtin_amdgcn_exp2f(fmaf(p[0][v], a.scale_log2, -l4[i]));
+          ds[0][v] = p[0][v] * (ds[0][v] - d4[i]);
+        }
+      }
+      dma_t<T, D, 1>(gx, g2, tb, p, dv);
+      DmaT<T, D> qx;
+      qx.load(q2, tb, 0);
+      dma_t<T, D, 1>(qx, q2, tb, ds, dk);
+    }
+  }
+  if (key >= a.lk) return;
+  const long long krow = (((long long)b * a.lk + key) * a.hk + kh) * a.d;
+  const long long ptotal = (long long)a.b * a.lk * a.hk * a.d;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const int c = 32 * nt + 8 * gq + 4 * hh;
+      float k4[4], v4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        k4[i] = live ? dk[nt][4 * gq + i] * a.scale : 0.f;
+        v4[i] = live ? dv[nt][4 * gq + i] : 0.f;
+      }
+      if (a.nsplit > 1) {
+        store4(a.part + split * ptotal + krow, c, a.d, k4);
+        store4(a.part2 + split * ptotal + krow, c, a.d, v4);
+      } else {
+        store4((T *)a.dk + krow, c, a.d, k4);
+        store4((T *)a.dv + krow, c, a.d, v4);
+      }
+    }
+}
+
 // ------------------------------------------------------------------------------------ host
 constexpr int kFewRows = 32;     // one tile of rows: the waves split the keys instead
 
@@ -1084,18 +1322,25 @@ Shares row_shares(const XaArgs &a, bool dma) {   // forward, dq: over the keys
   return shares(cdiv(a.rows, few(a.rows) ? 32 : dma ? dma_rows_per(a) : 128), (long long)a.b * a.hk,
                 a.lk, 128, 256);
 }
+bool aligned(const void *p, long long sb, long long sl, long long sh) {
+  return ((uintptr_t)p & 15) == 0 && ((sb | sl | sh) & 7) == 0 && sl <= (1 << 22);
+}
 // Can tiles of K and V go through LDS DMA?  Whole 16-byte units on 16-byte boundaries, rows apart
 // by at least a row, a tile's offsets within 31 bits.
 bool dma_ok(const XaArgs &a, int dtype) {
-  auto ok = [&](const void *p, long long sb, long long sl, long long sh) {
-    return ((uintptr_t)p & 15) == 0 && ((sb | sl | sh) & 7) == 0 && sl >= a.d &&
-           sl <= (1 << 22);
-  };
   return dtype != BTR_F32 && a.d % 8 == 0 && (a.d <= 64 || a.d > 96) &&
-         ok(a.k, a.k_sb, a.k_sl, a.k_sh) && ok(a.v, a.v_sb, a.v_sl, a.v_sh);
+         aligned(a.k, a.k_sb, a.k_sl, a.k_sh) && aligned(a.v, a.v_sb, a.v_sl, a.v_sh) &&
+         a.k_sl >= a.d && a.v_sl >= a.d;
 }
-Shares key_shares(int b, int lk, int hk, int rows) {   // dk, dv: over the rows
-  return shares(cdiv(lk, 128), (long long)b * hk, rows, 32, 128);
+// ... and tiles of query and dout rows?  The same of theirs, offsets within a tile of 64 rows below
+// 2^31, and groups that divide a tile.
+bool dma_rows_ok(const XaArgs &a, int dtype, const void *dout) {
+  return dtype != BTR_F32 && a.d % 8 == 0 && (a.d <= 64 || a.d > 96) && 64 % a.g == 0 &&
+         aligned(a.q, a.q_sb, a.q_sl, a.q_sh) && a.q_sl >= 0 && a.q_sh >= 0 &&
+         a.q_sh <= (1 << 22) && ((uintptr_t)dout & 15) == 0 && (long long)a.h * a.d <= (1 << 22);
+}
+Shares key_shares(const XaArgs &a) {                  // dk, dv: over the rows
+  return shares(cdiv(a.lk, 128), (long long)a.b * a.hk, a.rows, 64, 128);
 }
 
 template <typename T, int DP>
@@ -1119,16 +1364,33 @@ void launch_fwd(const XaArgs &a, bool dma, hipStream_t hs) {
     hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 4, 1, 2, 1>), grid, dim3(256), 0, hs, a);
 }
 template <typename T, int DP>
-void launch_bwd_q(const XaArgs &a, hipStream_t hs) {
+void launch_bwd_q(const XaArgs &a, bool dma, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
+  if constexpr (sizeof(T) == 2 && DP != 96) {
+    constexpr int D = DP < 64 ? 64 : DP;
+    if (dma && !few(a.rows)) {
+      if (dma_rows_per(a) == 256)
+        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, D, 8>), grid, dim3(512), 0, hs, a);
+      else
+        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, D, 4>), grid, dim3(256), 0, hs, a);
+      return;
+    }
+  }
   if (few(a.rows))
     hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 1, 4, 1>), grid, dim3(256), 0, hs, a);
   else
     hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 4, 1, 2>), grid, dim3(256), 0, hs, a);
 }
 template <typename T, int DP>
-void launch_bwd_kv(const XaArgs &a, hipStream_t hs) {
+void launch_bwd_kv(const XaArgs &a, bool dma, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
+  if constexpr (sizeof(T) == 2 && DP != 96) {
+    if (dma) {
+      hipLaunchKernelGGL((cross_attention_bwd_kv_dma_kernel<T, DP < 64 ? 64 : DP, 4>), grid,
+                         dim3(256), 0, hs, a);
+      return;
+    }
+  }
   hipLaunchKernelGGL((cross_attention_bwd_kv_kernel<T, DP>), grid, dim3(256), 0, hs, a);
 }
 
@@ -1180,9 +1442,9 @@ size_t fwd_bytes(const XaArgs &a, int dtype) {
   const size_t n = (size_t)s.n * a.b * a.hk * a.rows;
   return align256(n * a.d * 4) + align256(n * 8);
 }
-size_t bwd_bytes(const XaArgs &a) {   // D, then the shares of dq or of dk, dv
+size_t bwd_bytes(const XaArgs &a, int dtype) {   // D, then the shares of dq or of dk, dv
   const size_t delta = align256((size_t)a.b * a.hk * a.rows * 4);
-  const Shares q = row_shares(a, false), k = key_shares(a.b, a.lk, a.hk, a.rows);
+  const Shares q = row_shares(a, dma_ok(a, dtype)), k = key_shares(a);
   size_t nq = 0, nk = 0;
   if (q.n > 1) nq = align256((size_t)q.n * a.b * a.hk * a.rows * a.d * 4);
   if (k.n > 1) nk = 2 * align256((size_t)k.n * a.b * a.lk * a.hk * a.d * 4);
@@ -1203,7 +1465,7 @@ extern "C" size_t btr_cross_attention_fwd_workspace_bytes(const btr_cross_attent
 extern "C" size_t btr_cross_attention_bwd_workspace_bytes(const btr_cross_attention_t *p) {
   XaArgs a;
   if (check("cross_attention", p, a) != BTR_OK) return 0;
-  return bwd_bytes(a);
+  return bwd_bytes(a, p->dtype);
 }
 
 extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out, float *lse,
@@ -1245,7 +1507,7 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
   if (a.b == 0) return BTR_OK;
   BTR_REQUIRE((a.rows == 0 || (out && lse && dout && dq)) && (a.lk == 0 || (dk && dv)),
               "cross_attention_bwd: null pointer");
-  const size_t need = bwd_bytes(a);
+  const size_t need = bwd_bytes(a, p->dtype);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "cross_attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.out = const_cast<void *>(out);
@@ -1256,10 +1518,11 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
   float *ws = (float *)((char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4));
   hipStream_t hs = as_stream(stream);
   if (a.rows > 0) {
-    const Shares s = row_shares(a, false);
+    const bool dma = dma_ok(a, p->dtype);
+    const Shares s = row_shares(a, dma);
     XaArgs q = a;
     q.tiles = s.tiles; q.nsplit = s.n; q.chunk = s.chunk; q.part = ws;
-    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_q, q, hs));
+    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_q, q, dma, hs));
     if (s.n > 1) {
       const long long n = (long long)a.b * a.hk * a.rows * a.d;
       const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
@@ -1269,12 +1532,12 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
     }
   }
   if (a.lk > 0) {
-    const Shares s = key_shares(a.b, a.lk, a.hk, a.rows);
+    const Shares s = key_shares(a);
     XaArgs k = a;
     const long long n = (long long)a.b * a.lk * a.hk * a.d;
     k.tiles = s.tiles; k.nsplit = s.n; k.chunk = s.chunk; k.part = ws;
     k.part2 = (float *)((char *)ws + align256((size_t)s.n * n * 4));
-    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_kv, k, hs));
+    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_kv, k, dma_rows_ok(a, p->dtype, dout), hs));
     if (s.n > 1) {
       const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
       BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_sum_kernel<T, false>),
