@@ -31,6 +31,7 @@
 #include <cstdint>
 
 #include "decoder_ops.hpp"
+#include "lds_dma.hpp"
 
 #pragma clang fp contract(fast)
 
@@ -55,9 +56,6 @@ struct XaArgs {
   int tiles, nsplit, chunk;                      // workgroup tiles, shares of the long axis, its length
   float *part, *part2;                           // partial results of the shares
 };
-
-typedef __attribute__((address_space(3))) s16x4_t *lds_s16x4;
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------------------- tiles in LDS
 // Row-major [row][DP]; PITCH bytes a row.  16-bit: 64 mod 128 bytes and the 16-byte units of a row
@@ -741,68 +739,16 @@ __global__ __launch_bounds__(256) void cross_attention_sum_kernel(XaArgs a, long
 
 // =========================================================== 16-bit, aligned: tiles by LDS DMA
 // Heads of up to 64 or 128 columns, a multiple of 8, rows on 16-byte boundaries: the tiles go from
-// memory to LDS without passing through registers, a tile ahead of its use, which frees the 32
-// staging registers a lane (two waves per SIMD fit: 332 -> 1xx registers at D = 128) and the LDS
-// write instructions.  The DMA fills 64 consecutive 16-byte units per wave instruction, so rows
-// cannot be padded; instead lane -> unit is permuted: unit u of row r lies at u ^ swz(r), where the
-// 16 rows of a row read fall on 16 different units of the 64 banks and so do the four rows x 32
-// bytes of a transpose read.  Rows past the last key, masked keys and columns past d are loaded
-// from beyond the buffer's bound, which reads as zero.
-template <int D>
-struct Dma {
-  static constexpr int UNITS = D / 8, PITCH = D * 2;
-  static_assert(D == 64 || D == 128, "a row is a power of two of units");
-  __device__ static __forceinline__ int swz(int row) {
-    return D == 128 ? ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)
-                    : (row & 2) | ((row >> 2) & 1) | ((row >> 1) & 4);
-  }
-  // fragment j of tile row l31 (+ 32 per subtile as an immediate): base ^ (j << 5)
-  __device__ static __forceinline__ int row_base(int l31, int hh) {
-    return l31 * PITCH + ((hh ^ swz(l31)) << 4);
-  }
-  // transpose read of columns 32 nt .. + 31: base ^ (nt << 6); the eight rows further on: the
-  // swizzle's highest bit flips, + 8 rows
-  __device__ static __forceinline__ int tr_base(int lane) {
-    const int p = lane & 15, half = (lane >> 4) & 1, hh = lane >> 5, row = 4 * hh + (p >> 2);
-    return row * PITCH + (((2 * half + ((p & 3) >> 1)) ^ swz(row)) << 4) + (p & 1) * 8;
-  }
-  static constexpr int kTrHi = UNITS / 2 << 4;   // the bit that flips
-};
-
+// memory to LDS by DMA (lds_dma.hpp), a tile ahead of their use, which frees the 32 staging
+// registers a lane (two waves per SIMD fit: 332 -> 218 registers at D = 128) and the LDS write
+// instructions.  Rows past the last key, masked keys and columns past d are loaded from beyond the
+// buffer's bound, which reads as zero.
 // rows x columns of a (row stride sl) matrix that a DMA may touch; anything else reads as zero
 struct DmaSrc {
   const char *base;
   long long sl;                                  // bytes
   int d;                                         // bytes
 };
-constexpr int kFar = 0x7ffffff0;                 // an offset beyond every bound
-
-__device__ __forceinline__ i32x4_t dma_rsrc(const char *base, int bytes) {
-  // raw buffer descriptor: 48-bit base, bytes, 32-bit data
-  const unsigned long long at = (unsigned long long)base;
-  return i32x4_t{__builtin_amdgcn_readfirstlane((int)at),
-                 __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
-                 __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
-}
-// 64 lanes x 16 (4) bytes at their offsets -> 64 consecutive units from lds (the same in all lanes).
-// In assembly: the compiler would wait for every DMA in flight before any transpose read; the
-// kernels wait for a tile themselves, dma_wait, before the barrier in front of its first read.
-__device__ __forceinline__ unsigned lds_at(const char *lds) {
-  return __builtin_amdgcn_readfirstlane(
-      (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)lds);
-}
-__device__ __forceinline__ void dma16(i32x4_t rsrc, int off, const char *lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(lds_at(lds)), "v"(off), "s"(rsrc)
-               : "memory");
-}
-__device__ __forceinline__ void dma4(i32x4_t rsrc, int off, const char *lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :
-               : "s"(lds_at(lds)), "v"(off), "s"(rsrc)
-               : "memory");
-}
 
 // ROWS rows from row0 (those below `limit` and live) into `tile`, by THREADS threads
 template <int D, int ROWS, int THREADS>
@@ -822,11 +768,6 @@ __device__ __forceinline__ void dma_tile(const DmaSrc &s, int row0, int limit,
     dma16(rsrc, off, tile + (i * THREADS + (tid & ~63)) * 16);
   }
 }
-// The DMA instructions are the compiler's to count only through this: what it has loaded itself must
-// have arrived before the first of them, or it waits for everything in flight at the first use.
-__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // KT subtiles of 32 rows x the register operand.  The fragments are asked for in two batches ahead
 // of the products: read one by one just before its product, each would cost an LDS round trip.
 template <typename T, int D, int KT>

@@ -7,20 +7,26 @@
 // (reference: linear1 / linear2 and the projections of detection/GroupFree3D/models/
 // transformer.py:36-76; csrc/sa_mlp.hip has the float32 GEMMs with BatchNorm around them.)
 //
-// One tile kernel serves the three products; what differs is whether the reduction runs along a
-// row of the operand (x, W forward, dz for dx) or across its rows (W for dx; dz and x for dW).  Both
-// are staged the way memory has them, 16 bytes a lane along the rows; the second kind is read out
-// of LDS with gfx950's transpose read, so nothing is ever transposed in memory.
+// The three products differ in whether the reduction runs along a row of the operand (x, W forward,
+// dz for dx) or across its rows (W for dx; dz and x for dW).  Both kinds are staged the way memory
+// has them and the second is read out of LDS with gfx950's transpose read, so nothing is ever
+// transposed in memory.  16-bit operands go to LDS by DMA (linear_dma_kernel); rows that do not lie
+// on 16-byte boundaries in whole 16-byte units are first copied to rows that do, in the workspace.
+// f32 operands pass through registers, where they are split (linear_gemm_kernel).  Few rows
+// (single tokens) read W once, straight into the matrix instructions (linear_rows_kernel).
 //
 // Numbers: every product accumulates in f32 and the epilogue works on the f32 sums; y is rounded
 // once.  f32 operands are split into three bf16 terms (8 + 8 + 8 bits: exact up to the 24th) and
 // multiplied as the six products above 2^-24, which the bf16 matrix pipe does 2.7 times faster
-// than the f32 instructions do one; an infinite f32 element makes the sums it enters NaN.  z is kept
-// for the backward in the type of x (act' sees z with half an ulp of error), dz likewise is rounded
-// to the type of x before the two products that read it.
+// than the f32 instructions do one; an infinite f32 element makes the sums it enters NaN.  What the
+// backward needs of the activation is its slope act'(z), taken from the f32 sum in the forward's
+// epilogue and kept in the type of x (half an ulp; 0 and 1 of ReLU are exact); dz is rounded to the
+// type of x as well before the two products that read it.
 #include <algorithm>
+#include <cstdint>
 
 #include "decoder_ops.hpp"
+#include "lds_dma.hpp"
 
 #pragma clang fp contract(fast)
 
@@ -37,26 +43,22 @@ struct GemmArgs {
   const void *bias, *res;
   long long ldres;
   int act;
-  void *c, *z;               // contiguous (m, n); z: the sums before the activation, or NULL
+  void *c, *slope;           // contiguous (m, n); slope: act' of the sums, or NULL
   float *part;               // split reduction: (nsplit, m, n) partial sums
   int nsplit, chunk;         // shares of k, their length
   int mt, nt;                // tiles
 };
 
-typedef __attribute__((address_space(3))) s16x4_t *lds_s16x4;
-
 // what the matrix instructions eat: T itself, or three bf16 planes of f32
 template <typename T>
 struct Op {
-  static constexpr int P = 1, V = 8;
+  static constexpr int P = 1;
   typedef typename Elem<T>::Vec Frag;
-  typedef T E;
 };
 template <>
 struct Op<float> {
-  static constexpr int P = 3, V = 4;
+  static constexpr int P = 3;
   typedef bf16x8_t Frag;
-  typedef __bf16 E;
 };
 
 __device__ __forceinline__ f32x16_t mfma(bf16x8_t a, bf16x8_t b, f32x16_t c) {
@@ -80,12 +82,30 @@ __device__ __forceinline__ void split3(f32x4_t f, bf16x4_t (&p)[3]) {
   }
 }
 
-// R rows of the operand (its m or n axis) x BK of the reduction, in LDS.  TR false: [R][BK], read
+__device__ __forceinline__ f32x4_t mfma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mfma16(f16x8_t a, f16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// eight consecutive elements -> fragments
+template <typename V>
+__device__ __forceinline__ void pack(const V (&v)[1], V (&f)[1]) { f[0] = v[0]; }
+__device__ __forceinline__ void pack(const f32x4_t (&v)[2], bf16x8_t (&f)[3]) {
+  bf16x4_t a[3], b[3];
+  split3(v[0], a);
+  split3(v[1], b);
+#pragma unroll
+  for (int p = 0; p < 3; ++p)
+    f[p] = __builtin_shufflevector(a[p], b[p], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// f32: R rows of the operand (its m or n axis) x BK of the reduction, in LDS as three bf16 planes.  TR false: [R][BK], read
 // as rows; true: [BK][R], read transposed.  Row pitches: an odd number of 16-byte units (sixteen
 // rows at one column: distinct banks) / 64 mod 256 bytes (four rows x 64 bytes: distinct banks).
-template <typename T, bool TR, int R, int BK>
+template <bool TR, int R, int BK>
 struct Panel {
-  static constexpr int P = Op<T>::P, V = Op<T>::V;
+  static constexpr int P = 3, V = 4;
   static constexpr int ROWS = TR ? BK : R, COLS = TR ? R : BK;
   static constexpr int PITCH = TR ? (R * 2 / 256) * 256 + (R * 2 % 256 <= 64 ? 64 : R * 2 % 256 <= 192 ? 192 : 320)
                                   : COLS * 2 + 16;
@@ -93,17 +113,17 @@ struct Panel {
   static constexpr int PER_ROW = COLS / V, N = ROWS * PER_ROW / 256;
   static_assert(ROWS * PER_ROW % 256 == 0, "whole vectors per thread");
   static_assert(!TR || (PITCH >= R * 2 && (PITCH % 256 == 64 || PITCH % 256 == 192)), "pitch");
-  typename Elem<T>::Vec r[N];
+  f32x4_t r[N];
 
   // r0: first index of the operand's m / n axis, k0: of the reduction; beyond rmax / kmax zeros
-  __device__ __forceinline__ void fetch(const T *src, long long ld, int r0, int rmax, int k0,
+  __device__ __forceinline__ void fetch(const float *src, long long ld, int r0, int rmax, int k0,
                                         int kmax, int tid) {
     const int row0 = TR ? k0 : r0, col0 = TR ? r0 : k0, rows = TR ? kmax : rmax,
               cols = TR ? rmax : kmax;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + 256 * i, row = row0 + e / PER_ROW, col = col0 + (e % PER_ROW) * V;
-      r[i] = typename Elem<T>::Vec{};
+      r[i] = f32x4_t{};
       if (row < rows && col < cols) r[i] = load_row(src + row * ld, col, cols);
     }
   }
@@ -112,22 +132,18 @@ struct Panel {
     for (int i = 0; i < N; ++i) {
       const int e = tid + 256 * i;
       char *p = lds + (e / PER_ROW) * PITCH + (e % PER_ROW) * V * 2;
-      if constexpr (P == 1) {
-        *reinterpret_cast<typename Elem<T>::Vec *>(p) = r[i];
-      } else {
-        bf16x4_t q[3];
-        split3(r[i], q);
+      bf16x4_t q[3];
+      split3(r[i], q);
 #pragma unroll
-        for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x4_t *>(p + j * PLANE) = q[j];
-      }
+      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x4_t *>(p + j * PLANE) = q[j];
     }
   }
   // fragment of the 32 rows at r0 and the 16 reduction steps at ks
-  __device__ static __forceinline__ typename Op<T>::Frag frag(const char *lds, int plane, int r0,
+  __device__ static __forceinline__ bf16x8_t frag(const char *lds, int plane, int r0,
                                                               int ks, int lane) {
     const char *t = lds + plane * PLANE;
     if constexpr (!TR) {
-      return *reinterpret_cast<const typename Op<T>::Frag *>(
+      return *reinterpret_cast<const bf16x8_t *>(
           t + (r0 + (lane & 31)) * PITCH + (ks + 8 * (lane >> 5)) * 2);
     } else {
       // lane p of a group of 16 addresses row p / 4, columns 4 (p % 4) .. + 3 of a [4][16] block and
@@ -137,7 +153,7 @@ struct Panel {
                       (r0 + 16 * ((lane >> 4) & 1) + 4 * (p & 3)) * 2;
       union {
         s16x4_t s[2];
-        typename Op<T>::Frag f;
+        bf16x8_t f;
       } u;
       u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q);
       u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 4 * PITCH));
@@ -146,21 +162,47 @@ struct Panel {
   }
 };
 
-__device__ __forceinline__ float gelu_cdf(float z) {   // Phi(z); the tail without cancellation
-  return 0.5f * erfcf(-z * 0.70710678118654752f);
+// Phi(z) and the density phi(z) of the normal distribution.  erfcx(x) = e^(x^2) erfc(x) is smooth:
+// t P(t) with t = 1 / (1 + 0.3 x) and a P of degree 8, fitted here by reweighted least squares
+// (Lawson) on x in [0, 14], is good to 4e-8 relative, and Phi(-|z|) = e^(-z^2 / 2) erfcx(|z| / sqrt
+// 2) / 2 keeps that in the tail, where 1 + erf would cancel.  The exponential is shared with phi;
+// its argument's rounding errors (up to 1e-5 of the result far out) are added back to first order.
+__device__ __forceinline__ void normal(float z, float &cdf, float &pdf) {
+  const float q = z * z, qe = fmaf(z, z, -q);
+  const float a = q * -0.72134752044448170f, ae = fmaf(q, -0.72134752044448170f, -a);
+  float e = __builtin_amdgcn_exp2f(a);
+  e = fmaf(e, fmaf(ae, 0.69314718055994531f, qe * -0.5f), e);
+  if (!(q < 200.f)) e = q >= 200.f ? 0.f : q;    // (e is 0 from there on; NaN stays)
+  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, x, 1.f));
+  float p = -0.12661709327829032f;
+  p = fmaf(p, t, 0.4718284843770408f);
+  p = fmaf(p, t, -0.4846959475126719f);
+  p = fmaf(p, t, 0.5170530040780374f);
+  p = fmaf(p, t, -0.07405165572695369f);
+  p = fmaf(p, t, 0.20638609117498913f);
+  p = fmaf(p, t, 0.15046865829841485f);
+  p = fmaf(p, t, 0.1704237449651274f);
+  p = fmaf(p, t, 0.16920475194603254f);
+  const float half = 0.5f * e * (p * t);
+  cdf = z < 0.f ? half : 1.f - half;
+  pdf = e * 0.39894228040143268f;
 }
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == kActRelu) return z > 0.f ? z : z != z ? z : 0.f;
-  if (act == kActGelu) return z == -INFINITY ? 0.f : z * gelu_cdf(z);
-  return z;
-}
-__device__ __forceinline__ float activate_grad(float z, int act) {
-  if (act == kActRelu) return z > 0.f ? 1.f : 0.f;
-  if (act == kActGelu) {
-    if (__builtin_fabsf(z) > 30.f) return z > 0.f ? 1.f : 0.f;   // (beyond f32's smallest density)
-    return gelu_cdf(z) + z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+// act(z), and act'(z) into slope
+__device__ __forceinline__ float activate(float z, int act, float &slope) {
+  slope = 1.f;
+  if (act == kActRelu) {
+    slope = z > 0.f ? 1.f : 0.f;
+    return z > 0.f ? z : z != z ? z : 0.f;
   }
-  return 1.f;
+  if (act == kActGelu) {
+    float cdf, pdf;
+    normal(z, cdf, pdf);
+    const bool inf = __builtin_fabsf(z) == INFINITY;               // (inf * 0)
+    slope = inf ? cdf : fmaf(z, pdf, cdf);
+    return inf ? fmaxf(z, 0.f) : z * cdf;
+  }
+  return z;
 }
 
 // V consecutive columns of one row: bias, activation, residual, one rounding
@@ -168,86 +210,38 @@ template <typename T>
 __device__ __forceinline__ void epilogue(const GemmArgs &g, long long row, int col,
                                          const float (&s)[Elem<T>::kVec]) {
   constexpr int V = Elem<T>::kVec;
-  typename Elem<T>::Vec bias = {}, res = {}, z, y;
+  typename Elem<T>::Vec bias = {}, res = {}, slope, y;
   if (g.bias) bias = load_row((const T *)g.bias, col, g.n);
   if (g.res) res = load_row((const T *)g.res + row * g.ldres, col, g.n);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const float t = s[j] + (float)bias[j];
-    z[j] = (T)t;
-    y[j] = (T)(activate(t, g.act) + (float)res[j]);
+    float d;
+    y[j] = (T)(activate(s[j] + (float)bias[j], g.act, d) + (float)res[j]);
+    slope[j] = (T)d;
   }
-  if (g.z) store_row((T *)g.z + row * g.n, col, g.n, z);
+  if (g.slope) store_row((T *)g.slope + row * g.n, col, g.n, slope);
   store_row((T *)g.c + row * g.n, col, g.n, y);
 }
 
-// BM x BN tile by four waves (2 x 2), BK reduction steps at a time, the next in registers
-template <typename T, bool TA, bool TB, int BM, int BN>
-__global__ __launch_bounds__(256) void linear_gemm_kernel(GemmArgs g) {
-  constexpr int BK = sizeof(T) == 4 ? 32 : 64, P = Op<T>::P, V = Elem<T>::kVec;
-  constexpr int WM = BM / 2, WN = BN / 2, IM = WM / 32, IN = WN / 32;
-  typedef Panel<T, TA, BM, BK> PA;
-  typedef Panel<T, TB, BN, BK> PB;
-  constexpr int CP = WN + 4;                       // floats per row of the epilogue's slab
-  constexpr int SLAB = 4 * 32 * CP * 4, TILE = PA::BYTES + PB::BYTES;
-  __shared__ __attribute__((aligned(16))) char smem[TILE > SLAB ? TILE : SLAB];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  // workgroups land on the eight XCDs in turn: each XCD gets a contiguous eighth of the tiles, and
-  // walks them in columns of eight row tiles, so that what its L2 holds is read several times
+// workgroup -> tile and share.  Workgroups land on the eight XCDs in turn: each XCD gets a
+// contiguous eighth of the tiles, and walks them in columns of eight row tiles, so that what its L2
+// holds is read several times
+template <int BM, int BN>
+__device__ __forceinline__ void place(const GemmArgs &g, int &m0, int &n0, int &split) {
   const int total = gridDim.x, id = blockIdx.x, per = total / 8;
   int t = id < per * 8 ? (id & 7) * per + (id >> 3) : id;
-  const int split = t / (g.mt * g.nt);
+  split = t / (g.mt * g.nt);
   t -= split * (g.mt * g.nt);
   const int band = t / (8 * g.nt), in = t - band * 8 * g.nt, bh = min(8, g.mt - band * 8);
-  const int m0 = (band * 8 + in % bh) * BM, n0 = (in / bh) * BN;
-  const int kbeg = split * g.chunk, kend = min(g.k, kbeg + g.chunk);
-  const int wm = (w >> 1) * WM, wn = (w & 1) * WN;
+  m0 = (band * 8 + in % bh) * BM;
+  n0 = (in / bh) * BN;
+}
 
-  f32x16_t acc[IM][IN] = {};
-  PA pa;
-  PB pb;
-  char *la = smem, *lb = smem + PA::BYTES;
-  if (kbeg < kend) {
-    pa.fetch((const T *)g.a, g.lda, m0, g.m, kbeg, kend, tid);
-    pb.fetch((const T *)g.b, g.ldb, n0, g.n, kbeg, kend, tid);
-  }
-  for (int k0 = kbeg; k0 < kend; k0 += BK) {
-    lds_barrier();                                 // the previous step's reads are done
-    pa.store(la, tid);
-    pb.store(lb, tid);
-    if (k0 + BK < kend) {
-      pa.fetch((const T *)g.a, g.lda, m0, g.m, k0 + BK, kend, tid);
-      pb.fetch((const T *)g.b, g.ldb, n0, g.n, k0 + BK, kend, tid);
-    }
-    lds_barrier();
-#pragma unroll
-    for (int ks = 0; ks < BK; ks += 16) {
-      typename Op<T>::Frag fa[IM][P], fb[IN][P];
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-#pragma unroll
-        for (int i = 0; i < IM; ++i) fa[i][p] = PA::frag(la, p, wm + 32 * i, ks, lane);
-#pragma unroll
-        for (int j = 0; j < IN; ++j) fb[j][p] = PB::frag(lb, p, wn + 32 * j, ks, lane);
-      }
-#pragma unroll
-      for (int i = 0; i < IM; ++i)
-#pragma unroll
-        for (int j = 0; j < IN; ++j) {
-          if constexpr (P == 3) {                  // smallest terms first
-            acc[i][j] = mfma(fa[i][2], fb[j][0], acc[i][j]);
-            acc[i][j] = mfma(fa[i][0], fb[j][2], acc[i][j]);
-            acc[i][j] = mfma(fa[i][1], fb[j][1], acc[i][j]);
-            acc[i][j] = mfma(fa[i][1], fb[j][0], acc[i][j]);
-            acc[i][j] = mfma(fa[i][0], fb[j][1], acc[i][j]);
-          }
-          acc[i][j] = mfma(fa[i][0], fb[j][0], acc[i][j]);
-        }
-    }
-  }
-  // the tile leaves through LDS, 32 rows of a wave at a time, as 16-byte row pieces
-  float *slab = reinterpret_cast<float *>(smem) + w * 32 * CP;
-  __syncthreads();
+// a wave's IM x IN accumulators leave through LDS, 32 rows at a time, as 16-byte row pieces
+template <typename T, int IM, int IN>
+__device__ __forceinline__ void leave(const GemmArgs &g, const f32x16_t (&acc)[IM][IN], float *slab,
+                                      int row0, int col0, int split, int lane) {
+  constexpr int V = Elem<T>::kVec, WN = 32 * IN, CP = WN + 4, PR = WN / V;
 #pragma unroll
   for (int i = 0; i < IM; ++i) {
 #pragma unroll
@@ -257,14 +251,17 @@ __global__ __launch_bounds__(256) void linear_gemm_kernel(GemmArgs g) {
         slab[((v & 3) + 8 * (v >> 2) + 4 * (lane >> 5)) * CP + 32 * j + (lane & 31)] = acc[i][j][v];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-    constexpr int PR = WN / V;                     // pieces per row
 #pragma unroll
     for (int q = 0; q < 32 * PR / 64; ++q) {
       const int e = lane + 64 * q, row = e / PR, col = (e % PR) * V;
-      const int gr = m0 + wm + 32 * i + row, gc = n0 + wn + col;
+      const int gr = row0 + 32 * i + row, gc = col0 + col;
       float s[V];
 #pragma unroll
-      for (int u = 0; u < V; ++u) s[u] = slab[row * CP + col + u];
+      for (int u = 0; u < V; u += 4) {
+        const f32x4_t t = *reinterpret_cast<const f32x4_t *>(slab + row * CP + col + u);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[u + x] = t[x];
+      }
       if (gr < g.m && gc < g.n) {
         if (g.nsplit > 1) {
           float *dst = g.part + ((long long)split * g.m + gr) * g.n;
@@ -278,6 +275,266 @@ __global__ __launch_bounds__(256) void linear_gemm_kernel(GemmArgs g) {
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// f32: BM x BN tile by four waves (2 x 2), 32 reduction steps at a time, the next in registers
+template <bool TA, bool TB, int BM, int BN>
+__global__ __launch_bounds__(256) void linear_gemm_kernel(GemmArgs g) {
+  constexpr int BK = 32, WM = BM / 2, WN = BN / 2, IM = WM / 32, IN = WN / 32;
+  typedef Panel<TA, BM, BK> PA;
+  typedef Panel<TB, BN, BK> PB;
+  constexpr int SLAB = 4 * 32 * (WN + 4) * 4, TILE = PA::BYTES + PB::BYTES;
+  __shared__ __attribute__((aligned(16))) char smem[TILE > SLAB ? TILE : SLAB];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int m0, n0, split;
+  place<BM, BN>(g, m0, n0, split);
+  const int kbeg = split * g.chunk, kend = min(g.k, kbeg + g.chunk);
+  const int wm = (w >> 1) * WM, wn = (w & 1) * WN;
+
+  f32x16_t acc[IM][IN] = {};
+  PA pa;
+  PB pb;
+  char *la = smem, *lb = smem + PA::BYTES;
+  if (kbeg < kend) {
+    pa.fetch((const float *)g.a, g.lda, m0, g.m, kbeg, kend, tid);
+    pb.fetch((const float *)g.b, g.ldb, n0, g.n, kbeg, kend, tid);
+  }
+  for (int k0 = kbeg; k0 < kend; k0 += BK) {
+    lds_barrier();                                 // the previous step's reads are done
+    pa.store(la, tid);
+    pb.store(lb, tid);
+    if (k0 + BK < kend) {
+      pa.fetch((const float *)g.a, g.lda, m0, g.m, k0 + BK, kend, tid);
+      pb.fetch((const float *)g.b, g.ldb, n0, g.n, k0 + BK, kend, tid);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int ks = 0; ks < BK; ks += 16) {
+      bf16x8_t fa[IM][3], fb[IN][3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+#pragma unroll
+        for (int i = 0; i < IM; ++i) fa[i][p] = PA::frag(la, p, wm + 32 * i, ks, lane);
+#pragma unroll
+        for (int j = 0; j < IN; ++j) fb[j][p] = PB::frag(lb, p, wn + 32 * j, ks, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {             // smallest terms first
+          acc[i][j] = mfma(fa[i][2], fb[j][0], acc[i][j]);
+          acc[i][j] = mfma(fa[i][0], fb[j][2], acc[i][j]);
+          acc[i][j] = mfma(fa[i][1], fb[j][1], acc[i][j]);
+          acc[i][j] = mfma(fa[i][1], fb[j][0], acc[i][j]);
+          acc[i][j] = mfma(fa[i][0], fb[j][1], acc[i][j]);
+          acc[i][j] = mfma(fa[i][0], fb[j][0], acc[i][j]);
+        }
+    }
+  }
+  __syncthreads();
+  leave<float, IM, IN>(g, acc, reinterpret_cast<float *>(smem) + w * 32 * (WN + 4), m0 + wm, n0 + wn,
+                       split, lane);
+}
+
+// R rows (m / n axis) x 64 reduction steps of a 16-bit operand in LDS.  TR false: [R][64]; true:
+// [64][R] in blocks of 128 (or 64) columns.
+template <typename T, bool TR, int R, int THREADS>
+struct DmaPanel {
+  static constexpr int D = TR ? (R >= 128 ? 128 : 64) : 64, BLOCKS = TR ? R / D : 1;
+  typedef Dma<D> DM;
+  static constexpr int BLOCK = 64 * DM::PITCH, BYTES = R * 128;
+  static constexpr int N = R * 8 / THREADS;        // 16-byte units a thread moves
+  int off[N];                                      // byte offsets from the step's first element
+  // k position of unit i inside a step (its row / its column)
+  __device__ static __forceinline__ int kpos(int i, int tid) {
+    const int e = i * THREADS + tid;
+    if (TR) return e % (BLOCK / 16) / DM::UNITS;
+    return ((e % DM::UNITS) ^ DM::swz(e / DM::UNITS)) * 8;
+  }
+  __device__ __forceinline__ void init(long long ld, int r0, int rmax, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = i * THREADS + tid;
+      if (TR) {
+        const int blk = e / (BLOCK / 16), row = e % (BLOCK / 16) / DM::UNITS;
+        const int col = blk * D + ((e % DM::UNITS) ^ DM::swz(row)) * 8;
+        off[i] = r0 + col < rmax ? (row * (int)ld + col) * 2 : kFar;
+      } else {
+        const int row = e / DM::UNITS;
+        off[i] = r0 + row < rmax ? row * (int)ld * 2 + kpos(i, tid) * 2 : kFar;
+      }
+    }
+  }
+  // step at reduction index k0 of the operand at src (its first row / column already added)
+  __device__ __forceinline__ void issue(const T *src, long long ld, int k0, int kend, char *lds,
+                                        int tid) const {
+    const i32x4_t rs = dma_rsrc((const char *)(src + (TR ? k0 * ld : (long long)k0)), kFar);
+    if (k0 + 64 <= kend) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) dma16(rs, off[i], lds + (i * THREADS + (tid & ~63)) * 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        dma16(rs, k0 + kpos(i, tid) < kend ? off[i] : kFar, lds + (i * THREADS + (tid & ~63)) * 16);
+    }
+  }
+  // fragment: 32 rows at r0 (a multiple of 32), reduction steps 16 ks .. + 15; base: row_base / nat_base
+  __device__ static __forceinline__ int base(int lane) {
+    return TR ? DM::nat_base(lane) : DM::row_base(lane & 31, lane >> 5);
+  }
+  __device__ static __forceinline__ typename Elem<T>::Vec frag(const char *lds, int base, int r0,
+                                                               int ks) {
+    if constexpr (!TR) {
+      return *reinterpret_cast<const typename Elem<T>::Vec *>(lds + r0 * 128 + (base ^ (ks << 5)));
+    } else {
+      union {
+        s16x4_t s[2];
+        typename Elem<T>::Vec f;
+      } u;
+      const char *t = lds + r0 / D * BLOCK + 16 * ks * DM::PITCH;
+      const int at = base ^ (r0 % D / 32 << 6);
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(t + at));
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4)(t + (at ^ DM::kNatHi) + 4 * DM::PITCH));
+      return u.f;
+    }
+  }
+};
+
+// 16 bits: BM x BN tile by GM x GN waves, 64 reduction steps at a time, double-buffered by DMA: the
+// next step's tiles are asked for right behind the one barrier of a step
+template <typename T, bool TA, bool TB, int BM, int BN, int GM, int GN>
+__global__ __launch_bounds__(64 * GM * GN, 2) void linear_dma_kernel(GemmArgs g) {
+  constexpr int THREADS = 64 * GM * GN, WM = BM / GM, WN = BN / GN, IM = WM / 32, IN = WN / 32;
+  typedef DmaPanel<T, TA, BM, THREADS> PA;
+  typedef DmaPanel<T, TB, BN, THREADS> PB;
+  typedef typename Elem<T>::Vec Vec;
+  constexpr int TILE = PA::BYTES + PB::BYTES, SLAB = GM * GN * 32 * (WN + 4) * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * TILE > SLAB ? 2 * TILE : SLAB];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int m0, n0, split;
+  place<BM, BN>(g, m0, n0, split);
+  const int kbeg = split * g.chunk, kend = min(g.k, kbeg + g.chunk);
+  const int wm = w / GN * WM, wn = w % GN * WN;
+  const T *ap = (const T *)g.a + (TA ? (long long)m0 : m0 * g.lda);
+  const T *bp = (const T *)g.b + (TB ? (long long)n0 : n0 * g.ldb);
+  PA pa;
+  PB pb;
+  pa.init(g.lda, m0, g.m, tid);
+  pb.init(g.ldb, n0, g.n, tid);
+  const int ab = PA::base(lane), bb = PB::base(lane);
+
+  f32x16_t acc[IM][IN] = {};
+  auto issue = [&](int k0, int buf) {
+    pa.issue(ap, g.lda, k0, kend, smem + buf * TILE, tid);
+    pb.issue(bp, g.ldb, k0, kend, smem + buf * TILE + PA::BYTES, tid);
+  };
+  if (kbeg < kend) issue(kbeg, 0);
+  int buf = 0;
+  for (int k0 = kbeg; k0 < kend; k0 += 64) {
+    dma_wait();
+    lds_barrier();
+    if (k0 + 64 < kend) issue(k0 + 64, buf ^ 1);
+    const char *la = smem + buf * TILE, *lb = la + PA::BYTES;
+    buf ^= 1;
+    Vec fa[2][IM], fb[2][IN];
+    auto load = [&](int ks) {
+#pragma unroll
+      for (int i = 0; i < IM; ++i) fa[ks & 1][i] = PA::frag(la, ab, wm + 32 * i, ks);
+#pragma unroll
+      for (int j = 0; j < IN; ++j) fb[ks & 1][j] = PB::frag(lb, bb, wn + 32 * j, ks);
+    };
+    load(0);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks < 3) load(ks + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+          acc[i][j] = mfma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j]);
+    }
+  }
+  __syncthreads();
+  leave<T, IM, IN>(g, acc, reinterpret_cast<float *>(smem) + w * 32 * (WN + 4), m0 + wm, n0 + wn,
+                   split, lane);
+}
+
+// Few rows of x (up to 16 MT): a workgroup's eight waves share 16 rows of W and split the reduction
+// (wave w: the steps of 32 numbered w, w + 8, ..), W goes from memory into the matrix instructions,
+// the eight sums meet in LDS.  Bound by the bytes of W: eight loads of 1 KB in flight a wave.
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void linear_rows_kernel(GemmArgs g) {
+  constexpr int P = Op<T>::P, U = sizeof(T) == 4 ? 4 : 8;
+  __shared__ float part[8][MT][16][20];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l15 = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  f32x4_t acc[MT] = {};
+  const T *wrow = (const T *)g.b + min(n0 + l15, g.n - 1) * g.ldb;
+  const T *xrow[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xrow[t] = (const T *)g.a + min(16 * t + l15, g.m - 1) * g.lda;
+  // U steps of 32 at a time, their loads together
+  for (int s0 = w * U * 32; s0 < g.k; s0 += 8 * U * 32) {
+    typename Elem<T>::Vec wv[U][sizeof(T) / 2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+        wv[u][h] = load_row(wrow, s0 + 32 * u + 8 * q + 4 * h, g.k);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      typename Op<T>::Frag fw[P], fx[P];
+      pack(wv[u], fw);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        typename Elem<T>::Vec xv[sizeof(T) / 2];
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+          xv[h] = load_row(xrow[t], s0 + 32 * u + 8 * q + 4 * h, g.k);
+        pack(xv, fx);
+        if constexpr (P == 3) {
+          acc[t] = mfma16(fw[2], fx[0], acc[t]);
+          acc[t] = mfma16(fw[0], fx[2], acc[t]);
+          acc[t] = mfma16(fw[1], fx[1], acc[t]);
+          acc[t] = mfma16(fw[1], fx[0], acc[t]);
+          acc[t] = mfma16(fw[0], fx[1], acc[t]);
+        }
+        acc[t] = mfma16(fw[0], fx[0], acc[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)                     // [row of x][row of W]
+    *reinterpret_cast<f32x4_t *>(&part[w][t][l15][4 * q]) = acc[t];
+  __syncthreads();
+  // 16 outputs of a row in pieces of V columns
+  constexpr int V = Elem<T>::kVec, PR = 16 / V;
+  for (int e = tid; e < MT * 16 * PR; e += 512) {
+    const int row = e / PR, col = (e % PR) * V;
+    if (row >= g.m || n0 + col >= g.n) continue;
+    float s[V] = {};
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int u = 0; u < V; ++u) s[u] += part[k][row >> 4][row & 15][col + u];
+    epilogue<T>(g, row, n0 + col, s);
+  }
+}
+
+// 16-bit rows -> rows of ldd elements on 16-byte boundaries, zeros behind them
+template <typename T>
+__global__ __launch_bounds__(256) void linear_pack_kernel(long long rows, int cols, const T *src,
+                                                          long long ld, T *dst, int ldd) {
+  const long long total = rows * (ldd / 8);
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total;
+       e += (long long)gridDim.x * 256) {
+    const long long row = e / (ldd / 8);
+    const int col = (int)(e - row * (ldd / 8)) * 8;
+    *reinterpret_cast<typename Elem<T>::Vec *>(dst + row * ldd + col) =
+        load_row(src + row * ld, col, cols);
   }
 }
 
@@ -305,12 +562,13 @@ __global__ __launch_bounds__(256) void linear_join_kernel(GemmArgs g) {
   }
 }
 
-// dz = dy act'(z) and the column sums of dz over this workgroup's rows: 32 threads along the
-// columns (a vector each), 8 rows at a time
+// dz = dy slope (ReLU: dy where slope > 0) into rows of ldz elements, zeros behind them, and the
+// column sums of dz over this workgroup's rows: 32 threads along the columns (a vector each), 8 rows
+// at a time.  dz NULL: the sums only.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, const T *dy,
-                                                        long long lddy, const T *z, int act, T *dz,
-                                                        float *part) {
+                                                        long long lddy, const T *slope, int act,
+                                                        T *dz, int ldz, float *part) {
   constexpr int V = Elem<T>::kVec;
   __shared__ float red[8][32 * V];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, col = (blockIdx.x * 32 + cl) * V;
@@ -319,16 +577,16 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, cons
     for (long long row = (long long)blockIdx.y * 8 + rl; row < m; row += (long long)gridDim.y * 8) {
       typename Elem<T>::Vec g = load_row(dy + row * lddy, col, n);
       if (act != kActNone) {
-        const typename Elem<T>::Vec zz = load_row(z + row * n, col, n);
+        const typename Elem<T>::Vec d = load_row(slope + row * n, col, n);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (act == kActRelu)                     // (a select: an infinite dy stays out of it)
-            g[j] = (float)zz[j] > 0.f ? g[j] : (T)0.f;
+            g[j] = (float)d[j] > 0.f ? g[j] : (T)0.f;
           else
-            g[j] = (T)((float)g[j] * activate_grad((float)zz[j], act));
+            g[j] = (T)((float)g[j] * (float)d[j]);
         }
-        store_row(dz + row * n, col, n, g);
       }
+      if (dz) store_row(dz + row * ldz, col, ldz, g);
 #pragma unroll
       for (int j = 0; j < V; ++j) sum[j] += (float)g[j];
     }
@@ -365,43 +623,78 @@ __global__ __launch_bounds__(256) void linear_dbias_kernel(const float *part, in
 
 // --------------------------------------------------------------------------------------- host
 struct Plan {
-  int bm, mt, nt, nsplit, chunk;
+  int bm, bn, mt, nt, nsplit, chunk;
 };
 
-// 128 x 128 tiles where they give every CU one; else 64 x 64, and while those leave CUs idle the
-// reduction is cut into shares of at least 256 steps
-Plan plan_gemm(int m, int n, int k) {
+// The largest tile that still gives every CU a workgroup; below that the smallest, and while its
+// tiles leave CUs idle the reduction is cut into shares of at least 256 steps.
+Plan plan_gemm(int m, int n, int k, bool dma) {
   Plan p;
-  p.bm = (long long)cdiv(m, 128) * cdiv(n, 128) >= 256 ? 128 : 64;
+  auto tiles = [&](int b) { return (long long)cdiv(m, b) * cdiv(n, b); };
+  p.bm = p.bn = dma && tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 64;
   p.mt = cdiv(m, p.bm);
-  p.nt = cdiv(n, p.bm);
-  const long long tiles = (long long)p.mt * p.nt;
+  p.nt = cdiv(n, p.bn);
+  const long long t = (long long)p.mt * p.nt;
   long long s = 1;
-  if (tiles < 256) s = std::max<long long>(1, std::min<long long>((512 + tiles - 1) / tiles, k / 256));
+  if (t < 256) s = std::max<long long>(1, std::min<long long>((512 + t - 1) / t, k / 256));
   p.chunk = std::max(64, cdiv(cdiv(k, s), 64) * 64);
   p.nsplit = std::max(1, cdiv(k, p.chunk));
   return p;
 }
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
-size_t split_bytes(int m, int n, int k) {
-  const Plan p = plan_gemm(m, n, k);
+size_t split_bytes(int m, int n, int k, bool dma) {
+  const Plan p = plan_gemm(m, n, k, dma);
   return p.nsplit > 1 ? align256((size_t)p.nsplit * m * n * sizeof(float)) : 0;
 }
+int up8(int v) { return (v + 7) & ~7; }
+// rows a DMA may read where they are: whole 16-byte units on 16-byte boundaries, a tile's offsets
+// below 2^31
+bool dma_rows(const void *p, long long ld, int len) {
+  return ((uintptr_t)p & 15) == 0 && len % 8 == 0 && ld % 8 == 0 && ld <= (1 << 22);
+}
+size_t pack_bytes(const void *p, long long ld, long long rows, int len) {
+  return dma_rows(p, ld, len) ? 0 : align256((size_t)rows * up8(len) * 2);
+}
+constexpr int kFewRows = 16;       // linear_rows_kernel up to here
 // workgroups along the rows of the dz / dbias pass
 int dz_blocks(long long m, int n) {
   const long long cols = cdiv(n, 128);
   return (int)std::max<long long>(1, std::min<long long>((m + 31) / 32, (2048 + cols - 1) / cols));
 }
 
+// an operand as the DMA kernels want it: where it is, or packed into ws (which moves on)
+template <typename T>
+void pack_rows(const void *&p, long long &ld, long long rows, int len, char *&ws, hipStream_t hs) {
+  if (dma_rows(p, ld, len)) return;
+  const int ldd = up8(len);
+  const long long units = rows * (ldd / 8);
+  hipLaunchKernelGGL((linear_pack_kernel<T>),
+                     dim3((unsigned)std::min<long long>(4096, (units + 255) / 256)), dim3(256), 0, hs,
+                     rows, len, (const T *)p, ld, (T *)ws, ldd);
+  p = ws;
+  ld = ldd;
+  ws += align256((size_t)rows * ldd * 2);
+}
+
 template <typename T, bool TA, bool TB>
-void launch_gemm(GemmArgs g, float *ws, hipStream_t hs) {
-  const Plan p = plan_gemm(g.m, g.n, g.k);
-  g.mt = p.mt; g.nt = p.nt; g.nsplit = p.nsplit; g.chunk = p.chunk; g.part = ws;
+void launch_gemm(GemmArgs g, void *ws, hipStream_t hs) {
+  constexpr bool DMA = sizeof(T) == 2;
+  const Plan p = plan_gemm(g.m, g.n, g.k, DMA);
+  g.mt = p.mt; g.nt = p.nt; g.nsplit = p.nsplit; g.chunk = p.chunk; g.part = (float *)ws;
   const dim3 grid((unsigned)((long long)p.mt * p.nt * p.nsplit));
-  if (p.bm == 128)
-    hipLaunchKernelGGL((linear_gemm_kernel<T, TA, TB, 128, 128>), grid, dim3(256), 0, hs, g);
-  else
-    hipLaunchKernelGGL((linear_gemm_kernel<T, TA, TB, 64, 64>), grid, dim3(256), 0, hs, g);
+  if constexpr (DMA) {
+    if (p.bm == 256)
+      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 256, 2, 4>), grid, dim3(512), 0, hs, g);
+    else if (p.bm == 128)
+      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 128, 128, 2, 2>), grid, dim3(256), 0, hs, g);
+    else
+      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 64, 64, 2, 2>), grid, dim3(256), 0, hs, g);
+  } else {
+    if (p.bm == 128)
+      hipLaunchKernelGGL((linear_gemm_kernel<TA, TB, 128, 128>), grid, dim3(256), 0, hs, g);
+    else
+      hipLaunchKernelGGL((linear_gemm_kernel<TA, TB, 64, 64>), grid, dim3(256), 0, hs, g);
+  }
   if (p.nsplit > 1) {
     const long long pieces = (long long)g.m * cdiv(g.n, Elem<T>::kVec);
     hipLaunchKernelGGL((linear_join_kernel<T>),
@@ -410,15 +703,109 @@ void launch_gemm(GemmArgs g, float *ws, hipStream_t hs) {
   }
 }
 
-int check(const char *what, int dtype, int m, int n, int k, int act) {
-  BTR_REQUIRE(dtype >= BTR_F32 && dtype <= BTR_F16, "%s: unknown element type %d", what, dtype);
-  BTR_REQUIRE(act >= BTR_ACT_NONE && act <= BTR_ACT_GELU, "%s: unknown activation %d", what, act);
+int check(const char *what, const btr_linear_t *p) {
+  BTR_REQUIRE(p, "%s: null description", what);
+  BTR_REQUIRE(p->dtype >= BTR_F32 && p->dtype <= BTR_F16, "%s: unknown element type %d", what,
+              p->dtype);
+  BTR_REQUIRE(p->act >= BTR_ACT_NONE && p->act <= BTR_ACT_GELU, "%s: unknown activation %d", what,
+              p->act);
+  const int m = p->m, n = p->n, k = p->k;
   BTR_REQUIRE(m >= 0 && n >= 1 && k >= 1 && m <= (1 << 30) && n <= (1 << 30) && k <= (1 << 30) &&
                   ((long long)cdiv(m, 64) * cdiv(n, 64) <= (1 << 30)) &&
                   ((long long)cdiv(m, 64) * cdiv(k, 64) <= (1 << 30)) &&
                   ((long long)cdiv(n, 64) * cdiv(k, 64) <= (1 << 30)),
               "%s: (%d, %d) x (%d, %d)", what, m, k, n, k);
+  BTR_REQUIRE(m == 0 || (p->x && p->weight && p->ldx >= k && p->ldw >= k &&
+                         (!p->residual || p->ldr >= n)),
+              "%s: null pointer or a row stride below the row", what);
   return BTR_OK;
+}
+
+size_t fwd_bytes(const btr_linear_t &p) {
+  if (p.m <= kFewRows) return 0;
+  if (p.dtype == BTR_F32) return split_bytes(p.m, p.n, p.k, false);
+  return pack_bytes(p.x, p.ldx, p.m, p.k) + pack_bytes(p.weight, p.ldw, p.n, p.k) +
+         split_bytes(p.m, p.n, p.k, true);
+}
+
+template <typename T>
+void forward(const btr_linear_t &p, void *y, void *slope, void *workspace, hipStream_t hs) {
+  GemmArgs g{};
+  g.m = p.m; g.n = p.n; g.k = p.k;
+  g.a = p.x; g.lda = p.ldx; g.b = p.weight; g.ldb = p.ldw;
+  g.bias = p.bias; g.res = p.residual; g.ldres = p.ldr; g.act = p.act;
+  g.c = y; g.slope = slope;
+  if (p.m <= kFewRows) {
+    hipLaunchKernelGGL((linear_rows_kernel<T, 1>), dim3(cdiv(p.n, 16)), dim3(512), 0, hs, g);
+    return;
+  }
+  char *ws = (char *)workspace;
+  if constexpr (sizeof(T) == 2) {
+    pack_rows<T>(g.a, g.lda, p.m, p.k, ws, hs);
+    pack_rows<T>(g.b, g.ldb, p.n, p.k, ws, hs);
+  }
+  launch_gemm<T, false, false>(g, ws, hs);
+}
+
+// dz is written unless dy itself can be read as it is
+bool writes_dz(const btr_linear_t &p, const void *dy, long long lddy) {
+  return p.act != BTR_ACT_NONE || (p.dtype != BTR_F32 && !dma_rows(dy, lddy, p.n));
+}
+size_t bwd_bytes(const btr_linear_t &p, const void *dy, long long lddy) {
+  const int m = p.m, n = p.n, k = p.k;
+  if (m == 0) return 0;
+  const bool f32 = p.dtype == BTR_F32;
+  size_t v = align256((size_t)dz_blocks(m, n) * n * sizeof(float));
+  if (writes_dz(p, dy, lddy)) v += align256((size_t)m * (f32 ? n * 4ll : up8(n) * 2ll));
+  if (!f32) v += pack_bytes(p.x, p.ldx, m, k) + pack_bytes(p.weight, p.ldw, n, k);
+  return v + std::max(split_bytes(m, k, n, !f32), split_bytes(n, k, m, !f32));
+}
+
+template <typename T>
+void backward(const btr_linear_t &p, const void *slope, const void *dy, long long lddy, void *dx,
+              void *dweight, void *dbias, void *workspace, hipStream_t hs) {
+  const int m = p.m, n = p.n, k = p.k;
+  char *ws = (char *)workspace;
+  float *part = (float *)ws;
+  const int blocks = m > 0 ? dz_blocks(m, n) : 0;
+  const void *gz = dy;                             // what the two products read
+  long long ldg = lddy;
+  if (m > 0) {
+    ws += align256((size_t)blocks * n * sizeof(float));
+    void *dz = nullptr;
+    const int ldz = sizeof(T) == 4 ? n : up8(n);
+    if (writes_dz(p, dy, lddy)) {
+      dz = ws;
+      ws += align256((size_t)m * ldz * sizeof(T));
+      gz = dz;
+      ldg = ldz;
+    }
+    if (dz || dbias)
+      hipLaunchKernelGGL((linear_dz_kernel<T>), dim3(cdiv(n, 32 * Elem<T>::kVec), blocks), dim3(256),
+                         0, hs, (long long)m, n, (const T *)dy, lddy, (const T *)slope, p.act,
+                         (T *)dz, ldz, dbias ? part : nullptr);
+  }
+  if (dbias)   // (no rows: zeros)
+    hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3(cdiv(n, 32)), dim3(256), 0, hs, part, blocks, n,
+                       (T *)dbias);
+  const void *x = p.x, *wt = p.weight;
+  long long ldx = p.ldx, ldw = p.ldw;
+  if constexpr (sizeof(T) == 2) {
+    if (m > 0 && dweight) pack_rows<T>(x, ldx, m, k, ws, hs);
+    if (m > 0 && dx) pack_rows<T>(wt, ldw, n, k, ws, hs);
+  }
+  if (dx && m > 0) {
+    GemmArgs g{};
+    g.m = m; g.n = k; g.k = n;
+    g.a = gz; g.lda = ldg; g.b = wt; g.ldb = ldw; g.c = dx;
+    launch_gemm<T, false, true>(g, ws, hs);
+  }
+  if (dweight) {
+    GemmArgs g{};
+    g.m = n; g.n = k; g.k = m;                     // (no rows: an empty reduction writes zeros)
+    g.a = gz; g.lda = ldg; g.b = x; g.ldb = ldx; g.c = dweight;
+    launch_gemm<T, true, true>(g, ws, hs);
+  }
 }
 
 }  // namespace
@@ -426,85 +813,39 @@ int check(const char *what, int dtype, int m, int n, int k, int act) {
 
 using namespace btr;
 
-extern "C" size_t btr_linear_fwd_workspace_bytes(int m, int n, int k) {
-  if (check("linear_fwd", BTR_F32, m, n, k, 0) != BTR_OK || m == 0) return 0;
-  return split_bytes(m, n, k);
+extern "C" size_t btr_linear_fwd_workspace_bytes(const btr_linear_t *p) {
+  return check("linear_fwd", p) == BTR_OK ? fwd_bytes(*p) : 0;
 }
 
-extern "C" int btr_linear_fwd(int dtype, int m, int n, int k, const void *x, long long ldx,
-                              const void *weight, long long ldw, const void *bias, int act,
-                              const void *residual, long long ldr, void *y, void *z,
-                              void *workspace, size_t workspace_bytes, btr_stream_t stream) {
-  const int rc = check("linear_fwd", dtype, m, n, k, act);
+extern "C" int btr_linear_fwd(const btr_linear_t *p, void *y, void *slope, void *workspace,
+                              size_t workspace_bytes, btr_stream_t stream) {
+  const int rc = check("linear_fwd", p);
   if (rc != BTR_OK) return rc;
-  if (m == 0) return BTR_OK;
-  BTR_REQUIRE(x && weight && y && ldx >= k && ldw >= k && (!residual || ldr >= n),
-              "linear_fwd: null pointer or a row stride below the row");
-  const size_t need = btr_linear_fwd_workspace_bytes(m, n, k);
+  if (p->m == 0) return BTR_OK;
+  BTR_REQUIRE(y, "linear_fwd: null pointer");
+  const size_t need = fwd_bytes(*p);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "linear_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  GemmArgs g{};
-  g.m = m; g.n = n; g.k = k;
-  g.a = x; g.lda = ldx; g.b = weight; g.ldb = ldw;
-  g.bias = bias; g.res = residual; g.ldres = ldr; g.act = act;
-  g.c = y; g.z = z;
-  BTR_DISPATCH_DTYPE(dtype, (launch_gemm<T, false, false>(g, (float *)workspace, as_stream(stream))));
+  BTR_DISPATCH_DTYPE(p->dtype, forward<T>(*p, y, slope, workspace, as_stream(stream)));
   return check_launch("linear_fwd");
 }
 
-extern "C" size_t btr_linear_bwd_workspace_bytes(int dtype, int m, int n, int k) {
-  if (check("linear_bwd", dtype, m, n, k, 0) != BTR_OK || m == 0) return 0;
-  const size_t elem = dtype == BTR_F32 ? 4 : 2;
-  return align256((size_t)m * n * elem) + align256((size_t)dz_blocks(m, n) * n * sizeof(float)) +
-         std::max(split_bytes(m, k, n), split_bytes(n, k, m));
+extern "C" size_t btr_linear_bwd_workspace_bytes(const btr_linear_t *p, const void *dy,
+                                                 long long lddy) {
+  return check("linear_bwd", p) == BTR_OK ? bwd_bytes(*p, dy, lddy) : 0;
 }
 
-extern "C" int btr_linear_bwd(int dtype, int m, int n, int k, const void *x, long long ldx,
-                              const void *weight, long long ldw, int act, const void *z,
-                              const void *dy, long long lddy, void *dx, void *dweight,
-                              void *dbias, void *workspace, size_t workspace_bytes,
-                              btr_stream_t stream) {
-  const int rc = check("linear_bwd", dtype, m, n, k, act);
+extern "C" int btr_linear_bwd(const btr_linear_t *p, const void *slope, const void *dy,
+                              long long lddy, void *dx, void *dweight, void *dbias,
+                              void *workspace, size_t workspace_bytes, btr_stream_t stream) {
+  const int rc = check("linear_bwd", p);
   if (rc != BTR_OK) return rc;
-  hipStream_t hs = as_stream(stream);
-  BTR_REQUIRE(m == 0 || (dy && lddy >= n && (act == BTR_ACT_NONE || z) &&
-                         (!dx || (weight && ldw >= k)) && (!dweight || (x && ldx >= k))),
+  BTR_REQUIRE(p->m == 0 || (dy && lddy >= p->n && (p->act == BTR_ACT_NONE || slope)),
               "linear_bwd: null pointer or a row stride below the row");
-  const size_t need = btr_linear_bwd_workspace_bytes(dtype, m, n, k);
+  const size_t need = bwd_bytes(*p, dy, lddy);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "linear_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  const size_t elem = dtype == BTR_F32 ? 4 : 2;
-  char *ws = (char *)workspace;
-  void *dz = ws;
-  float *part = (float *)(ws + align256((size_t)m * n * elem));
-  float *share = (float *)((char *)part + align256((size_t)dz_blocks(m, n) * n * sizeof(float)));
-  const void *gz = dy;                             // what the two products read
-  long long ldg = lddy;
-  if (m > 0 && (act != BTR_ACT_NONE || dbias)) {
-    const int blocks = dz_blocks(m, n);
-    BTR_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(
-        (linear_dz_kernel<T>), dim3(cdiv(n, 32 * Elem<T>::kVec), blocks), dim3(256), 0, hs,
-        (long long)m, n, (const T *)dy, lddy, (const T *)z, act, (T *)dz, dbias ? part : nullptr));
-    if (act != BTR_ACT_NONE) {
-      gz = dz;
-      ldg = n;
-    }
-  }
-  if (dbias)   // (no rows: zeros)
-    BTR_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3(cdiv(n, 32)),
-                                                 dim3(256), 0, hs, part,
-                                                 m > 0 ? dz_blocks(m, n) : 0, n, (T *)dbias));
-  if (dx && m > 0) {
-    GemmArgs g{};
-    g.m = m; g.n = k; g.k = n;
-    g.a = gz; g.lda = ldg; g.b = weight; g.ldb = ldw; g.c = dx;
-    BTR_DISPATCH_DTYPE(dtype, (launch_gemm<T, false, true>(g, share, hs)));
-  }
-  if (dweight) {
-    GemmArgs g{};
-    g.m = n; g.n = k; g.k = m;                     // (no rows: an empty reduction writes zeros)
-    g.a = gz; g.lda = ldg; g.b = x; g.ldb = ldx; g.c = dweight;
-    BTR_DISPATCH_DTYPE(dtype, (launch_gemm<T, true, true>(g, share, hs)));
-  }
+  BTR_DISPATCH_DTYPE(p->dtype, backward<T>(*p, slope, dy, lddy, dx, dweight, dbias, workspace,
+                                           as_stream(stream)));
   return check_launch("linear_bwd");
 }

@@ -141,26 +141,28 @@ class _Linear(Function):
         b = None if bias is None else bias.contiguous()
         dev = x.device
         y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
-        keep, z = None, None      # keep: what act' is taken from in the backward
+        keep, slope = None, None      # keep: what dz is made of in the backward
         if act and any(ctx.needs_input_grad[:3]):
             if act == _ACTIVATIONS["relu"] and residual is None:
                 keep = y                                          # y > 0 exactly where z > 0
             else:
-                keep = z = torch.empty((m, n), dtype=x.dtype, device=dev)
-        nbytes = _lib.btr_linear_fwd_workspace_bytes(m, n, k)
+                keep = slope = torch.empty((m, n), dtype=x.dtype, device=dev)
+        p = _ext.Linear(_DTYPES[x.dtype], m, n, k, act, xr.data_ptr(), wr.data_ptr(), _ptr(b),
+                        _ptr(rr), ldx, ldw, ldr)
+        addr = ctypes.addressof(p)
+        nbytes = _lib.btr_linear_fwd_workspace_bytes(addr)
         ws = _workspace(nbytes, dev)
         with _on(x) as d:
-            _call(_lib.btr_linear_fwd, _DTYPES[x.dtype], m, n, k, _ptr(xr), ldx, _ptr(wr), ldw,
-                  _ptr(b), act, _ptr(rr), ldr, _ptr(y), _ptr(z), _ptr(ws), nbytes, _stream(d))
+            _call(_lib.btr_linear_fwd, addr, y.data_ptr(), _ptr(slope), _ptr(ws), nbytes, _stream(d))
         ctx.save_for_backward(xr, wr, keep)
-        ctx.layout = (m, n, k, ldx, ldw, act, x.shape)
+        ctx.layout = (m, n, k, act, ldx, ldw, x.shape)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, keep = ctx.saved_tensors
-        m, n, k, ldx, ldw, act, shape = ctx.layout
+        m, n, k, act, ldx, ldw, shape = ctx.layout
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         dev, dtype = x.device, x.dtype
         dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
@@ -168,12 +170,14 @@ class _Linear(Function):
         db = torch.empty((n,), dtype=dtype, device=dev) if need_b else None
         if need_x or need_w or need_b:
             gr, ldg = _rows(dy)
-            nbytes = _lib.btr_linear_bwd_workspace_bytes(_DTYPES[dtype], m, n, k)
+            p = _ext.Linear(_DTYPES[dtype], m, n, k, act, x.data_ptr(), weight.data_ptr(), None, None,
+                            ldx, ldw, 0)
+            addr = ctypes.addressof(p)
+            nbytes = _lib.btr_linear_bwd_workspace_bytes(addr, gr.data_ptr(), ldg)
             ws = _workspace(nbytes, dev)
             with _on(x) as d:
-                _call(_lib.btr_linear_bwd, _DTYPES[dtype], m, n, k, _ptr(x), ldx, _ptr(weight),
-                      ldw, act, _ptr(keep), _ptr(gr), ldg, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
-                      nbytes, _stream(d))
+                _call(_lib.btr_linear_bwd, addr, _ptr(keep), gr.data_ptr(), ldg, _ptr(dx), _ptr(dw),
+                      _ptr(db), _ptr(ws), nbytes, _stream(d))
         return dx, dw, db, dy if need_r else None, None
 
 

@@ -136,12 +136,10 @@ _SIGNATURES = {
     "btr_layer_norm_bwd_workspace_bytes": (_sz, [_ll, _ci]),
     "btr_layer_norm_bwd": (_ci, [_ci, _ll, _ci, _vp, _ll, _vp, _ll, _vp, _ll] + [_vp] * 6 +
                            [_sz, _vp]),
-    "btr_linear_fwd_workspace_bytes": (_sz, [_ci] * 3),
-    "btr_linear_fwd": (_ci, [_ci] * 4 + [_vp, _ll, _vp, _ll, _vp, _ci, _vp, _ll, _vp, _vp, _vp, _sz,
-                                         _vp]),
-    "btr_linear_bwd_workspace_bytes": (_sz, [_ci] * 4),
-    "btr_linear_bwd": (_ci, [_ci] * 4 + [_vp, _ll, _vp, _ll, _ci, _vp, _vp, _ll] + [_vp] * 4 +
-                       [_sz, _vp]),
+    "btr_linear_fwd_workspace_bytes": (_sz, [_vp]),
+    "btr_linear_fwd": (_ci, [_vp] * 4 + [_sz, _vp]),
+    "btr_linear_bwd_workspace_bytes": (_sz, [_vp, _vp, _ll]),
+    "btr_linear_bwd": (_ci, [_vp] * 3 + [_ll] + [_vp] * 4 + [_sz, _vp]),
     "btr_cross_attention_fwd_workspace_bytes": (_sz, [_vp]),
     "btr_cross_attention_fwd": (_ci, [_vp] * 4 + [_sz, _vp]),
     "btr_cross_attention_bwd_workspace_bytes": (_sz, [_vp]),
@@ -339,6 +337,13 @@ class DecoderPlan(ctypes.Structure):
         "bwd_scratch_bytes", "g_sa_in_w", "g_sa_in_b", "g_sa_out_w", "g_sa_out_b", "g_ca_in_w",
         "g_ca_in_b", "g_ca_out_w", "g_ca_out_b", "g_lin1_w", "g_lin1_b", "g_lin2_w",
         "g_lin2_b")] + [("g_ln", _sz3), ("grads_floats", _sz)]
+
+
+class Linear(ctypes.Structure):
+    """btr_linear_t: one linear layer (sizes, operands, element row strides)."""
+    _fields_ = [(n, _ci) for n in ("dtype", "m", "n", "k", "act")] + \
+        [(n, _vp) for n in ("x", "weight", "bias", "residual")] + \
+        [(n, _ll) for n in ("ldx", "ldw", "ldr")]
 
 
 class CrossAttention(ctypes.Structure):

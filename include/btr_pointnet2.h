@@ -1133,22 +1133,26 @@ int btr_layer_norm_bwd(int dtype, long long rows, int width, const void *x, long
                        void *dbias, void *workspace, size_t workspace_bytes, btr_stream_t stream);
 
 /* z = x weight^T + bias, y = act(z) [+ residual]: x (m, k), weight (n, k), bias (n) or NULL, residual
- * (m, n) or NULL, y (m, n) contiguous.  act: BTR_ACT_*; GELU is the erf form.  z (m, n) contiguous
- * in the type of x: what the backward of an activation needs, or NULL.  n, k >= 1. */
+ * (m, n) or NULL, y (m, n) contiguous.  act: BTR_ACT_*; GELU is the erf form.  slope (m, n) contiguous
+ * in the type of x: receives act'(z), what the backward of an activation needs, or NULL.  n, k >= 1. */
 #define BTR_ACT_NONE 0
 #define BTR_ACT_RELU 1
 #define BTR_ACT_GELU 2
-size_t btr_linear_fwd_workspace_bytes(int m, int n, int k);
-int btr_linear_fwd(int dtype, int m, int n, int k, const void *x, long long ldx, const void *weight,
-                   long long ldw, const void *bias, int act, const void *residual, long long ldr,
-                   void *y, void *z, void *workspace, size_t workspace_bytes, btr_stream_t stream);
+typedef struct {
+  int dtype, m, n, k, act;
+  const void *x, *weight, *bias, *residual;
+  long long ldx, ldw, ldr;        /* row strides of x, weight, residual */
+} btr_linear_t;
+
+size_t btr_linear_fwd_workspace_bytes(const btr_linear_t *p);
+int btr_linear_fwd(const btr_linear_t *p, void *y, void *slope, void *workspace,
+                   size_t workspace_bytes, btr_stream_t stream);
 /* dx (m, k), dweight (n, k), dbias (n), contiguous, each may be NULL; the gradient of the residual
- * is dy itself.  z as the forward left it (ReLU without a residual: y serves as well), unused and
- * may be NULL without activation. */
-size_t btr_linear_bwd_workspace_bytes(int dtype, int m, int n, int k);
-int btr_linear_bwd(int dtype, int m, int n, int k, const void *x, long long ldx, const void *weight,
-                   long long ldw, int act, const void *z, const void *dy, long long lddy, void *dx,
-                   void *dweight, void *dbias, void *workspace, size_t workspace_bytes,
+ * is dy itself (bias and residual of the description are not read).  slope as the forward left it
+ * (ReLU without a residual: y serves as well), unused and may be NULL without activation. */
+size_t btr_linear_bwd_workspace_bytes(const btr_linear_t *p, const void *dy, long long lddy);
+int btr_linear_bwd(const btr_linear_t *p, const void *slope, const void *dy, long long lddy,
+                   void *dx, void *dweight, void *dbias, void *workspace, size_t workspace_bytes,
                    btr_stream_t stream);
 
 /* out = softmax(scale q k^T) v per head, q (b, lq, h, d), k / v (b, lk, hk, d) with strides

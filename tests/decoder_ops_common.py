@@ -93,7 +93,7 @@ def linear(x, weight, bias, act, residual, dy=None):
     pdf = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     if act == "relu":
         a, slope, ea = z.clamp(min=0), (z > 0).double(), ez
-    elif act == "gelu":                    # |gelu'| <= 1.13; the kernel's erfc is good to 16 ulp
+    elif act == "gelu":                    # |gelu'| <= 1.13; the kernel's Phi is good to 40 f relative
         a, slope, ea = z * cdf, cdf + z * pdf, 1.13 * ez + 40 * F * (z * cdf).abs()
     else:
         a, slope, ea = z, torch.ones_like(z), ez
@@ -106,8 +106,8 @@ def linear(x, weight, bias, act, residual, dy=None):
     dz = g * slope
     if act == "relu":      # z within its error of zero may fall on either side
         edz = g.abs() * (z.abs() <= ez + tiny(dtype)).double()
-    elif act == "gelu":    # kept z: half a step; |gelu''| <= 0.8; 2^-20 for the slope's own arithmetic
-        edz = g.abs() * (0.8 * (u * z.abs() + ez + tiny(dtype)) + 2.0 ** -20) + u * dz.abs() + tiny(dtype)
+    elif act == "gelu":    # the kept slope: half a step; |gelu''| <= 0.8; 2^-20 for its own arithmetic
+        edz = g.abs() * (u * slope.abs() + tiny(dtype) + 0.8 * ez + 2.0 ** -20) + u * dz.abs() + tiny(dtype)
     else:
         edz = torch.zeros_like(g)
     dx, dw, db = dz @ W, dz.t() @ X, dz.sum(0)

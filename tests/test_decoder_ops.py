@@ -45,17 +45,31 @@ def test_layer_norm_entry_refuses():
 
 
 def test_linear_entry_refuses():
-    def fwd(dtype=0, m=4, n=8, k=16, x=PTR, ldx=16, w=PTR, ldw=16, act=0, r=None, ldr=0, y=PTR):
-        return lib.btr_linear_fwd(dtype, m, n, k, x, ldx, w, ldw, None, act, r, ldr, y, None, None, 0,
-                                  None)
-    for bad in (dict(dtype=9), dict(m=-1), dict(n=0), dict(k=0), dict(x=None), dict(w=None),
-                dict(y=None), dict(ldx=15), dict(ldw=15), dict(r=PTR, ldr=7), dict(act=3)):
-        assert fwd(**bad) == -1 and "linear_fwd" in _error(), bad
-    assert fwd(m=1, n=64, k=100000, ldx=100000, ldw=100000) == -1 and "workspace" in _error()
-    assert fwd(m=0, x=None, w=None, y=None) == 0
+    def desc(**kw):
+        p = _ext.Linear(dtype=0, m=40, n=8, k=16, act=0, x=PTR, weight=PTR, ldx=16, ldw=16)
+        for name, value in kw.items():
+            setattr(p, name, value)
+        return p
 
-    def bwd(ldg=8, act=0, z=None, dy=PTR, ws=PTR, nbytes=1 << 20):
-        return lib.btr_linear_bwd(0, 4, 8, 16, PTR, 16, PTR, 16, act, z, dy, ldg, PTR, PTR, PTR, ws,
+    def fwd(p, y=PTR, ws=None, nbytes=0):
+        return lib.btr_linear_fwd(ctypes.addressof(p), y, None, ws, nbytes, None)
+    for bad in (dict(dtype=9), dict(m=-1), dict(n=0), dict(k=0), dict(x=None), dict(weight=None),
+                dict(ldx=15), dict(ldw=15), dict(residual=PTR, ldr=7), dict(act=3), dict(act=-1),
+                dict(m=2 ** 30, n=2 ** 30)):
+        assert fwd(desc(**bad)) == -1 and "linear_fwd" in _error(), bad
+        assert lib.btr_linear_fwd_workspace_bytes(ctypes.addressof(desc(**bad))) == 0
+    assert fwd(desc(), y=None) == -1
+    assert lib.btr_linear_fwd(None, PTR, None, None, 0, None) == -1
+    long = desc(m=40, k=100000, ldx=100000, ldw=100000)       # shares of the reduction
+    need = lib.btr_linear_fwd_workspace_bytes(ctypes.addressof(long))
+    assert need > 0 and fwd(long, ws=PTR, nbytes=need - 1) == -1 and "workspace" in _error()
+    assert fwd(long, ws=None, nbytes=need) == -1
+    odd = desc(dtype=1, k=15, ldx=15, ldw=15)                 # rows that are packed first
+    assert lib.btr_linear_fwd_workspace_bytes(ctypes.addressof(odd)) > 0
+    assert fwd(desc(m=0, x=None, weight=None), y=None) == 0
+
+    def bwd(ldg=8, act=0, slope=None, dy=PTR, ws=PTR, nbytes=1 << 20):
+        return lib.btr_linear_bwd(ctypes.addressof(desc(act=act)), slope, dy, ldg, PTR, PTR, PTR, ws,
                                   nbytes, None)
     for bad in (dict(ldg=7), dict(act=2), dict(dy=None), dict(ws=None), dict(nbytes=16)):
         assert bwd(**bad) == -1 and "linear_bwd" in _error(), bad
