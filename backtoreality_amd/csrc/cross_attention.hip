@@ -993,7 +993,7 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
       lv.words(k0 + 128, min(kend, k0 + 160), lane, next);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the reads of the buffer it refills
       issue(k0 + 128, buf ^ 1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * 32 * Dma<D>::UNITS / 64) : "memory");
+      dma_wait<2 * 32 * Dma<D>::UNITS / 64>();
       if (mask) lv.fetch(mask, k0 + 256, min(kend, k0 + 288), lane);
     } else {
       dma_wait();

@@ -163,32 +163,49 @@ struct Panel {
 };
 
 // Phi(z) and the density phi(z) of the normal distribution.  erfcx(x) = e^(x^2) erfc(x) is smooth:
-// t P(t) with t = 1 / (1 + 0.3 x) and a P of degree 8, fitted here by reweighted least squares
-// (Lawson) on x in [0, 14], is good to 4e-8 relative, and Phi(-|z|) = e^(-z^2 / 2) erfcx(|z| / sqrt
-// 2) / 2 keeps that in the tail, where 1 + erf would cancel.  The exponential is shared with phi;
-// its argument's rounding errors (up to 1e-5 of the result far out) are added back to first order.
+// t P(t) with t = 1 / (1 + c x) and polynomials P fitted here by reweighted least squares (Lawson),
+// and Phi(-|z|) = e^(-z^2 / 2) erfcx(|z| / sqrt 2) / 2 keeps their relative error in the tail, where
+// 1 + erf would cancel.  The exponential is shared with phi.
+// f32: degree 9 on x <= 14, 4e-8; the exponential's argument is rounded to 2^-24 of up to 100, which
+// is added back to first order.  16 bits: degree 6 on x <= 9.5, 5e-6 (half an ulp is 5e-4), no
+// corrections: the 16 384 x 4 096 epilogue is 67 M of these, 45 instructions each took 80 us.
+template <bool F32>
 __device__ __forceinline__ void normal(float z, float &cdf, float &pdf) {
-  const float q = z * z, qe = fmaf(z, z, -q);
-  const float a = q * -0.72134752044448170f, ae = fmaf(q, -0.72134752044448170f, -a);
-  float e = __builtin_amdgcn_exp2f(a);
-  e = fmaf(e, fmaf(ae, 0.69314718055994531f, qe * -0.5f), e);
-  if (!(q < 200.f)) e = q >= 200.f ? 0.f : q;    // (e is 0 from there on; NaN stays)
-  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, x, 1.f));
-  float p = -0.12661709327829032f;
-  p = fmaf(p, t, 0.4718284843770408f);
-  p = fmaf(p, t, -0.4846959475126719f);
-  p = fmaf(p, t, 0.5170530040780374f);
-  p = fmaf(p, t, -0.07405165572695369f);
-  p = fmaf(p, t, 0.20638609117498913f);
-  p = fmaf(p, t, 0.15046865829841485f);
-  p = fmaf(p, t, 0.1704237449651274f);
-  p = fmaf(p, t, 0.16920475194603254f);
-  const float half = 0.5f * e * (p * t);
+  const float q = z * z, az = __builtin_fabsf(z);
+  float e, half;
+  if (F32) {
+    const float qe = fmaf(z, z, -q);
+    const float a = q * -0.72134752044448170f, ae = fmaf(q, -0.72134752044448170f, -a);
+    e = __builtin_amdgcn_exp2f(a);
+    e = fmaf(e, fmaf(ae, 0.69314718055994531f, qe * -0.5f), e);
+    if (!(q < 200.f)) e = q >= 200.f ? 0.f : q;  // (e is 0 from there on; NaN stays)
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.21213203435596426f, az, 1.f));
+    float p = -0.12661709327829032f;
+    p = fmaf(p, t, 0.4718284843770408f);
+    p = fmaf(p, t, -0.4846959475126719f);
+    p = fmaf(p, t, 0.5170530040780374f);
+    p = fmaf(p, t, -0.07405165572695369f);
+    p = fmaf(p, t, 0.20638609117498913f);
+    p = fmaf(p, t, 0.15046865829841485f);
+    p = fmaf(p, t, 0.1704237449651274f);
+    p = fmaf(p, t, 0.16920475194603254f);
+    half = 0.5f * e * (p * t);
+  } else {                                       // (coefficients halved)
+    e = __builtin_amdgcn_exp2f(q * -0.72134752044448170f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.31112698372208094f, az, 1.f));
+    float p = -0.07305363353615859f;
+    p = fmaf(p, t, 0.17532868755186397f);
+    p = fmaf(p, t, 0.020362677464951965f);
+    p = fmaf(p, t, 0.1317947989864053f);
+    p = fmaf(p, t, 0.1212842819944461f);
+    p = fmaf(p, t, 0.12428055388327505f);
+    half = e * (p * t);
+  }
   cdf = z < 0.f ? half : 1.f - half;
   pdf = e * 0.39894228040143268f;
 }
 // act(z), and act'(z) into slope
+template <bool F32>
 __device__ __forceinline__ float activate(float z, int act, float &slope) {
   slope = 1.f;
   if (act == kActRelu) {
@@ -197,10 +214,10 @@ __device__ __forceinline__ float activate(float z, int act, float &slope) {
   }
   if (act == kActGelu) {
     float cdf, pdf;
-    normal(z, cdf, pdf);
-    const bool inf = __builtin_fabsf(z) == INFINITY;               // (inf * 0)
-    slope = inf ? cdf : fmaf(z, pdf, cdf);
-    return inf ? fmaxf(z, 0.f) : z * cdf;
+    normal<F32>(z, cdf, pdf);
+    const float far = __builtin_amdgcn_fmed3f(z, -1e4f, 1e4f);     // (the products of an infinity
+    slope = fmaf(z == z ? far : z, pdf, cdf);                      // with the 0 of its density)
+    return (z < 0.f ? far : z) * cdf;
   }
   return z;
 }
@@ -216,7 +233,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs &g, long long row, int c
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float d;
-    y[j] = (T)(activate(s[j] + (float)bias[j], g.act, d) + (float)res[j]);
+    y[j] = (T)(activate<sizeof(T) == 4>(s[j] + (float)bias[j], g.act, d) + (float)res[j]);
     slope[j] = (T)d;
   }
   if (g.slope) store_row((T *)g.slope + row * g.n, col, g.n, slope);
@@ -337,14 +354,15 @@ __global__ __launch_bounds__(256) void linear_gemm_kernel(GemmArgs g) {
                        split, lane);
 }
 
-// R rows (m / n axis) x 64 reduction steps of a 16-bit operand in LDS.  TR false: [R][64]; true:
-// [64][R] in blocks of 128 (or 64) columns.
+// R rows (m / n axis) x 32 reduction steps of a 16-bit operand in LDS.  TR false: [R][32]; true:
+// [32][R] in blocks of 128 (or 64) columns.
+constexpr int kStep = 32;
 template <typename T, bool TR, int R, int THREADS>
 struct DmaPanel {
-  static constexpr int D = TR ? (R >= 128 ? 128 : 64) : 64, BLOCKS = TR ? R / D : 1;
+  static constexpr int D = TR ? (R >= 128 ? 128 : 64) : kStep;
   typedef Dma<D> DM;
-  static constexpr int BLOCK = 64 * DM::PITCH, BYTES = R * 128;
-  static constexpr int N = R * 8 / THREADS;        // 16-byte units a thread moves
+  static constexpr int BLOCK = kStep * DM::PITCH, BYTES = R * kStep * 2;
+  static constexpr int N = BYTES / 16 / THREADS;   // 16-byte units a thread moves
   int off[N];                                      // byte offsets from the step's first element
   // k position of unit i inside a step (its row / its column)
   __device__ static __forceinline__ int kpos(int i, int tid) {
@@ -370,7 +388,7 @@ struct DmaPanel {
   __device__ __forceinline__ void issue(const T *src, long long ld, int k0, int kend, char *lds,
                                         int tid) const {
     const i32x4_t rs = dma_rsrc((const char *)(src + (TR ? k0 * ld : (long long)k0)), kFar);
-    if (k0 + 64 <= kend) {
+    if (k0 + kStep <= kend) {
 #pragma unroll
       for (int i = 0; i < N; ++i) dma16(rs, off[i], lds + (i * THREADS + (tid & ~63)) * 16);
     } else {
@@ -386,7 +404,8 @@ struct DmaPanel {
   __device__ static __forceinline__ typename Elem<T>::Vec frag(const char *lds, int base, int r0,
                                                                int ks) {
     if constexpr (!TR) {
-      return *reinterpret_cast<const typename Elem<T>::Vec *>(lds + r0 * 128 + (base ^ (ks << 5)));
+      return *reinterpret_cast<const typename Elem<T>::Vec *>(lds + r0 * DM::PITCH +
+                                                              (base ^ (ks << 5)));
     } else {
       union {
         s16x4_t s[2];
@@ -402,8 +421,13 @@ struct DmaPanel {
   }
 };
 
-// 16 bits: BM x BN tile by GM x GN waves, 64 reduction steps at a time, double-buffered by DMA: the
-// next step's tiles are asked for right behind the one barrier of a step
+// 16 bits: BM x BN tile by GM x GN waves, 32 reduction steps at a time through a ring of four tile
+// pairs that DMA fills three steps ahead (a step of the 256 x 256 tile is 1 024 cycles of products;
+// with two pairs of 64 steps, one ahead, memory's latency showed: 850 -> 1 0xx TFLOP/s).  A group of
+// 16 steps' fragments is read during the products of the group before, and the one barrier of a
+// step stands in front of its LAST group's products: every wave has then read all of this step's
+// tiles (refilled at once) and the next step's have landed, so no first fragments are waited for
+// with the matrix pipe idle.
 template <typename T, bool TA, bool TB, int BM, int BN, int GM, int GN>
 __global__ __launch_bounds__(64 * GM * GN, 2) void linear_dma_kernel(GemmArgs g) {
   constexpr int THREADS = 64 * GM * GN, WM = BM / GM, WN = BN / GN, IM = WM / 32, IN = WN / 32;
@@ -411,7 +435,8 @@ __global__ __launch_bounds__(64 * GM * GN, 2) void linear_dma_kernel(GemmArgs g)
   typedef DmaPanel<T, TB, BN, THREADS> PB;
   typedef typename Elem<T>::Vec Vec;
   constexpr int TILE = PA::BYTES + PB::BYTES, SLAB = GM * GN * 32 * (WN + 4) * 4;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * TILE > SLAB ? 2 * TILE : SLAB];
+  constexpr int NDMA = PA::N + PB::N;              // instructions a wave issues per step
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE > SLAB ? 4 * TILE : SLAB];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int m0, n0, split;
   place<BM, BN>(g, m0, n0, split);
@@ -430,32 +455,48 @@ __global__ __launch_bounds__(64 * GM * GN, 2) void linear_dma_kernel(GemmArgs g)
     pa.issue(ap, g.lda, k0, kend, smem + buf * TILE, tid);
     pb.issue(bp, g.ldb, k0, kend, smem + buf * TILE + PA::BYTES, tid);
   };
-  if (kbeg < kend) issue(kbeg, 0);
-  int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += 64) {
-    dma_wait();
-    lds_barrier();
-    if (k0 + 64 < kend) issue(k0 + 64, buf ^ 1);
+  Vec fa[2][IM], fb[2][IN];
+  auto load = [&](int buf, int ks) {
     const char *la = smem + buf * TILE, *lb = la + PA::BYTES;
-    buf ^= 1;
-    Vec fa[2][IM], fb[2][IN];
-    auto load = [&](int ks) {
 #pragma unroll
-      for (int i = 0; i < IM; ++i) fa[ks & 1][i] = PA::frag(la, ab, wm + 32 * i, ks);
+    for (int i = 0; i < IM; ++i) fa[ks][i] = PA::frag(la, ab, wm + 32 * i, ks);
 #pragma unroll
-      for (int j = 0; j < IN; ++j) fb[ks & 1][j] = PB::frag(lb, bb, wn + 32 * j, ks);
-    };
-    load(0);
+    for (int j = 0; j < IN; ++j) fb[ks][j] = PB::frag(lb, bb, wn + 32 * j, ks);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto products = [&](int ks) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      if (ks < 3) load(ks + 1);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < IM; ++i)
 #pragma unroll
-      for (int i = 0; i < IM; ++i)
-#pragma unroll
-        for (int j = 0; j < IN; ++j)
-          acc[i][j] = mfma(fa[ks & 1][i], fb[ks & 1][j], acc[i][j]);
+      for (int j = 0; j < IN; ++j) acc[i][j] = mfma(fa[ks][i], fb[ks][j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // waits for the step at k0 with the steps behind it in flight
+  auto arrived = [&](int k0) {
+    if (k0 + 2 * kStep < kend) dma_wait<2 * NDMA>();
+    else if (k0 + kStep < kend) dma_wait<NDMA>();
+    else dma_wait<0>();
+    lds_barrier();
+  };
+  for (int i = 0; i < 3; ++i)
+    if (kbeg + i * kStep < kend) issue(kbeg + i * kStep, i);
+  if (kbeg < kend) {
+    arrived(kbeg);
+    if (kbeg + 3 * kStep < kend) issue(kbeg + 3 * kStep, 3);
+    load(0, 0);
+  }
+  int buf = 0;
+  for (int k0 = kbeg; k0 < kend; k0 += kStep) {
+    load(buf, 1);
+    products(0);
+    const int next = (buf + 1) & 3;
+    if (k0 + kStep < kend) {
+      arrived(k0 + kStep);
+      if (k0 + 4 * kStep < kend) issue(k0 + 4 * kStep, buf);
+      load(next, 0);
     }
+    products(1);
+    buf = next;
   }
   __syncthreads();
   leave<T, IM, IN>(g, acc, reinterpret_cast<float *>(smem) + w * 32 * (WN + 4), m0 + wm, n0 + wn,
@@ -626,20 +667,32 @@ struct Plan {
   int bm, bn, mt, nt, nsplit, chunk;
 };
 
-// The largest tile that still gives every CU a workgroup; below that the smallest, and while its
-// tiles leave CUs idle the reduction is cut into shares of at least 256 steps.
+// Tile and shares of the reduction by estimated time: rounds of resident workgroups x (steps of 64 at
+// what one costs a full CU + what a workgroup costs besides), plus the partial sums' way through
+// memory.  us per step and per workgroup as measured for bf16: 256 x 256 tiles 0.95 and 6 (one per
+// CU), 128 x 128 0.75 and 3 (two), 64 x 64 0.5 and 2.5 (four).  (f32: no 256 x 256 tiles.)
 Plan plan_gemm(int m, int n, int k, bool dma) {
-  Plan p;
-  auto tiles = [&](int b) { return (long long)cdiv(m, b) * cdiv(n, b); };
-  p.bm = p.bn = dma && tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 64;
-  p.mt = cdiv(m, p.bm);
-  p.nt = cdiv(n, p.bn);
-  const long long t = (long long)p.mt * p.nt;
-  long long s = 1;
-  if (t < 256) s = std::max<long long>(1, std::min<long long>((512 + t - 1) / t, k / 256));
-  p.chunk = std::max(64, cdiv(cdiv(k, s), 64) * 64);
-  p.nsplit = std::max(1, cdiv(k, p.chunk));
-  return p;
+  static const struct { int b, per_cu; double step, fixed; } kTile[3] = {
+      {256, 1, 0.95, 6.0}, {128, 2, 0.75, 3.0}, {64, 4, 0.5, 2.5}};
+  Plan best{};
+  double least = 1e30;
+  for (int i = dma ? 0 : 1; i < 3; ++i) {
+    const auto &t = kTile[i];
+    const int mt = cdiv(m, t.b), nt = cdiv(n, t.b);
+    const long long tiles = (long long)mt * nt;
+    for (int s = 1; s <= 32 && (s == 1 || (k / s >= 128 && tiles * s <= 2048)); ++s) {
+      const int chunk = std::max(64, cdiv(cdiv(k, s), 64) * 64), real = std::max(1, cdiv(k, chunk));
+      if (real != s) continue;
+      double us = (double)((tiles * s + 256 * t.per_cu - 1) / (256 * t.per_cu)) *
+                  (chunk / 64 * t.step + t.fixed);
+      if (s > 1) us += 4.0 + (2.0 * s + 1.0) * m * n * 4.0 / 4e6;
+      if (us < least) {
+        least = us;
+        best = Plan{t.b, t.b, mt, nt, s, chunk};
+      }
+    }
+  }
+  return best;
 }
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 size_t split_bytes(int m, int n, int k, bool dma) {

@@ -93,8 +93,10 @@ def linear(x, weight, bias, act, residual, dy=None):
     pdf = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     if act == "relu":
         a, slope, ea = z.clamp(min=0), (z > 0).double(), ez
-    elif act == "gelu":                    # |gelu'| <= 1.13; the kernel's Phi is good to 40 f relative
-        a, slope, ea = z * cdf, cdf + z * pdf, 1.13 * ez + 40 * F * (z * cdf).abs()
+    elif act == "gelu":    # |gelu'| <= 1.13; the kernel's Phi: 40 f relative, for 16-bit types 2^-17 and
+        # the rounding of the exponential's argument z^2 / 2
+        a, slope = z * cdf, cdf + z * pdf
+        ea = 1.13 * ez + (40 * F if f32 else 2.0 ** -17 + z * z * F) * (z * cdf).abs()
     else:
         a, slope, ea = z, torch.ones_like(z), ez
     y = a if residual is None else a + residual.double().reshape(m, n)
@@ -107,7 +109,9 @@ def linear(x, weight, bias, act, residual, dy=None):
     if act == "relu":      # z within its error of zero may fall on either side
         edz = g.abs() * (z.abs() <= ez + tiny(dtype)).double()
     elif act == "gelu":    # the kept slope: half a step; |gelu''| <= 0.8; 2^-20 for its own arithmetic
-        edz = g.abs() * (u * slope.abs() + tiny(dtype) + 0.8 * ez + 2.0 ** -20) + u * dz.abs() + tiny(dtype)
+        # (16 bits: Phi <= 1 and z phi <= 0.25 to 2^-17)
+        own = 2.0 ** -20 if f32 else 2.0 ** -16
+        edz = g.abs() * (u * slope.abs() + tiny(dtype) + 0.8 * ez + own) + u * dz.abs() + tiny(dtype)
     else:
         edz = torch.zeros_like(g)
     dx, dw, db = dz @ W, dz.t() @ X, dz.sum(0)
