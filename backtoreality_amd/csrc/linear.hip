@@ -162,17 +162,21 @@ struct Panel {
   }
 };
 
-// Phi(z) and the density phi(z) of the normal distribution.  erfcx(x) = e^(x^2) erfc(x) is smooth:
-// t P(t) with t = 1 / (1 + c x) and polynomials P fitted here by reweighted least squares (Lawson),
-// and Phi(-|z|) = e^(-z^2 / 2) erfcx(|z| / sqrt 2) / 2 keeps their relative error in the tail, where
-// 1 + erf would cancel.  The exponential is shared with phi.
+// GELU and its slope through the normal distribution's tail h = Phi(-|z|) and density phi:
+//   z Phi(z) = max(z, 0) - |z| h,     (z Phi(z))' = [z > 0] + sign(z) (|z| phi(z) - h)
+// (no cancellation: h is small where the rest is).  erfcx(x) = e^(x^2) erfc(x) is smooth -- t P(t)
+// with t = 1 / (1 + c x) and polynomials P fitted here by reweighted least squares (Lawson) -- and h
+// = e^(-z^2 / 2) erfcx(|z| / sqrt 2) / 2 keeps its relative error in the tail; phi shares the
+// exponential.
 // f32: degree 9 on x <= 14, 4e-8; the exponential's argument is rounded to 2^-24 of up to 100, which
-// is added back to first order.  16 bits: degree 6 on x <= 9.5, 5e-6 (half an ulp is 5e-4), no
-// corrections: the 16 384 x 4 096 epilogue is 67 M of these, 45 instructions each took 80 us.
+// is added back to first order.  16 bits: degree 5 on x <= 9.5, 4e-5 (half an ulp is 5e-4 or more),
+// no corrections: the 67 M elements of 16 384 x 4 096 are 20 us of a full chip's VALU per 10
+// instructions.  |z| is cut at 30, where h and phi are 0, so that infinities meet no 0 times inf; NaN
+// comes through the exponential.
 template <bool F32>
-__device__ __forceinline__ void normal(float z, float &cdf, float &pdf) {
-  const float q = z * z, az = __builtin_fabsf(z);
-  float e, half;
+__device__ __forceinline__ float gelu(float z, float &slope) {
+  const float q = z * z, az = fminf(__builtin_fabsf(z), 30.f);
+  float e, h;
   if (F32) {
     const float qe = fmaf(z, z, -q);
     const float a = q * -0.72134752044448170f, ae = fmaf(q, -0.72134752044448170f, -a);
@@ -189,20 +193,21 @@ __device__ __forceinline__ void normal(float z, float &cdf, float &pdf) {
     p = fmaf(p, t, 0.15046865829841485f);
     p = fmaf(p, t, 0.1704237449651274f);
     p = fmaf(p, t, 0.16920475194603254f);
-    half = 0.5f * e * (p * t);
+    h = 0.5f * e * (p * t);
   } else {                                       // (coefficients halved)
     e = __builtin_amdgcn_exp2f(q * -0.72134752044448170f);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.31112698372208094f, az, 1.f));
-    float p = -0.07305363353615859f;
-    p = fmaf(p, t, 0.17532868755186397f);
-    p = fmaf(p, t, 0.020362677464951965f);
-    p = fmaf(p, t, 0.1317947989864053f);
-    p = fmaf(p, t, 0.1212842819944461f);
-    p = fmaf(p, t, 0.12428055388327505f);
-    half = e * (p * t);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.38183766184073570f, az, 1.f));
+    float p = -0.08940045184499485f;
+    p = fmaf(p, t, 0.18426239198220193f);
+    p = fmaf(p, t, 0.09526708661515707f);
+    p = fmaf(p, t, 0.15783040089614615f);
+    p = fmaf(p, t, 0.15202110402571496f);
+    h = e * (p * t);
   }
-  cdf = z < 0.f ? half : 1.f - half;
-  pdf = e * 0.39894228040143268f;
+  const float u = fmaf(az * 0.39894228040143268f, e, -h);
+  const int bits = __float_as_int(z);            // (the sign bit in both places: z = 0 either way)
+  slope = (bits >= 0 ? 1.f : 0.f) + __int_as_float(__float_as_int(u) ^ (bits & (int)0x80000000));
+  return fmaf(-az, h, fmaxf(z, 0.f));
 }
 // act(z), and act'(z) into slope
 template <bool F32>
@@ -212,24 +217,25 @@ __device__ __forceinline__ float activate(float z, int act, float &slope) {
     slope = z > 0.f ? 1.f : 0.f;
     return z > 0.f ? z : z != z ? z : 0.f;
   }
-  if (act == kActGelu) {
-    float cdf, pdf;
-    normal<F32>(z, cdf, pdf);
-    const float far = __builtin_amdgcn_fmed3f(z, -1e4f, 1e4f);     // (the products of an infinity
-    slope = fmaf(z == z ? far : z, pdf, cdf);                      // with the 0 of its density)
-    return (z < 0.f ? far : z) * cdf;
-  }
+  if (act == kActGelu) return gelu<F32>(z, slope);
   return z;
 }
 
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Vec bias_at(const GemmArgs &g, int col) {
+  return g.bias ? load_row((const T *)g.bias, col, g.n) : typename Elem<T>::Vec{};
+}
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Vec res_at(const GemmArgs &g, long long row, int col) {
+  return g.res ? load_row((const T *)g.res + row * g.ldres, col, g.n) : typename Elem<T>::Vec{};
+}
 // V consecutive columns of one row: bias, activation, residual, one rounding
 template <typename T>
 __device__ __forceinline__ void epilogue(const GemmArgs &g, long long row, int col,
-                                         const float (&s)[Elem<T>::kVec]) {
+                                         const float (&s)[Elem<T>::kVec],
+                                         typename Elem<T>::Vec bias, typename Elem<T>::Vec res) {
   constexpr int V = Elem<T>::kVec;
-  typename Elem<T>::Vec bias = {}, res = {}, slope, y;
-  if (g.bias) bias = load_row((const T *)g.bias, col, g.n);
-  if (g.res) res = load_row((const T *)g.res + row * g.ldres, col, g.n);
+  typename Elem<T>::Vec slope, y;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float d;
@@ -254,13 +260,27 @@ __device__ __forceinline__ void place(const GemmArgs &g, int &m0, int &n0, int &
   n0 = (in / bh) * BN;
 }
 
-// a wave's IM x IN accumulators leave through LDS, 32 rows at a time, as 16-byte row pieces
+// A wave's IM x IN accumulators leave through LDS, 32 rows at a time, as 16-byte row pieces.  A lane's
+// pieces all lie in the same columns: their bias is read once, and a slab's residuals before its
+// sums go through LDS (read piece by piece they cost a memory round trip each: 21 us a tile).
 template <typename T, int IM, int IN>
 __device__ __forceinline__ void leave(const GemmArgs &g, const f32x16_t (&acc)[IM][IN], float *slab,
                                       int row0, int col0, int split, int lane) {
-  constexpr int V = Elem<T>::kVec, WN = 32 * IN, CP = WN + 4, PR = WN / V;
+  constexpr int V = Elem<T>::kVec, WN = 32 * IN, CP = WN + 4, PR = WN / V, NQ = 32 * PR / 64;
+  static_assert(64 % PR == 0, "a lane keeps its columns");
+  typedef typename Elem<T>::Vec Vec;
+  const int col = (lane % PR) * V, gc = col0 + col;
+  const bool whole = g.nsplit == 1;
+  Vec bias = {}, res[NQ];
+  if (whole && gc < g.n) bias = bias_at<T>(g, gc);
 #pragma unroll
   for (int i = 0; i < IM; ++i) {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int gr = row0 + 32 * i + lane / PR + 64 / PR * q;
+      res[q] = Vec{};
+      if (whole && gr < g.m && gc < g.n) res[q] = res_at<T>(g, gr, gc);
+    }
 #pragma unroll
     for (int j = 0; j < IN; ++j)
 #pragma unroll
@@ -269,9 +289,8 @@ __device__ __forceinline__ void leave(const GemmArgs &g, const f32x16_t (&acc)[I
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int q = 0; q < 32 * PR / 64; ++q) {
-      const int e = lane + 64 * q, row = e / PR, col = (e % PR) * V;
-      const int gr = row0 + 32 * i + row, gc = col0 + col;
+    for (int q = 0; q < NQ; ++q) {
+      const int row = lane / PR + 64 / PR * q, gr = row0 + 32 * i + row;
       float s[V];
 #pragma unroll
       for (int u = 0; u < V; u += 4) {
@@ -280,13 +299,13 @@ __device__ __forceinline__ void leave(const GemmArgs &g, const f32x16_t (&acc)[I
         for (int x = 0; x < 4; ++x) s[u + x] = t[x];
       }
       if (gr < g.m && gc < g.n) {
-        if (g.nsplit > 1) {
+        if (whole) {
+          epilogue<T>(g, gr, gc, s, bias, res[q]);
+        } else {
           float *dst = g.part + ((long long)split * g.m + gr) * g.n;
 #pragma unroll
           for (int u = 0; u < V; u += 4)
             store_row(dst, gc + u, g.n, f32x4_t{s[u], s[u + 1], s[u + 2], s[u + 3]});
-        } else {
-          epilogue<T>(g, gr, gc, s);
         }
       }
     }
@@ -384,18 +403,14 @@ struct DmaPanel {
       }
     }
   }
-  // step at reduction index k0 of the operand at src (its first row / column already added)
-  __device__ __forceinline__ void issue(const T *src, long long ld, int k0, int kend, char *lds,
-                                        int tid) const {
-    const i32x4_t rs = dma_rsrc((const char *)(src + (TR ? k0 * ld : (long long)k0)), kFar);
-    if (k0 + kStep <= kend) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) dma16(rs, off[i], lds + (i * THREADS + (tid & ~63)) * 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        dma16(rs, k0 + kpos(i, tid) < kend ? off[i] : kFar, lds + (i * THREADS + (tid & ~63)) * 16);
-    }
+  // the descriptor of the step at reduction index k0 (src: the operand's first row / column added)
+  __device__ static __forceinline__ i32x4_t rsrc(const T *src, long long ld, int k0) {
+    return dma_rsrc((const char *)(src + (TR ? k0 * ld : (long long)k0)), kFar);
+  }
+  // unit i of a step that has `left` reduction steps (none: zeros); wave: tid / 64, uniform
+  __device__ __forceinline__ void issue(i32x4_t rs, int i, int left, char *lds, int tid,
+                                        int wave) const {
+    dma16(rs, kpos(i, tid) < left ? off[i] : kFar, lds + (i * THREADS + wave * 64) * 16);
   }
   // fragment: 32 rows at r0 (a multiple of 32), reduction steps 16 ks .. + 15; base: row_base / nat_base
   __device__ static __forceinline__ int base(int lane) {
@@ -421,23 +436,32 @@ struct DmaPanel {
   }
 };
 
-// 16 bits: BM x BN tile by GM x GN waves, 32 reduction steps at a time through a ring of four tile
-// pairs that DMA fills three steps ahead (a step of the 256 x 256 tile is 1 024 cycles of products;
-// with two pairs of 64 steps, one ahead, memory's latency showed: 850 -> 1 0xx TFLOP/s).  A group of
-// 16 steps' fragments is read during the products of the group before, and the one barrier of a
-// step stands in front of its LAST group's products: every wave has then read all of this step's
-// tiles (refilled at once) and the next step's have landed, so no first fragments are waited for
-// with the matrix pipe idle.
-template <typename T, bool TA, bool TB, int BM, int BN, int GM, int GN>
-__global__ __launch_bounds__(64 * GM * GN, 2) void linear_dma_kernel(GemmArgs g) {
+// 16 bits: BM x BN tile by GM x GN waves, 32 reduction steps at a time through a ring of NBUF tile
+// pairs that DMA fills NBUF - 1 steps ahead, always: steps past the end are filled with zeros, so that
+// the number of instructions in flight is a constant.  A group of 16 steps' fragments is read during
+// the products of the group before.  The one barrier of a step stands in front of its SECOND group's
+// products: every wave has then read all of this step's tiles (which are refilled during those
+// products) and the next step's have landed (its first fragments are read during them as well).
+// LDS reads and DMA instructions go out one between two products (in front of them they cost the
+// matrix pipe their own issue time), and a wave among its products goes before one that has still
+// to reach the barrier (s_setprio: 1 060 -> 1 170 TFLOP/s at 16 384 x 4 096 x 1 024 bf16).  The same
+// loop with neither DMA nor LDS reads runs at 1 450 TFLOP/s, which is the clock's doing; the DMA
+// costs 20 %, the reads 10 %.  256 x 256 tiles, a ring of four and one workgroup per CU for large
+// products; 256 x 128 with a ring of three fits a CU twice and wins only where the large tile leaves
+// CUs idle (8 192 x 4 096 x 1 024: 98 -> 79 us).
+template <typename T, bool TA, bool TB, int BM, int BN, int GM, int GN, int NBUF,
+          int OCC>
+__global__ __launch_bounds__(64 * GM * GN, OCC) void linear_dma_kernel(GemmArgs g) {
   constexpr int THREADS = 64 * GM * GN, WM = BM / GM, WN = BN / GN, IM = WM / 32, IN = WN / 32;
   typedef DmaPanel<T, TA, BM, THREADS> PA;
   typedef DmaPanel<T, TB, BN, THREADS> PB;
   typedef typename Elem<T>::Vec Vec;
   constexpr int TILE = PA::BYTES + PB::BYTES, SLAB = GM * GN * 32 * (WN + 4) * 4;
   constexpr int NDMA = PA::N + PB::N;              // instructions a wave issues per step
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE > SLAB ? 4 * TILE : SLAB];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  constexpr int NF = IM + IN, NP = IM * IN;        // fragments and products of a group
+  constexpr int LQ = (NF + NP - 1) / NP, DQ = (NDMA + NP - 1) / NP;   // between two products, at most
+  __shared__ __attribute__((aligned(1024))) char smem[NBUF * TILE > SLAB ? NBUF * TILE : SLAB];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   int m0, n0, split;
   place<BM, BN>(g, m0, n0, split);
   const int kbeg = split * g.chunk, kend = min(g.k, kbeg + g.chunk);
@@ -451,53 +475,59 @@ __global__ __launch_bounds__(64 * GM * GN, 2) void linear_dma_kernel(GemmArgs g)
   const int ab = PA::base(lane), bb = PB::base(lane);
 
   f32x16_t acc[IM][IN] = {};
-  auto issue = [&](int k0, int buf) {
-    pa.issue(ap, g.lda, k0, kend, smem + buf * TILE, tid);
-    pb.issue(bp, g.ldb, k0, kend, smem + buf * TILE + PA::BYTES, tid);
-  };
   Vec fa[2][IM], fb[2][IN];
-  auto load = [&](int buf, int ks) {
+  auto load = [&](int buf, int ks, int i) {        // fragment i of a group
     const char *la = smem + buf * TILE, *lb = la + PA::BYTES;
-#pragma unroll
-    for (int i = 0; i < IM; ++i) fa[ks][i] = PA::frag(la, ab, wm + 32 * i, ks);
-#pragma unroll
-    for (int j = 0; j < IN; ++j) fb[ks][j] = PB::frag(lb, bb, wn + 32 * j, ks);
-    __builtin_amdgcn_sched_barrier(0);
+    if (i < IM) fa[ks][i] = PA::frag(la, ab, wm + 32 * i, ks);
+    else fb[ks][i - IM] = PB::frag(lb, bb, wn + 32 * (i - IM), ks);
   };
-  auto products = [&](int ks) {
-#pragma unroll
-    for (int i = 0; i < IM; ++i)
-#pragma unroll
-      for (int j = 0; j < IN; ++j) acc[i][j] = mfma(fa[ks][i], fb[ks][j], acc[i][j]);
-    __builtin_amdgcn_sched_barrier(0);
+  i32x4_t ra, rb;
+  auto issue = [&](int k0, int buf, int i) {       // DMA instruction i of a step
+    char *la = smem + buf * TILE;
+    if (i == 0) ra = PA::rsrc(ap, g.lda, k0);
+    if (i == PA::N) rb = PB::rsrc(bp, g.ldb, k0);
+    if (i < PA::N) pa.issue(ra, i, kend - k0, la, tid, w);
+    else pb.issue(rb, i - PA::N, kend - k0, la + PA::BYTES, tid, w);
   };
-  // waits for the step at k0 with the steps behind it in flight
-  auto arrived = [&](int k0) {
-    if (k0 + 2 * kStep < kend) dma_wait<2 * NDMA>();
-    else if (k0 + kStep < kend) dma_wait<NDMA>();
-    else dma_wait<0>();
-    lds_barrier();
-  };
-  for (int i = 0; i < 3; ++i)
-    if (kbeg + i * kStep < kend) issue(kbeg + i * kStep, i);
   if (kbeg < kend) {
-    arrived(kbeg);
-    if (kbeg + 3 * kStep < kend) issue(kbeg + 3 * kStep, 3);
-    load(0, 0);
+#pragma unroll
+    for (int t = 0; t < NBUF - 1; ++t)
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) issue(kbeg + t * kStep, t, i);
+    dma_wait<(NBUF - 2) * NDMA>();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < NDMA; ++i) issue(kbeg + (NBUF - 1) * kStep, NBUF - 1, i);
+#pragma unroll
+    for (int i = 0; i < NF; ++i) load(0, 0, i);
   }
   int buf = 0;
   for (int k0 = kbeg; k0 < kend; k0 += kStep) {
-    load(buf, 1);
-    products(0);
-    const int next = (buf + 1) & 3;
-    if (k0 + kStep < kend) {
-      arrived(k0 + kStep);
-      if (k0 + 4 * kStep < kend) issue(k0 + 4 * kStep, buf);
-      load(next, 0);
+    const int next = buf + 1 == NBUF ? 0 : buf + 1;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      if (q == 0) __builtin_amdgcn_s_setprio(1);
+      acc[q / IN][q % IN] = mfma(fa[0][q / IN], fb[0][q % IN], acc[q / IN][q % IN]);
+#pragma unroll
+      for (int i = q * LQ; i < NF && i < (q + 1) * LQ; ++i) load(buf, 1, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    products(1);
+    __builtin_amdgcn_s_setprio(0);
+    dma_wait<(NBUF - 2) * NDMA>();
+    lds_barrier();
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      if (q == 0) __builtin_amdgcn_s_setprio(1);
+      acc[q / IN][q % IN] = mfma(fa[1][q / IN], fb[1][q % IN], acc[q / IN][q % IN]);
+#pragma unroll
+      for (int i = q * LQ; i < NF && i < (q + 1) * LQ; ++i) load(next, 0, i);
+#pragma unroll
+      for (int i = q * DQ; i < NDMA && i < (q + 1) * DQ; ++i) issue(k0 + NBUF * kStep, buf, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     buf = next;
   }
+  dma_wait();
   __syncthreads();
   leave<T, IM, IN>(g, acc, reinterpret_cast<float *>(smem) + w * 32 * (WN + 4), m0 + wm, n0 + wn,
                    split, lane);
@@ -561,7 +591,7 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(GemmArgs g) {
     for (int k = 0; k < 8; ++k)
 #pragma unroll
       for (int u = 0; u < V; ++u) s[u] += part[k][row >> 4][row & 15][col + u];
-    epilogue<T>(g, row, n0 + col, s);
+    epilogue<T>(g, row, n0 + col, s, bias_at<T>(g, n0 + col), res_at<T>(g, row, n0 + col));
   }
 }
 
@@ -599,7 +629,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(GemmArgs g) {
         for (int i = 0; i < 4; ++i) s[u + i] += q[i];
       }
     }
-    epilogue<T>(g, row, col, s);
+    epilogue<T>(g, row, col, s, bias_at<T>(g, col), res_at<T>(g, row, col));
   }
 }
 
@@ -667,28 +697,30 @@ struct Plan {
   int bm, bn, mt, nt, nsplit, chunk;
 };
 
-// Tile and shares of the reduction by estimated time: rounds of resident workgroups x (steps of 64 at
-// what one costs a full CU + what a workgroup costs besides), plus the partial sums' way through
-// memory.  us per step and per workgroup as measured for bf16: 256 x 256 tiles 0.95 and 6 (one per
-// CU), 128 x 128 0.75 and 3 (two), 64 x 64 0.5 and 2.5 (four).  (f32: no 256 x 256 tiles.)
+// Tile and shares of the reduction by estimated time: workgroups a CU gets x (64-step pieces x what
+// one costs + what a workgroup costs besides), not below one workgroup's own latency, plus the
+// partial sums' way through memory.  The figures are us, measured for bf16 at 16 384 x 4 096 x 1 024
+// and 16 384 x 1 024 x 4 096 with each tile in turn.  (f32 has the two small tiles.)
 Plan plan_gemm(int m, int n, int k, bool dma) {
-  static const struct { int b, per_cu; double step, fixed; } kTile[3] = {
-      {256, 1, 0.95, 6.0}, {128, 2, 0.75, 3.0}, {64, 4, 0.5, 2.5}};
+  static const struct { int bm, bn; double step, fixed, alone; } kTile[4] = {
+      {256, 256, 1.65, 11.0, 1.65}, {256, 128, 1.02, 6.7, 1.02}, {128, 128, 0.6, 3.4, 0.75},
+      {64, 64, 0.26, 1.3, 0.45}};
   Plan best{};
   double least = 1e30;
-  for (int i = dma ? 0 : 1; i < 3; ++i) {
+  for (int i = dma ? 0 : 2; i < 4; ++i) {
     const auto &t = kTile[i];
-    const int mt = cdiv(m, t.b), nt = cdiv(n, t.b);
+    const int mt = cdiv(m, t.bm), nt = cdiv(n, t.bn);
     const long long tiles = (long long)mt * nt;
     for (int s = 1; s <= 32 && (s == 1 || (k / s >= 128 && tiles * s <= 2048)); ++s) {
       const int chunk = std::max(64, cdiv(cdiv(k, s), 64) * 64), real = std::max(1, cdiv(k, chunk));
       if (real != s) continue;
-      double us = (double)((tiles * s + 256 * t.per_cu - 1) / (256 * t.per_cu)) *
-                  (chunk / 64 * t.step + t.fixed);
+      const double steps = chunk / 64;
+      double us = std::max((double)((tiles * s + 255) / 256) * (steps * t.step + t.fixed),
+                           steps * t.alone + t.fixed);
       if (s > 1) us += 4.0 + (2.0 * s + 1.0) * m * n * 4.0 / 4e6;
       if (us < least) {
         least = us;
-        best = Plan{t.b, t.b, mt, nt, s, chunk};
+        best = Plan{t.bm, t.bn, mt, nt, s, chunk};
       }
     }
   }
@@ -736,12 +768,14 @@ void launch_gemm(GemmArgs g, void *ws, hipStream_t hs) {
   g.mt = p.mt; g.nt = p.nt; g.nsplit = p.nsplit; g.chunk = p.chunk; g.part = (float *)ws;
   const dim3 grid((unsigned)((long long)p.mt * p.nt * p.nsplit));
   if constexpr (DMA) {
-    if (p.bm == 256)
-      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 256, 2, 4>), grid, dim3(512), 0, hs, g);
+    if (p.bm == 256 && p.bn == 128)
+      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 128, 4, 2, 3, 4>), grid, dim3(512), 0, hs, g);
+    else if (p.bm == 256)
+      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 256, 2, 4, 4, 2>), grid, dim3(512), 0, hs, g);
     else if (p.bm == 128)
-      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 128, 128, 2, 2>), grid, dim3(256), 0, hs, g);
+      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 128, 128, 2, 2, 4, 2>), grid, dim3(256), 0, hs, g);
     else
-      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 64, 64, 2, 2>), grid, dim3(256), 0, hs, g);
+      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 64, 64, 2, 2, 4, 2>), grid, dim3(256), 0, hs, g);
   } else {
     if (p.bm == 128)
       hipLaunchKernelGGL((linear_gemm_kernel<TA, TB, 128, 128>), grid, dim3(256), 0, hs, g);

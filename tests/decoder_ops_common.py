@@ -93,10 +93,11 @@ def linear(x, weight, bias, act, residual, dy=None):
     pdf = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     if act == "relu":
         a, slope, ea = z.clamp(min=0), (z > 0).double(), ez
-    elif act == "gelu":    # |gelu'| <= 1.13; the kernel's Phi: 40 f relative, for 16-bit types 2^-17 and
-        # the rounding of the exponential's argument z^2 / 2
+    elif act == "gelu":    # |gelu'| <= 1.13; the kernel's tail Phi(-|z|): 40 f relative, for 16-bit types
+        # 2^-14 (the fit's 4e-5, and f z^2 for the exponential's argument); gelu = max(z, 0) - |z| Phi(-|z|)
         a, slope = z * cdf, cdf + z * pdf
-        ea = 1.13 * ez + (40 * F if f32 else 2.0 ** -17 + z * z * F) * (z * cdf).abs()
+        tail = torch.special.erfc(z.abs() / math.sqrt(2)) / 2
+        ea = 1.13 * ez + (40 * F if f32 else 2.0 ** -14 + z * z * F) * z.abs() * tail + 2 * F * a.abs()
     else:
         a, slope, ea = z, torch.ones_like(z), ez
     y = a if residual is None else a + residual.double().reshape(m, n)
@@ -109,8 +110,8 @@ def linear(x, weight, bias, act, residual, dy=None):
     if act == "relu":      # z within its error of zero may fall on either side
         edz = g.abs() * (z.abs() <= ez + tiny(dtype)).double()
     elif act == "gelu":    # the kept slope: half a step; |gelu''| <= 0.8; 2^-20 for its own arithmetic
-        # (16 bits: Phi <= 1 and z phi <= 0.25 to 2^-17)
-        own = 2.0 ** -20 if f32 else 2.0 ** -16
+        # (16 bits: the tail, at most a half, to 2^-14)
+        own = 2.0 ** -20 if f32 else 2.0 ** -15
         edz = g.abs() * (u * slope.abs() + tiny(dtype) + 0.8 * ez + own) + u * dz.abs() + tiny(dtype)
     else:
         edz = torch.zeros_like(g)
