@@ -10,15 +10,15 @@
 // The three products differ in whether the reduction runs along a row of the operand (x, W forward,
 // dz for dx) or across its rows (W for dx; dz and x for dW).  Both kinds are staged the way memory
 // has them and the second is read out of LDS with gfx950's transpose read, so nothing is ever
-// transposed in memory.  16-bit operands go to LDS by DMA (linear_dma_kernel); rows that do not lie
-// on 16-byte boundaries in whole 16-byte units are first copied to rows that do, in the workspace.
-// f32 operands pass through registers, where they are split (linear_gemm_kernel).  Few rows
-// (single tokens) read W once, straight into the matrix instructions (linear_rows_kernel).
+// transposed in memory.  Operands go to LDS by DMA (linear_dma_kernel); 16-bit rows that do not lie
+// on 16-byte boundaries in whole 16-byte units are first copied to rows that do, in the workspace,
+// f32 ones are split into three bf16 planes there.  Few rows (single tokens) read W once, straight
+// into the matrix instructions (linear_rows_kernel).
 //
 // Numbers: every product accumulates in f32 and the epilogue works on the f32 sums; y is rounded
 // once.  f32 operands are split into three bf16 terms (8 + 8 + 8 bits: exact up to the 24th) and
-// multiplied as the six products above 2^-24, which the bf16 matrix pipe does 2.7 times faster
-// than the f32 instructions do one; an infinite f32 element makes the sums it enters NaN.  What the
+// multiplied as the six products above 2^-24, the smallest first, as one reduction six times as
+// long, which the bf16 matrix pipe does 2.7 times faster than the f32 instructions do one; an infinite f32 element makes the sums it enters NaN.  What the
 // backward needs of the activation is its slope act'(z), taken from the f32 sum in the forward's
 // epilogue and kept in the type of x (half an ulp; 0 and 1 of ReLU are exact); dz is rounded to the
 // type of x as well before the two products that read it.
@@ -46,6 +46,7 @@ struct GemmArgs {
   void *c, *slope;           // contiguous (m, n); slope: act' of the sums, or NULL
   float *part;               // split reduction: (nsplit, m, n) partial sums
   int nsplit, chunk;         // shares of k, their length
+  long long aplane, bplane;  // f32: elements from one bf16 plane of an operand to the next
   int mt, nt;                // tiles
 };
 
@@ -59,6 +60,15 @@ template <>
 struct Op<float> {
   static constexpr int P = 3;
   typedef bf16x8_t Frag;
+};
+
+template <typename T>
+struct Matrix {
+  typedef T E;
+};
+template <>
+struct Matrix<float> {
+  typedef __bf16 E;
 };
 
 __device__ __forceinline__ f32x16_t mfma(bf16x8_t a, bf16x8_t b, f32x16_t c) {
@@ -99,68 +109,6 @@ __device__ __forceinline__ void pack(const f32x4_t (&v)[2], bf16x8_t (&f)[3]) {
   for (int p = 0; p < 3; ++p)
     f[p] = __builtin_shufflevector(a[p], b[p], 0, 1, 2, 3, 4, 5, 6, 7);
 }
-
-// f32: R rows of the operand (its m or n axis) x BK of the reduction, in LDS as three bf16 planes.  TR false: [R][BK], read
-// as rows; true: [BK][R], read transposed.  Row pitches: an odd number of 16-byte units (sixteen
-// rows at one column: distinct banks) / 64 mod 256 bytes (four rows x 64 bytes: distinct banks).
-template <bool TR, int R, int BK>
-struct Panel {
-  static constexpr int P = 3, V = 4;
-  static constexpr int ROWS = TR ? BK : R, COLS = TR ? R : BK;
-  static constexpr int PITCH = TR ? (R * 2 / 256) * 256 + (R * 2 % 256 <= 64 ? 64 : R * 2 % 256 <= 192 ? 192 : 320)
-                                  : COLS * 2 + 16;
-  static constexpr int PLANE = ROWS * PITCH, BYTES = P * PLANE;
-  static constexpr int PER_ROW = COLS / V, N = ROWS * PER_ROW / 256;
-  static_assert(ROWS * PER_ROW % 256 == 0, "whole vectors per thread");
-  static_assert(!TR || (PITCH >= R * 2 && (PITCH % 256 == 64 || PITCH % 256 == 192)), "pitch");
-  f32x4_t r[N];
-
-  // r0: first index of the operand's m / n axis, k0: of the reduction; beyond rmax / kmax zeros
-  __device__ __forceinline__ void fetch(const float *src, long long ld, int r0, int rmax, int k0,
-                                        int kmax, int tid) {
-    const int row0 = TR ? k0 : r0, col0 = TR ? r0 : k0, rows = TR ? kmax : rmax,
-              cols = TR ? rmax : kmax;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = tid + 256 * i, row = row0 + e / PER_ROW, col = col0 + (e % PER_ROW) * V;
-      r[i] = f32x4_t{};
-      if (row < rows && col < cols) r[i] = load_row(src + row * ld, col, cols);
-    }
-  }
-  __device__ __forceinline__ void store(char *lds, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = tid + 256 * i;
-      char *p = lds + (e / PER_ROW) * PITCH + (e % PER_ROW) * V * 2;
-      bf16x4_t q[3];
-      split3(r[i], q);
-#pragma unroll
-      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x4_t *>(p + j * PLANE) = q[j];
-    }
-  }
-  // fragment of the 32 rows at r0 and the 16 reduction steps at ks
-  __device__ static __forceinline__ bf16x8_t frag(const char *lds, int plane, int r0,
-                                                              int ks, int lane) {
-    const char *t = lds + plane * PLANE;
-    if constexpr (!TR) {
-      return *reinterpret_cast<const bf16x8_t *>(
-          t + (r0 + (lane & 31)) * PITCH + (ks + 8 * (lane >> 5)) * 2);
-    } else {
-      // lane p of a group of 16 addresses row p / 4, columns 4 (p % 4) .. + 3 of a [4][16] block and
-      // receives column p, rows 0 .. 3
-      const int p = lane & 15;
-      const char *q = t + (ks + 8 * (lane >> 5) + (p >> 2)) * PITCH +
-                      (r0 + 16 * ((lane >> 4) & 1) + 4 * (p & 3)) * 2;
-      union {
-        s16x4_t s[2];
-        bf16x8_t f;
-      } u;
-      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q);
-      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 4 * PITCH));
-      return u.f;
-    }
-  }
-};
 
 // GELU and its slope through the normal distribution's tail h = Phi(-|z|) and density phi:
 //   z Phi(z) = max(z, 0) - |z| h,     (z Phi(z))' = [z > 0] + sign(z) (|z| phi(z) - h)
@@ -314,65 +262,6 @@ __device__ __forceinline__ void leave(const GemmArgs &g, const f32x16_t (&acc)[I
   }
 }
 
-// f32: BM x BN tile by four waves (2 x 2), 32 reduction steps at a time, the next in registers
-template <bool TA, bool TB, int BM, int BN>
-__global__ __launch_bounds__(256) void linear_gemm_kernel(GemmArgs g) {
-  constexpr int BK = 32, WM = BM / 2, WN = BN / 2, IM = WM / 32, IN = WN / 32;
-  typedef Panel<TA, BM, BK> PA;
-  typedef Panel<TB, BN, BK> PB;
-  constexpr int SLAB = 4 * 32 * (WN + 4) * 4, TILE = PA::BYTES + PB::BYTES;
-  __shared__ __attribute__((aligned(16))) char smem[TILE > SLAB ? TILE : SLAB];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  int m0, n0, split;
-  place<BM, BN>(g, m0, n0, split);
-  const int kbeg = split * g.chunk, kend = min(g.k, kbeg + g.chunk);
-  const int wm = (w >> 1) * WM, wn = (w & 1) * WN;
-
-  f32x16_t acc[IM][IN] = {};
-  PA pa;
-  PB pb;
-  char *la = smem, *lb = smem + PA::BYTES;
-  if (kbeg < kend) {
-    pa.fetch((const float *)g.a, g.lda, m0, g.m, kbeg, kend, tid);
-    pb.fetch((const float *)g.b, g.ldb, n0, g.n, kbeg, kend, tid);
-  }
-  for (int k0 = kbeg; k0 < kend; k0 += BK) {
-    lds_barrier();                                 // the previous step's reads are done
-    pa.store(la, tid);
-    pb.store(lb, tid);
-    if (k0 + BK < kend) {
-      pa.fetch((const float *)g.a, g.lda, m0, g.m, k0 + BK, kend, tid);
-      pb.fetch((const float *)g.b, g.ldb, n0, g.n, k0 + BK, kend, tid);
-    }
-    lds_barrier();
-#pragma unroll
-    for (int ks = 0; ks < BK; ks += 16) {
-      bf16x8_t fa[IM][3], fb[IN][3];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-#pragma unroll
-        for (int i = 0; i < IM; ++i) fa[i][p] = PA::frag(la, p, wm + 32 * i, ks, lane);
-#pragma unroll
-        for (int j = 0; j < IN; ++j) fb[j][p] = PB::frag(lb, p, wn + 32 * j, ks, lane);
-      }
-#pragma unroll
-      for (int i = 0; i < IM; ++i)
-#pragma unroll
-        for (int j = 0; j < IN; ++j) {             // smallest terms first
-          acc[i][j] = mfma(fa[i][2], fb[j][0], acc[i][j]);
-          acc[i][j] = mfma(fa[i][0], fb[j][2], acc[i][j]);
-          acc[i][j] = mfma(fa[i][1], fb[j][1], acc[i][j]);
-          acc[i][j] = mfma(fa[i][1], fb[j][0], acc[i][j]);
-          acc[i][j] = mfma(fa[i][0], fb[j][1], acc[i][j]);
-          acc[i][j] = mfma(fa[i][0], fb[j][0], acc[i][j]);
-        }
-    }
-  }
-  __syncthreads();
-  leave<float, IM, IN>(g, acc, reinterpret_cast<float *>(smem) + w * 32 * (WN + 4), m0 + wm, n0 + wn,
-                       split, lane);
-}
-
 // R rows (m / n axis) x 32 reduction steps of a 16-bit operand in LDS.  TR false: [R][32]; true:
 // [32][R] in blocks of 128 (or 64) columns.
 constexpr int kStep = 32;
@@ -449,25 +338,30 @@ struct DmaPanel {
 // costs 20 %, the reads 10 %.  256 x 256 tiles, a ring of four and one workgroup per CU for large
 // products; 256 x 128 with a ring of three fits a CU twice and wins only where the large tile leaves
 // CUs idle (8 192 x 4 096 x 1 024: 98 -> 79 us).
-template <typename T, bool TA, bool TB, int BM, int BN, int GM, int GN, int NBUF,
-          int OCC>
+// f32 (T): the operands are bf16 planes (E), the reduction runs six times over k with the planes of
+// kPlanes.
+constexpr unsigned kPlanesA = 0x001102, kPlanesB = 0x010120;   // digit i: plane of the i-th pass
+template <typename T, bool TA, bool TB, int BM, int BN, int GM, int GN, int NBUF, int OCC>
 __global__ __launch_bounds__(64 * GM * GN, OCC) void linear_dma_kernel(GemmArgs g) {
+  typedef typename Matrix<T>::E E;
   constexpr int THREADS = 64 * GM * GN, WM = BM / GM, WN = BN / GN, IM = WM / 32, IN = WN / 32;
-  typedef DmaPanel<T, TA, BM, THREADS> PA;
-  typedef DmaPanel<T, TB, BN, THREADS> PB;
-  typedef typename Elem<T>::Vec Vec;
+  typedef DmaPanel<E, TA, BM, THREADS> PA;
+  typedef DmaPanel<E, TB, BN, THREADS> PB;
+  typedef typename Elem<E>::Vec Vec;
   constexpr int TILE = PA::BYTES + PB::BYTES, SLAB = GM * GN * 32 * (WN + 4) * 4;
   constexpr int NDMA = PA::N + PB::N;              // instructions a wave issues per step
   constexpr int NF = IM + IN, NP = IM * IN;        // fragments and products of a group
   constexpr int LQ = (NF + NP - 1) / NP, DQ = (NDMA + NP - 1) / NP;   // between two products, at most
+  constexpr int PASSES = sizeof(T) == 4 ? 6 : 1;
   __shared__ __attribute__((aligned(1024))) char smem[NBUF * TILE > SLAB ? NBUF * TILE : SLAB];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   int m0, n0, split;
   place<BM, BN>(g, m0, n0, split);
   const int kbeg = split * g.chunk, kend = min(g.k, kbeg + g.chunk);
+  const int nk = kend > kbeg ? (kend - kbeg + kStep - 1) / kStep : 0, steps = nk * PASSES;
   const int wm = w / GN * WM, wn = w % GN * WN;
-  const T *ap = (const T *)g.a + (TA ? (long long)m0 : m0 * g.lda);
-  const T *bp = (const T *)g.b + (TB ? (long long)n0 : n0 * g.ldb);
+  const E *ap = (const E *)g.a + (TA ? (long long)m0 : m0 * g.lda);
+  const E *bp = (const E *)g.b + (TB ? (long long)n0 : n0 * g.ldb);
   PA pa;
   PB pb;
   pa.init(g.lda, m0, g.m, tid);
@@ -482,27 +376,35 @@ __global__ __launch_bounds__(64 * GM * GN, OCC) void linear_dma_kernel(GemmArgs 
     else fb[ks][i - IM] = PB::frag(lb, bb, wn + 32 * (i - IM), ks);
   };
   i32x4_t ra, rb;
-  auto issue = [&](int k0, int buf, int i) {       // DMA instruction i of a step
+  int ik = 0, pass = 0;                            // the next step to be asked for
+  auto issue = [&](int buf, int i) {               // DMA instruction i of it
     char *la = smem + buf * TILE;
-    if (i == 0) ra = PA::rsrc(ap, g.lda, k0);
-    if (i == PA::N) rb = PB::rsrc(bp, g.ldb, k0);
-    if (i < PA::N) pa.issue(ra, i, kend - k0, la, tid, w);
-    else pb.issue(rb, i - PA::N, kend - k0, la + PA::BYTES, tid, w);
+    const int k0 = kbeg + ik * kStep, left = pass < PASSES ? kend - k0 : 0;
+    if (i == 0)
+      ra = PA::rsrc(ap + (PASSES > 1 ? (kPlanesA >> (4 * pass) & 15) * g.aplane : 0), g.lda, k0);
+    if (i == PA::N)
+      rb = PB::rsrc(bp + (PASSES > 1 ? (kPlanesB >> (4 * pass) & 15) * g.bplane : 0), g.ldb, k0);
+    if (i < PA::N) pa.issue(ra, i, left, la, tid, w);
+    else pb.issue(rb, i - PA::N, left, la + PA::BYTES, tid, w);
+    if (i == NDMA - 1 && ++ik >= nk) {
+      ik = 0;
+      ++pass;
+    }
   };
-  if (kbeg < kend) {
+  if (steps) {
 #pragma unroll
     for (int t = 0; t < NBUF - 1; ++t)
 #pragma unroll
-      for (int i = 0; i < NDMA; ++i) issue(kbeg + t * kStep, t, i);
+      for (int i = 0; i < NDMA; ++i) issue(t, i);
     dma_wait<(NBUF - 2) * NDMA>();
     lds_barrier();
 #pragma unroll
-    for (int i = 0; i < NDMA; ++i) issue(kbeg + (NBUF - 1) * kStep, NBUF - 1, i);
+    for (int i = 0; i < NDMA; ++i) issue(NBUF - 1, i);
 #pragma unroll
     for (int i = 0; i < NF; ++i) load(0, 0, i);
   }
   int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += kStep) {
+  for (int step = 0; step < steps; ++step) {
     const int next = buf + 1 == NBUF ? 0 : buf + 1;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
@@ -522,7 +424,7 @@ __global__ __launch_bounds__(64 * GM * GN, OCC) void linear_dma_kernel(GemmArgs 
 #pragma unroll
       for (int i = q * LQ; i < NF && i < (q + 1) * LQ; ++i) load(next, 0, i);
 #pragma unroll
-      for (int i = q * DQ; i < NDMA && i < (q + 1) * DQ; ++i) issue(k0 + NBUF * kStep, buf, i);
+      for (int i = q * DQ; i < NDMA && i < (q + 1) * DQ; ++i) issue(buf, i);
       __builtin_amdgcn_sched_barrier(0);
     }
     buf = next;
@@ -531,6 +433,131 @@ __global__ __launch_bounds__(64 * GM * GN, OCC) void linear_dma_kernel(GemmArgs 
   __syncthreads();
   leave<T, IM, IN>(g, acc, reinterpret_cast<float *>(smem) + w * 32 * (WN + 4), m0 + wm, n0 + wn,
                    split, lane);
+}
+
+// Small products: a 64 x 64 tile whose reduction steps the four waves deal out among themselves (wave
+// w: steps w, w + 4, ..), each through two tile pairs of its own, without a barrier until their sums
+// meet in LDS.  A product of few tiles is bound by the latency of its chain of steps: with the tile
+// cut into 32 x 32 per wave (one product between two LDS round trips and a barrier) a step took 0.45
+// us, here a wave's step is eight products behind one round trip and four run at once.  (Rings of
+// four fit a CU once: 1 024 x 2 048 outputs, 128 / 1 024 steps 9.9 / 14.6 us against 6.9 / 12.1.)
+template <typename T, bool TA, bool TB>
+__global__ __launch_bounds__(256) void linear_stream_kernel(GemmArgs g) {
+  typedef typename Matrix<T>::E E;
+  typedef DmaPanel<E, TA, 64, 64> PA;
+  typedef DmaPanel<E, TB, 64, 64> PB;
+  typedef typename Elem<E>::Vec Vec;
+  constexpr int TILE = PA::BYTES + PB::BYTES, NDMA = PA::N + PB::N, CP = 64 + 4;
+  constexpr int PASSES = sizeof(T) == 4 ? 6 : 1, SUMS = 4 * 64 * CP * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[8 * TILE > SUMS ? 8 * TILE : SUMS];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int m0, n0, split;
+  place<64, 64>(g, m0, n0, split);
+  const int kbeg = split * g.chunk, kend = min(g.k, kbeg + g.chunk);
+  const int nk = kend > kbeg ? (kend - kbeg + kStep - 1) / kStep : 0, steps = nk * PASSES;
+  const E *ap = (const E *)g.a + (TA ? (long long)m0 : m0 * g.lda);
+  const E *bp = (const E *)g.b + (TB ? (long long)n0 : n0 * g.ldb);
+  PA pa;
+  PB pb;
+  pa.init(g.lda, m0, g.m, lane);
+  pb.init(g.ldb, n0, g.n, lane);
+  const int ab = PA::base(lane), bb = PB::base(lane);
+  char *ring = smem + w * 2 * TILE;
+
+  f32x16_t acc[2][2] = {};
+  int ik = w, pass = 0;                            // the next step to be asked for
+  while (nk && ik >= nk && pass < PASSES) {
+    ik -= nk;
+    ++pass;
+  }
+  auto issue = [&](int buf) {
+    char *la = ring + buf * TILE;
+    const int k0 = kbeg + ik * kStep, left = pass < PASSES ? kend - k0 : 0;
+    const i32x4_t ra =
+        PA::rsrc(ap + (PASSES > 1 ? (kPlanesA >> (4 * pass) & 15) * g.aplane : 0), g.lda, k0);
+    const i32x4_t rb =
+        PB::rsrc(bp + (PASSES > 1 ? (kPlanesB >> (4 * pass) & 15) * g.bplane : 0), g.ldb, k0);
+#pragma unroll
+    for (int i = 0; i < PA::N; ++i) pa.issue(ra, i, left, la, lane, 0);
+#pragma unroll
+    for (int i = 0; i < PB::N; ++i) pb.issue(rb, i, left, la + PA::BYTES, lane, 0);
+    ik += 4;
+    while (ik >= nk && pass < PASSES) {
+      ik -= nk;
+      ++pass;
+    }
+  };
+  if (w < steps)
+    for (int t = 0; t < 2; ++t) issue(t);
+  int buf = 0;
+  for (int step = w; step < steps; step += 4) {
+    dma_wait<NDMA>();
+    const char *la = ring + buf * TILE, *lb = la + PA::BYTES;
+    Vec fa[2][2], fb[2][2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[ks][i] = PA::frag(la, ab, 32 * i, ks);
+        fb[ks][i] = PB::frag(lb, bb, 32 * i, ks);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    issue(buf);                                    // two steps on, into the pair just read
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma(fa[ks][i], fb[ks][j], acc[i][j]);
+    buf ^= 1;
+  }
+  dma_wait();
+  __syncthreads();
+  float *own = reinterpret_cast<float *>(smem) + w * 64 * CP;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        own[(32 * i + (v & 3) + 8 * (v >> 2) + 4 * (lane >> 5)) * CP + 32 * j + (lane & 31)] =
+            acc[i][j][v];
+  __syncthreads();
+  constexpr int V = Elem<T>::kVec, PR = 64 / V, NQ = 64 * PR / 256;
+  const int col = (tid % PR) * V, gc = n0 + col;
+  if (gc >= g.n) return;
+  const bool whole = g.nsplit == 1;
+  typename Elem<T>::Vec bias = {}, res[NQ];
+  if (whole) bias = bias_at<T>(g, gc);
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int gr = m0 + tid / PR + 256 / PR * q;
+    res[q] = typename Elem<T>::Vec{};
+    if (whole && gr < g.m) res[q] = res_at<T>(g, gr, gc);
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int row = tid / PR + 256 / PR * q, gr = m0 + row;
+    if (gr >= g.m) continue;
+    float s[V] = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int u = 0; u < V; u += 4) {
+        const f32x4_t t = *reinterpret_cast<const f32x4_t *>(
+            reinterpret_cast<const float *>(smem) + (k * 64 + row) * CP + col + u);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[u + x] += t[x];
+      }
+    if (whole) {
+      epilogue<T>(g, gr, gc, s, bias, res[q]);
+    } else {
+      float *dst = g.part + ((long long)split * g.m + gr) * g.n;
+#pragma unroll
+      for (int u = 0; u < V; u += 4)
+        store_row(dst, gc + u, g.n, f32x4_t{s[u], s[u + 1], s[u + 2], s[u + 3]});
+    }
+  }
 }
 
 // Few rows of x (up to 16 MT): a workgroup's eight waves share 16 rows of W and split the reduction
@@ -595,17 +622,35 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(GemmArgs g) {
   }
 }
 
-// 16-bit rows -> rows of ldd elements on 16-byte boundaries, zeros behind them
+// Rows of up to two operands (blockIdx.y) -> rows of ldd elements on 16-byte boundaries, zeros behind
+// them; f32: three bf16 planes of such rows
+struct PackArgs {
+  struct One {
+    long long rows, ld, plane;
+    int cols, ldd;
+    const void *src;
+    void *dst;
+  } op[2];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void linear_pack_kernel(long long rows, int cols, const T *src,
-                                                          long long ld, T *dst, int ldd) {
-  const long long total = rows * (ldd / 8);
+__global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
+  typedef typename Op<T>::Frag Frag;
+  constexpr int V = Elem<T>::kVec, H = 8 / V;
+  const PackArgs::One o = a.op[blockIdx.y];
+  const int units = o.ldd / 8;
+  const long long total = o.rows * units;
   for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total;
        e += (long long)gridDim.x * 256) {
-    const long long row = e / (ldd / 8);
-    const int col = (int)(e - row * (ldd / 8)) * 8;
-    *reinterpret_cast<typename Elem<T>::Vec *>(dst + row * ldd + col) =
-        load_row(src + row * ld, col, cols);
+    const long long row = e / units;
+    const int col = (int)(e - row * units) * 8;
+    typename Elem<T>::Vec v[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) v[h] = load_row((const T *)o.src + row * o.ld, col + h * V, o.cols);
+    Frag p[Op<T>::P];
+    pack(v, p);
+#pragma unroll
+    for (int i = 0; i < Op<T>::P; ++i)
+      *reinterpret_cast<Frag *>((typename Matrix<T>::E *)o.dst + i * o.plane + row * o.ldd + col) = p[i];
   }
 }
 
@@ -633,44 +678,54 @@ __global__ __launch_bounds__(256) void linear_join_kernel(GemmArgs g) {
   }
 }
 
-// dz = dy slope (ReLU: dy where slope > 0) into rows of ldz elements, zeros behind them, and the
-// column sums of dz over this workgroup's rows: 32 threads along the columns (a vector each), 8 rows
-// at a time.  dz NULL: the sums only.
+// dz = dy slope (ReLU: dy where slope > 0) into rows of ldz elements, zeros behind them (f32: into
+// its three planes), and the column sums of dz over this workgroup's rows: 32 threads along the
+// columns (8 each), 8 rows at a time.  dz NULL: the sums only.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, const T *dy,
                                                         long long lddy, const T *slope, int act,
-                                                        T *dz, int ldz, float *part) {
-  constexpr int V = Elem<T>::kVec;
-  __shared__ float red[8][32 * V];
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, col = (blockIdx.x * 32 + cl) * V;
-  float sum[V] = {};
+                                                        typename Matrix<T>::E *dz, int ldz,
+                                                        long long plane, float *part) {
+  constexpr int V = Elem<T>::kVec, H = 8 / V;
+  typedef typename Elem<T>::Vec Vec;
+  __shared__ float red[8][32 * 8];
+  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, col = (blockIdx.x * 32 + cl) * 8;
+  float sum[8] = {};
   if (col < n)
     for (long long row = (long long)blockIdx.y * 8 + rl; row < m; row += (long long)gridDim.y * 8) {
-      typename Elem<T>::Vec g = load_row(dy + row * lddy, col, n);
-      if (act != kActNone) {
-        const typename Elem<T>::Vec d = load_row(slope + row * n, col, n);
+      Vec g[H], d[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        g[h] = load_row(dy + row * lddy, col + h * V, n);
+        if (act != kActNone) d[h] = load_row(slope + row * n, col + h * V, n);
+      }
+#pragma unroll
+      for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (act == kActRelu)                     // (a select: an infinite dy stays out of it)
-            g[j] = (float)d[j] > 0.f ? g[j] : (T)0.f;
-          else
-            g[j] = (T)((float)g[j] * (float)d[j]);
+            g[h][j] = (float)d[h][j] > 0.f ? g[h][j] : (T)0.f;
+          else if (act != kActNone)
+            g[h][j] = (T)((float)g[h][j] * (float)d[h][j]);
+          sum[h * V + j] += (float)g[h][j];
         }
-      }
-      if (dz) store_row(dz + row * ldz, col, ldz, g);
+      if (dz) {
+        typename Op<T>::Frag f[Op<T>::P];
+        pack(g, f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[j] += (float)g[j];
+        for (int p = 0; p < Op<T>::P; ++p)
+          *reinterpret_cast<typename Op<T>::Frag *>(dz + p * plane + row * ldz + col) = f[p];
+      }
     }
   if (!part) return;
 #pragma unroll
-  for (int j = 0; j < V; ++j) red[rl][cl * V + j] = sum[j];
+  for (int j = 0; j < 8; ++j) red[rl][cl * 8 + j] = sum[j];
   __syncthreads();
-  for (int c = threadIdx.x; c < 32 * V; c += 256) {
-    float t = 0.f;
+  const int c = threadIdx.x;
+  float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += red[k][c];
-    if (blockIdx.x * 32 * V + c < n) part[(long long)blockIdx.y * n + blockIdx.x * 32 * V + c] = t;
-  }
+  for (int k = 0; k < 8; ++k) t += red[k][c];
+  if (blockIdx.x * 256 + c < n) part[(long long)blockIdx.y * n + blockIdx.x * 256 + c] = t;
 }
 
 // dbias = sum of the workgroups' rows, in order: 32 columns x 8 row groups a workgroup
@@ -699,25 +754,25 @@ struct Plan {
 
 // Tile and shares of the reduction by estimated time: workgroups a CU gets x (64-step pieces x what
 // one costs + what a workgroup costs besides), not below one workgroup's own latency, plus the
-// partial sums' way through memory.  The figures are us, measured for bf16 at 16 384 x 4 096 x 1 024
-// and 16 384 x 1 024 x 4 096 with each tile in turn.  (f32 has the two small tiles.)
-Plan plan_gemm(int m, int n, int k, bool dma) {
+// partial sums' way through memory.  The figures are us, measured for bf16 with each tile in turn: a
+// full chip at 16 384 x 4 096 x 1 024 and 16 384 x 1 024 x 4 096, one workgroup or two per CU at 1 024 x
+// (32 .. 2 048) x 2 048.  f32 runs six passes over k.
+Plan plan_gemm(int m, int n, int k, int passes) {
   static const struct { int bm, bn; double step, fixed, alone; } kTile[4] = {
-      {256, 256, 1.65, 11.0, 1.65}, {256, 128, 1.02, 6.7, 1.02}, {128, 128, 0.6, 3.4, 0.75},
-      {64, 64, 0.26, 1.3, 0.45}};
+      {256, 256, 1.65, 11.0, 1.06}, {256, 128, 1.02, 6.7, 0.62}, {128, 128, 0.65, 5.5, 0.8},
+      {64, 64, 0.22, 2.0, 0.2}};
   Plan best{};
   double least = 1e30;
-  for (int i = dma ? 0 : 2; i < 4; ++i) {
-    const auto &t = kTile[i];
+  for (const auto &t : kTile) {
     const int mt = cdiv(m, t.bm), nt = cdiv(n, t.bn);
     const long long tiles = (long long)mt * nt;
-    for (int s = 1; s <= 32 && (s == 1 || (k / s >= 128 && tiles * s <= 2048)); ++s) {
+    for (int s = 1; s <= 32 && (s == 1 || (k / s * passes >= 128 && tiles * s <= 2048)); ++s) {
       const int chunk = std::max(64, cdiv(cdiv(k, s), 64) * 64), real = std::max(1, cdiv(k, chunk));
       if (real != s) continue;
-      const double steps = chunk / 64;
+      const double steps = chunk / 64 * passes;
       double us = std::max((double)((tiles * s + 255) / 256) * (steps * t.step + t.fixed),
-                           steps * t.alone + t.fixed);
-      if (s > 1) us += 4.0 + (2.0 * s + 1.0) * m * n * 4.0 / 4e6;
+                           steps * t.alone + t.fixed + 1.5);
+      if (s > 1) us += 3.0 + (2.0 * s + 1.0) * m * n * 4.0 / 5e6;
       if (us < least) {
         least = us;
         best = Plan{t.bm, t.bn, mt, nt, s, chunk};
@@ -726,62 +781,79 @@ Plan plan_gemm(int m, int n, int k, bool dma) {
   }
   return best;
 }
+int passes_of(int dtype) { return dtype == BTR_F32 ? 6 : 1; }
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
-size_t split_bytes(int m, int n, int k, bool dma) {
-  const Plan p = plan_gemm(m, n, k, dma);
+size_t split_bytes(int m, int n, int k, int dtype) {
+  const Plan p = plan_gemm(m, n, k, passes_of(dtype));
   return p.nsplit > 1 ? align256((size_t)p.nsplit * m * n * sizeof(float)) : 0;
 }
 int up8(int v) { return (v + 7) & ~7; }
-// rows a DMA may read where they are: whole 16-byte units on 16-byte boundaries, a tile's offsets
-// below 2^31
-bool dma_rows(const void *p, long long ld, int len) {
-  return ((uintptr_t)p & 15) == 0 && len % 8 == 0 && ld % 8 == 0 && ld <= (1 << 22);
+// rows a DMA may read where they are: 16 bits, whole 16-byte units on 16-byte boundaries, a tile's
+// offsets below 2^31
+bool dma_rows(int dtype, const void *p, long long ld, int len) {
+  return dtype != BTR_F32 && ((uintptr_t)p & 15) == 0 && len % 8 == 0 && ld % 8 == 0 &&
+         ld <= (1 << 22);
 }
-size_t pack_bytes(const void *p, long long ld, long long rows, int len) {
-  return dma_rows(p, ld, len) ? 0 : align256((size_t)rows * up8(len) * 2);
+// one plane of packed rows in elements, and the bytes of all
+long long plane_of(long long rows, int len) { return (long long)(align256((size_t)rows * up8(len) * 2) / 2); }
+size_t packed_bytes(int dtype, long long rows, int len) {
+  return (size_t)plane_of(rows, len) * 2 * (dtype == BTR_F32 ? 3 : 1);
+}
+size_t pack_bytes(int dtype, const void *p, long long ld, long long rows, int len) {
+  return dma_rows(dtype, p, ld, len) ? 0 : packed_bytes(dtype, rows, len);
 }
 constexpr int kFewRows = 16;       // linear_rows_kernel up to here
 // workgroups along the rows of the dz / dbias pass
 int dz_blocks(long long m, int n) {
-  const long long cols = cdiv(n, 128);
-  return (int)std::max<long long>(1, std::min<long long>((m + 31) / 32, (2048 + cols - 1) / cols));
+  const long long cols = cdiv(n, 256);
+  return (int)std::max<long long>(1, std::min<long long>((m + 31) / 32, (1024 + cols - 1) / cols));
 }
 
-// an operand as the DMA kernels want it: where it is, or packed into ws (which moves on)
+// operands as the DMA kernel wants them: where they are, or packed / split into ws (which moves on),
+// one launch for both
+struct Rows {
+  const void *p;
+  long long ld, plane, rows;
+  int len;
+};
 template <typename T>
-void pack_rows(const void *&p, long long &ld, long long rows, int len, char *&ws, hipStream_t hs) {
-  if (dma_rows(p, ld, len)) return;
-  const int ldd = up8(len);
-  const long long units = rows * (ldd / 8);
-  hipLaunchKernelGGL((linear_pack_kernel<T>),
-                     dim3((unsigned)std::min<long long>(4096, (units + 255) / 256)), dim3(256), 0, hs,
-                     rows, len, (const T *)p, ld, (T *)ws, ldd);
-  p = ws;
-  ld = ldd;
-  ws += align256((size_t)rows * ldd * 2);
+void pack_rows(Rows *r, int count, char *&ws, hipStream_t hs) {
+  constexpr int dtype = sizeof(T) == 4 ? BTR_F32 : BTR_BF16;
+  PackArgs a{};
+  long long most = 0;
+  int n = 0;
+  for (int i = 0; i < count; ++i) {
+    if (dma_rows(dtype, r[i].p, r[i].ld, r[i].len)) continue;
+    const int ldd = up8(r[i].len);
+    const long long plane = plane_of(r[i].rows, r[i].len);
+    a.op[n++] = PackArgs::One{r[i].rows, r[i].ld, plane, r[i].len, ldd, r[i].p, ws};
+    most = std::max(most, r[i].rows * (ldd / 8));
+    r[i].p = ws;
+    r[i].ld = ldd;
+    r[i].plane = plane;
+    ws += packed_bytes(dtype, r[i].rows, r[i].len);
+  }
+  if (n)
+    hipLaunchKernelGGL((linear_pack_kernel<T>),
+                       dim3((unsigned)std::min<long long>(4096, (most + 255) / 256), n), dim3(256), 0,
+                       hs, a);
 }
 
 template <typename T, bool TA, bool TB>
-void launch_gemm(GemmArgs g, void *ws, hipStream_t hs) {
-  constexpr bool DMA = sizeof(T) == 2;
-  const Plan p = plan_gemm(g.m, g.n, g.k, DMA);
+void launch_gemm(GemmArgs g, Rows a, Rows b, void *ws, hipStream_t hs) {
+  const Plan p = plan_gemm(g.m, g.n, g.k, sizeof(T) == 4 ? 6 : 1);
+  g.a = a.p; g.lda = a.ld; g.aplane = a.plane;
+  g.b = b.p; g.ldb = b.ld; g.bplane = b.plane;
   g.mt = p.mt; g.nt = p.nt; g.nsplit = p.nsplit; g.chunk = p.chunk; g.part = (float *)ws;
   const dim3 grid((unsigned)((long long)p.mt * p.nt * p.nsplit));
-  if constexpr (DMA) {
-    if (p.bm == 256 && p.bn == 128)
-      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 128, 4, 2, 3, 4>), grid, dim3(512), 0, hs, g);
-    else if (p.bm == 256)
-      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 256, 2, 4, 4, 2>), grid, dim3(512), 0, hs, g);
-    else if (p.bm == 128)
-      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 128, 128, 2, 2, 4, 2>), grid, dim3(256), 0, hs, g);
-    else
-      hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 64, 64, 2, 2, 4, 2>), grid, dim3(256), 0, hs, g);
-  } else {
-    if (p.bm == 128)
-      hipLaunchKernelGGL((linear_gemm_kernel<TA, TB, 128, 128>), grid, dim3(256), 0, hs, g);
-    else
-      hipLaunchKernelGGL((linear_gemm_kernel<TA, TB, 64, 64>), grid, dim3(256), 0, hs, g);
-  }
+  if (p.bm == 256 && p.bn == 256)
+    hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 256, 2, 4, 4, 2>), grid, dim3(512), 0, hs, g);
+  else if (p.bm == 256)
+    hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 256, 128, 4, 2, 3, 4>), grid, dim3(512), 0, hs, g);
+  else if (p.bm == 128)
+    hipLaunchKernelGGL((linear_dma_kernel<T, TA, TB, 128, 128, 2, 2, 4, 2>), grid, dim3(256), 0, hs, g);
+  else
+    hipLaunchKernelGGL((linear_stream_kernel<T, TA, TB>), grid, dim3(256), 0, hs, g);
   if (p.nsplit > 1) {
     const long long pieces = (long long)g.m * cdiv(g.n, Elem<T>::kVec);
     hipLaunchKernelGGL((linear_join_kernel<T>),
@@ -797,7 +869,7 @@ int check(const char *what, const btr_linear_t *p) {
   BTR_REQUIRE(p->act >= BTR_ACT_NONE && p->act <= BTR_ACT_GELU, "%s: unknown activation %d", what,
               p->act);
   const int m = p->m, n = p->n, k = p->k;
-  BTR_REQUIRE(m >= 0 && n >= 1 && k >= 1 && m <= (1 << 30) && n <= (1 << 30) && k <= (1 << 30) &&
+  BTR_REQUIRE(m >= 0 && n >= 1 && k >= 1 && m <= (1 << 30) && n <= (1 << 22) && k <= (1 << 22) &&
                   ((long long)cdiv(m, 64) * cdiv(n, 64) <= (1 << 30)) &&
                   ((long long)cdiv(m, 64) * cdiv(k, 64) <= (1 << 30)) &&
                   ((long long)cdiv(n, 64) * cdiv(k, 64) <= (1 << 30)),
@@ -810,88 +882,77 @@ int check(const char *what, const btr_linear_t *p) {
 
 size_t fwd_bytes(const btr_linear_t &p) {
   if (p.m <= kFewRows) return 0;
-  if (p.dtype == BTR_F32) return split_bytes(p.m, p.n, p.k, false);
-  return pack_bytes(p.x, p.ldx, p.m, p.k) + pack_bytes(p.weight, p.ldw, p.n, p.k) +
-         split_bytes(p.m, p.n, p.k, true);
+  return pack_bytes(p.dtype, p.x, p.ldx, p.m, p.k) + pack_bytes(p.dtype, p.weight, p.ldw, p.n, p.k) +
+         split_bytes(p.m, p.n, p.k, p.dtype);
 }
 
 template <typename T>
 void forward(const btr_linear_t &p, void *y, void *slope, void *workspace, hipStream_t hs) {
   GemmArgs g{};
   g.m = p.m; g.n = p.n; g.k = p.k;
-  g.a = p.x; g.lda = p.ldx; g.b = p.weight; g.ldb = p.ldw;
   g.bias = p.bias; g.res = p.residual; g.ldres = p.ldr; g.act = p.act;
-  g.c = y; g.slope = slope;
+  g.c = y; g.slope = slope; g.nsplit = 1;
   if (p.m <= kFewRows) {
+    g.a = p.x; g.lda = p.ldx; g.b = p.weight; g.ldb = p.ldw;
     hipLaunchKernelGGL((linear_rows_kernel<T, 1>), dim3(cdiv(p.n, 16)), dim3(512), 0, hs, g);
     return;
   }
   char *ws = (char *)workspace;
-  if constexpr (sizeof(T) == 2) {
-    pack_rows<T>(g.a, g.lda, p.m, p.k, ws, hs);
-    pack_rows<T>(g.b, g.ldb, p.n, p.k, ws, hs);
-  }
-  launch_gemm<T, false, false>(g, ws, hs);
+  Rows op[2] = {{p.x, p.ldx, 0, p.m, p.k}, {p.weight, p.ldw, 0, p.n, p.k}};
+  pack_rows<T>(op, 2, ws, hs);
+  launch_gemm<T, false, false>(g, op[0], op[1], ws, hs);
 }
 
 // dz is written unless dy itself can be read as it is
 bool writes_dz(const btr_linear_t &p, const void *dy, long long lddy) {
-  return p.act != BTR_ACT_NONE || (p.dtype != BTR_F32 && !dma_rows(dy, lddy, p.n));
+  return p.act != BTR_ACT_NONE || !dma_rows(p.dtype, dy, lddy, p.n);
 }
 size_t bwd_bytes(const btr_linear_t &p, const void *dy, long long lddy) {
   const int m = p.m, n = p.n, k = p.k;
   if (m == 0) return 0;
-  const bool f32 = p.dtype == BTR_F32;
   size_t v = align256((size_t)dz_blocks(m, n) * n * sizeof(float));
-  if (writes_dz(p, dy, lddy)) v += align256((size_t)m * (f32 ? n * 4ll : up8(n) * 2ll));
-  if (!f32) v += pack_bytes(p.x, p.ldx, m, k) + pack_bytes(p.weight, p.ldw, n, k);
-  return v + std::max(split_bytes(m, k, n, !f32), split_bytes(n, k, m, !f32));
+  if (writes_dz(p, dy, lddy)) v += packed_bytes(p.dtype, m, n);
+  v += pack_bytes(p.dtype, p.x, p.ldx, m, k) + pack_bytes(p.dtype, p.weight, p.ldw, n, k);
+  return v + std::max(split_bytes(m, k, n, p.dtype), split_bytes(n, k, m, p.dtype));
 }
 
 template <typename T>
 void backward(const btr_linear_t &p, const void *slope, const void *dy, long long lddy, void *dx,
               void *dweight, void *dbias, void *workspace, hipStream_t hs) {
+  typedef typename Matrix<T>::E E;
   const int m = p.m, n = p.n, k = p.k;
   char *ws = (char *)workspace;
   float *part = (float *)ws;
   const int blocks = m > 0 ? dz_blocks(m, n) : 0;
-  const void *gz = dy;                             // what the two products read
-  long long ldg = lddy;
+  Rows dz{dy, lddy, 0, m, n};                      // what the two products read
   if (m > 0) {
     ws += align256((size_t)blocks * n * sizeof(float));
-    void *dz = nullptr;
-    const int ldz = sizeof(T) == 4 ? n : up8(n);
-    if (writes_dz(p, dy, lddy)) {
-      dz = ws;
-      ws += align256((size_t)m * ldz * sizeof(T));
-      gz = dz;
-      ldg = ldz;
+    E *out = nullptr;
+    if (writes_dz(p, dy, lddy) && (dx || dweight)) {
+      out = (E *)ws;
+      dz = Rows{ws, up8(n), plane_of(m, n), m, n};
+      ws += packed_bytes(p.dtype, m, n);
     }
-    if (dz || dbias)
-      hipLaunchKernelGGL((linear_dz_kernel<T>), dim3(cdiv(n, 32 * Elem<T>::kVec), blocks), dim3(256),
-                         0, hs, (long long)m, n, (const T *)dy, lddy, (const T *)slope, p.act,
-                         (T *)dz, ldz, dbias ? part : nullptr);
+    if (out || dbias)
+      hipLaunchKernelGGL((linear_dz_kernel<T>), dim3(cdiv(n, 256), blocks), dim3(256), 0, hs,
+                         (long long)m, n, (const T *)dy, lddy, (const T *)slope, p.act, out, up8(n),
+                         dz.plane, dbias ? part : nullptr);
   }
   if (dbias)   // (no rows: zeros)
     hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3(cdiv(n, 32)), dim3(256), 0, hs, part, blocks, n,
                        (T *)dbias);
-  const void *x = p.x, *wt = p.weight;
-  long long ldx = p.ldx, ldw = p.ldw;
-  if constexpr (sizeof(T) == 2) {
-    if (m > 0 && dweight) pack_rows<T>(x, ldx, m, k, ws, hs);
-    if (m > 0 && dx) pack_rows<T>(wt, ldw, n, k, ws, hs);
-  }
+  Rows op[2] = {{p.weight, p.ldw, 0, n, k}, {p.x, p.ldx, 0, m, k}};
+  if (m > 0 && (dx || dweight))
+    pack_rows<T>(op + (dx ? 0 : 1), (dx ? 1 : 0) + (dweight ? 1 : 0), ws, hs);
   if (dx && m > 0) {
     GemmArgs g{};
-    g.m = m; g.n = k; g.k = n;
-    g.a = gz; g.lda = ldg; g.b = wt; g.ldb = ldw; g.c = dx;
-    launch_gemm<T, false, true>(g, ws, hs);
+    g.m = m; g.n = k; g.k = n; g.c = dx;
+    launch_gemm<T, false, true>(g, dz, op[0], ws, hs);
   }
   if (dweight) {
     GemmArgs g{};
-    g.m = n; g.n = k; g.k = m;                     // (no rows: an empty reduction writes zeros)
-    g.a = gz; g.lda = ldg; g.b = x; g.ldb = ldx; g.c = dweight;
-    launch_gemm<T, true, true>(g, ws, hs);
+    g.m = n; g.n = k; g.k = m; g.c = dweight;      // (no rows: an empty reduction writes zeros)
+    launch_gemm<T, true, true>(g, dz, op[1], ws, hs);
   }
 }
 
