@@ -39,6 +39,7 @@ namespace btr {
 namespace {
 
 constexpr int kMaxShares = 1024;    // of a row's keys
+constexpr int kFewShares = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct XaArgs {
@@ -447,7 +448,39 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
   }
 }
 
-// Joins the shares of one row (a workgroup each): the weights once into LDS, then eight groups of 32
+// Joins the shares.  A weight of a share without a finite score is its sum itself, which is 0, or NaN
+// if its scores were.  Few shares: 32 threads a row, the shares in order.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_attention_join_few_kernel(XaArgs a) {
+  const long long nrow = (long long)a.b * a.hk * a.rows;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= nrow) return;
+  const int bh = (int)(row / a.rows), r = (int)(row - (long long)bh * a.rows);
+  const int c = 4 * (threadIdx.x & 31);
+  float m[kFewShares], l[kFewShares], M = -INFINITY, L = 0.f;
+  f32x4_t p[kFewShares], t = {};
+#pragma unroll
+  for (int s = 0; s < kFewShares; ++s) {         // (every load in flight at once)
+    const long long at = (s < a.nsplit ? s : 0) * nrow + row;
+    m[s] = a.part2[2 * at];
+    l[s] = a.part2[2 * at + 1];
+    p[s] = load_row(a.part + at * a.d, c, a.d);
+    if (s < a.nsplit) M = fmaxf(M, m[s]);
+  }
+#pragma unroll
+  for (int s = 0; s < kFewShares; ++s)
+    if (s < a.nsplit) {
+      const float w = m[s] == -INFINITY ? l[s] : __builtin_amdgcn_exp2f(m[s] - M);
+      t += p[s] * w;
+      L = fmaf(l[s], w, L);
+    }
+  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  const Rows<T> rows{a, bh / a.hk, bh % a.hk};
+  const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
+  store4((T *)a.out + rows.o(r), c, a.d, v4);
+  if (c == 0 && a.lse) a.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+}
+// Many shares (of few rows): a workgroup a row, the weights once into LDS, then eight groups of 32
 // threads add every eighth share, and the groups' sums are added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void cross_attention_join_kernel(XaArgs a) {
@@ -464,7 +497,6 @@ __global__ __launch_bounds__(256) void cross_attention_join_kernel(XaArgs a) {
   if ((tid & 63) == 0) red[0][tid >> 6] = M;
   __syncthreads();
   M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  // a share's weight: without a finite score its sum itself, which is 0, or NaN if its scores were
   for (int s = tid; s < a.nsplit; s += 256) {
     const float m = wt[s];
     wt[s] = m == -INFINITY ? a.part2[2 * (s * nrow + row) + 1] : __builtin_amdgcn_exp2f(m - M);
@@ -738,8 +770,8 @@ __global__ __launch_bounds__(256) void cross_attention_sum_kernel(XaArgs a, long
 }
 
 // =========================================================== 16-bit, aligned: tiles by LDS DMA
-// Heads of up to 64 or 128 columns, a multiple of 8, rows on 16-byte boundaries: the tiles go from
-// memory to LDS by DMA (lds_dma.hpp), a tile ahead of their use, which frees the 32 staging
+// Head widths of whole 16-byte units, rows on 16-byte boundaries: the tiles go from memory to LDS by
+// DMA (lds_dma.hpp; rows of 64 or 128 columns, of which the products take 32 NT), a tile ahead of their use, which frees the 32 staging
 // registers a lane (two waves per SIMD fit: 332 -> 218 registers at D = 128) and the LDS write
 // instructions.  Rows past the last key, masked keys and columns past d are loaded from beyond the
 // buffer's bound, which reads as zero.
@@ -770,10 +802,11 @@ __device__ __forceinline__ void dma_tile(const DmaSrc &s, int row0, int limit,
 }
 // KT subtiles of 32 rows x the register operand.  The fragments are asked for in two batches ahead
 // of the products: read one by one just before its product, each would cost an LDS round trip.
-template <typename T, int D, int KT>
+constexpr int row_of(int nt) { return nt <= 2 ? 64 : 128; }   // columns of a tile row in LDS
+template <typename T, int NT, int KT>
 __device__ __forceinline__ void dma_rows(const char *tile, int base, const typename Elem<T>::Vec *f,
                                          f32x16_t (&acc)[KT]) {
-  constexpr int J = D / 16, HALF = J / 2;
+  constexpr int D = row_of(NT), J = 2 * NT, HALF = NT;
   typename Elem<T>::Vec x[J][KT];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -793,9 +826,9 @@ __device__ __forceinline__ void dma_rows(const char *tile, int base, const typen
     for (int t = 0; t < KT; ++t) acc[t] = mma<T>(x[j][t], f[j], acc[t]);
 }
 // acc[nt] += tile[32 rows]^T w: the next 16 rows' fragments are in flight during a step's products
-template <typename T, int D>
+template <typename T, int NT>
 struct DmaT {
-  static constexpr int NT = D / 32;
+  static constexpr int D = row_of(NT);
   s16x4_t x[2][NT][2];
   __device__ __forceinline__ void load(const char *tile, int base, int s) {
 #pragma unroll
@@ -823,8 +856,8 @@ struct DmaT {
   }
 };
 // ... over KT subtiles; the first step's fragments have been loaded
-template <typename T, int D, int KT>
-__device__ __forceinline__ void dma_t(DmaT<T, D> &v, const char *tile, int base,
+template <typename T, int NT, int KT>
+__device__ __forceinline__ void dma_t(DmaT<T, NT> &v, const char *tile, int base,
                                       const f32x16_t (&w)[KT], f32x16_t *acc) {
 #pragma unroll
   for (int s = 0; s < 2 * KT; ++s) {
@@ -877,10 +910,10 @@ __device__ __forceinline__ void drop_dead(f32x16_t (&s)[KT], unsigned long long 
 }
 
 // forward: WR waves x 32 rows share tiles of 64 keys, double-buffered, one barrier a tile
-template <typename T, int D, int WR>
+template <typename T, int NT, int WR>
 __global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
-  constexpr int NT = D / 32, TB = 64 * Dma<D>::PITCH;
+  constexpr int D = row_of(NT), TB = 64 * Dma<D>::PITCH;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TB];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
   int tile, bh, split;
@@ -892,9 +925,9 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaA
   const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
   const Rows<T> rows{a, b, kh};
   const int r = (tile * WR + w) * 32 + l31;
-  Vec qf[D / 16];
+  Vec qf[2 * NT];
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
+  for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = Vec{};
     if (r < a.rows && 16 * j + 8 * hh < a.d)
       qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + 16 * j + 8 * hh);
@@ -929,24 +962,24 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaA
     const char *kt = smem + buf * 2 * TB, *vt = kt + TB;
     buf ^= 1;
     f32x16_t s[2];
-    dma_rows<T, D, 2>(kt, rb, qf, s);
+    dma_rows<T, NT, 2>(kt, rb, qf, s);
     drop_dead<2>(s, live[0], hh);
-    DmaT<T, D> v;
+    DmaT<T, NT> v;
     v.load(vt, tb, 0);
     online<2, NT>(s, m, l, o, a.scale_log2);
-    dma_t<T, D, 2>(v, vt, tb, s, o);
+    dma_t<T, NT, 2>(v, vt, tb, s, o);
   }
   l += other_half(l);
-  if (r < a.rows) finish_row<T, D>(a, rows, bh, split, r, hh, m, l, o);
+  if (r < a.rows) finish_row<T, 32 * NT>(a, rows, bh, split, r, hh, m, l, o);
 }
 
 // few rows (32): every wave streams its own tiles of 32 keys -- wave w those of index w, w + 4, ..
 // -- through its own double buffer, without a barrier until the four merge.  Bound by HBM: 64 KB a
 // CU in flight.
-template <typename T, int D>
+template <typename T, int NT>
 __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
-  constexpr int NT = D / 32, TB = 32 * Dma<D>::PITCH, MERGE = 4 * 32 * (D + kMergePitch) * 4;
+  constexpr int D = row_of(NT), TB = 32 * Dma<D>::PITCH, MERGE = 4 * 32 * (32 * NT + kMergePitch) * 4;
   __shared__ __attribute__((aligned(1024))) char smem[16 * TB > MERGE ? 16 * TB : MERGE];
   __shared__ float mx[4 * 32], sm[4 * 32];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
@@ -959,9 +992,9 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
   const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
   const Rows<T> rows{a, b, kh};
   const int r = tile * 32 + l31;
-  Vec qf[D / 16];
+  Vec qf[2 * NT];
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
+  for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = Vec{};
     if (r < a.rows && 16 * j + 8 * hh < a.d)
       qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + 16 * j + 8 * hh);
@@ -1001,22 +1034,22 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
     const char *kt = own + buf * 2 * TB, *vt = kt + TB;
     buf ^= 1;
     f32x16_t s[1];
-    dma_rows<T, D, 1>(kt, rb, qf, s);
+    dma_rows<T, NT, 1>(kt, rb, qf, s);
     drop_dead<1>(s, live[0], hh);
-    DmaT<T, D> v;
+    DmaT<T, NT> v;
     v.load(vt, tb, 0);
     online<1, NT>(s, m, l, o, a.scale_log2);
-    dma_t<T, D, 1>(v, vt, tb, s, o);
+    dma_t<T, NT, 1>(v, vt, tb, s, o);
   }
   l += other_half(l);
-  merge_rows<T, D, 4>(a, rows, bh, split, tile, w, tid, m, l, o, (float *)smem, mx, sm);
+  merge_rows<T, 32 * NT, 4>(a, rows, bh, split, tile, w, tid, m, l, o, (float *)smem, mx, sm);
 }
 
 // dq: WR waves x 32 rows share tiles of 64 keys as in the forward
-template <typename T, int D, int WR>
+template <typename T, int NT, int WR>
 __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
-  constexpr int NT = D / 32, TB = 64 * Dma<D>::PITCH;
+  constexpr int D = row_of(NT), TB = 64 * Dma<D>::PITCH;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TB];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
   int tile, bh, split;
@@ -1028,10 +1061,10 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
   const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
   const Rows<T> rows{a, b, kh};
   const int r = (tile * WR + w) * 32 + l31;
-  Vec qf[D / 16], gf[D / 16];
+  Vec qf[2 * NT], gf[2 * NT];
   float delta = 0.f, lse = INFINITY;
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
+  for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = gf[j] = Vec{};
     if (r < a.rows && 16 * j + 8 * hh < a.d) {
       const int c = 16 * j + 8 * hh;
@@ -1080,9 +1113,9 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
     for (int t = 0; t < 2; ++t) {
       const char *kt2 = kt + 32 * t * Dma<D>::PITCH;
       f32x16_t s[1], dp[1];
-      dma_rows<T, D, 1>(kt2, rb, qf, s);
-      dma_rows<T, D, 1>(vt + 32 * t * Dma<D>::PITCH, rb, gf, dp);
-      DmaT<T, D> kx;
+      dma_rows<T, NT, 1>(kt2, rb, qf, s);
+      dma_rows<T, NT, 1>(vt + 32 * t * Dma<D>::PITCH, rb, gf, dp);
+      DmaT<T, NT> kx;
       kx.load(kt2, tb, 0);
 #pragma unroll
       for (int v = 0; v < 16; ++v)
@@ -1093,7 +1126,7 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
         for (int v = 0; v < 16; ++v)
           s[0][v] = (bits >> (4 * hh)) & (1u << acc_row(v, 0)) ? s[0][v] : 0.f;
       }
-      dma_t<T, D, 1>(kx, kt2, tb, s, dq);
+      dma_t<T, NT, 1>(kx, kt2, tb, s, dq);
     }
   }
   if (r >= a.rows) return;
@@ -1115,11 +1148,10 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
 // dk, dv: WK waves x 32 keys, tiles of 64 rows.  A lane owns one key, its column of both results
 // depends on no other key: what a padded key's lane computes is dropped at the end, nothing is
 // selected on the way.  Rows past the end read as zeros (P = 1, but dout, dP - D and q are 0).
-// Needs 64 % g == 0: a lane's row of a tile is then the same head and offset in every tile.
-template <typename T, int D, int WK>
-__global__ __launch_bounds__(64 * WK, D == 64 ? 2 : 1) void cross_attention_bwd_kv_dma_kernel(XaArgs a) {
+template <typename T, int NT, int WK>
+__global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_kv_dma_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
-  constexpr int NT = D / 32, TB = 64 * Dma<D>::PITCH, THREADS = 64 * WK;
+  constexpr int D = row_of(NT), TB = 64 * Dma<D>::PITCH, THREADS = 64 * WK;
   constexpr int N = 64 * Dma<D>::UNITS / THREADS;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TB];
   __shared__ __attribute__((aligned(1024))) float stat[2][2][64];
@@ -1133,9 +1165,9 @@ __global__ __launch_bounds__(64 * WK, D == 64 ? 2 : 1) void cross_attention_bwd_
   if (tile * 32 * WK >= nk) rend = rbeg;         // padding only: zeros
   const int key = (tile * WK + w) * 32 + l31;
   const bool live = key < nk && !(a.mask && a.mask[b * a.mask_sb + key]);
-  Vec kf[D / 16], vf[D / 16];
+  Vec kf[2 * NT], vf[2 * NT];
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
+  for (int j = 0; j < 2 * NT; ++j) {
     kf[j] = vf[j] = Vec{};
     if (live && 16 * j + 8 * hh < a.d) {
       const int c = 16 * j + 8 * hh;
@@ -1148,28 +1180,26 @@ __global__ __launch_bounds__(64 * WK, D == 64 ? 2 : 1) void cross_attention_bwd_
   f32x16_t dk[NT] = {}, dv[NT] = {};
   const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
 
-  // this thread's units of a tile: row and byte offset from the tile's first query
-  int row[N], qo[N], go[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = i * THREADS + tid, u = (e % Dma<D>::UNITS) ^ Dma<D>::swz(e / Dma<D>::UNITS);
-    row[i] = e / Dma<D>::UNITS;
-    const int l = row[i] / a.g, hd = row[i] - l * a.g;
-    qo[i] = 2 * (l * (int)a.q_sl + hd * (int)a.q_sh + 8 * u);
-    go[i] = 2 * ((l * a.h + hd) * a.d + 8 * u);
-    if (8 * u >= a.d) row[i] = 1 << 30;          // a column past the head's width
-  }
   const char *qb = (const char *)((const T *)a.q + b * a.q_sb + (long long)kh * a.g * a.q_sh);
   const char *gb = (const char *)((const T *)a.dout + ((long long)b * a.lq * a.h + kh * a.g) * a.d);
+  // row r0 + row of the tile is query l0 + l, head hd of the group; (rem + row) / g by a multiplication
+  // (exact: below 64 + g <= 192, times a reciprocal rounded up by less than g / 65 536)
+  const int inv_g = (65536 + a.g - 1) / a.g;
   auto issue = [&](int r0, int buf) {
     char *qt = smem + buf * 2 * TB, *gt = qt + TB;
-    const int l0 = r0 / a.g;                     // (whole: 64 % g == 0)
+    const int l0 = r0 / a.g, rem = r0 - l0 * a.g;
     const i32x4_t qr = dma_rsrc(qb + 2 * (l0 * a.q_sl), kFar);
     const i32x4_t gr = dma_rsrc(gb + 2 * ((long long)l0 * a.h * a.d), kFar);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      dma16(qr, r0 + row[i] < rend ? qo[i] : kFar, qt + (i * THREADS + (tid & ~63)) * 16);
-      dma16(gr, r0 + row[i] < rend ? go[i] : kFar, gt + (i * THREADS + (tid & ~63)) * 16);
+      const int e = i * THREADS + tid, row = e / Dma<D>::UNITS;
+      const int u = (e % Dma<D>::UNITS) ^ Dma<D>::swz(row);
+      const int l = (rem + row) * inv_g >> 16, hd = rem + row - l * a.g;
+      const bool in = r0 + row < rend && 8 * u < a.d;
+      dma16(qr, in ? 2 * (l * (int)a.q_sl + hd * (int)a.q_sh + 8 * u) : kFar,
+            qt + (i * THREADS + (tid & ~63)) * 16);
+      dma16(gr, in ? 2 * ((l * a.h + hd) * a.d + 8 * u) : kFar,
+            gt + (i * THREADS + (tid & ~63)) * 16);
     }
     if (w < 2) {                                 // lse, D of the rows
       const float *src = (w ? a.delta : a.lse) + (long long)bh * a.rows + r0;
@@ -1190,9 +1220,9 @@ __global__ __launch_bounds__(64 * WK, D == 64 ? 2 : 1) void cross_attention_bwd_
     for (int t = 0; t < 2; ++t) {
       const char *q2 = qt + 32 * t * Dma<D>::PITCH, *g2 = gt + 32 * t * Dma<D>::PITCH;
       f32x16_t p[1], ds[1];
-      dma_rows<T, D, 1>(q2, rb, kf, p);
-      dma_rows<T, D, 1>(g2, rb, vf, ds);
-      DmaT<T, D> gx;
+      dma_rows<T, NT, 1>(q2, rb, kf, p);
+      dma_rows<T, NT, 1>(g2, rb, vf, ds);
+      DmaT<T, NT> gx;
       gx.load(g2, tb, 0);
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq) {
@@ -1205,10 +1235,10 @@ __global__ __launch_bounds__(64 * WK, D == 64 ? 2 : 1) void cross_attention_bwd_
           ds[0][v] = p[0][v] * (ds[0][v] - d4[i]);
         }
       }
-      dma_t<T, D, 1>(gx, g2, tb, p, dv);
-      DmaT<T, D> qx;
+      dma_t<T, NT, 1>(gx, g2, tb, p, dv);
+      DmaT<T, NT> qx;
       qx.load(q2, tb, 0);
-      dma_t<T, D, 1>(qx, q2, tb, ds, dk);
+      dma_t<T, NT, 1>(qx, q2, tb, ds, dk);
     }
   }
   if (key >= a.lk) return;
@@ -1269,14 +1299,14 @@ bool aligned(const void *p, long long sb, long long sl, long long sh) {
 // Can tiles of K and V go through LDS DMA?  Whole 16-byte units on 16-byte boundaries, rows apart
 // by at least a row, a tile's offsets within 31 bits.
 bool dma_ok(const XaArgs &a, int dtype) {
-  return dtype != BTR_F32 && a.d % 8 == 0 && (a.d <= 64 || a.d > 96) &&
+  return dtype != BTR_F32 && a.d % 8 == 0 &&
          aligned(a.k, a.k_sb, a.k_sl, a.k_sh) && aligned(a.v, a.v_sb, a.v_sl, a.v_sh) &&
          a.k_sl >= a.d && a.v_sl >= a.d;
 }
 // ... and tiles of query and dout rows?  The same of theirs, offsets within a tile of 64 rows below
-// 2^31, and groups that divide a tile.
+// 2^31, and groups of at most 128.
 bool dma_rows_ok(const XaArgs &a, int dtype, const void *dout) {
-  return dtype != BTR_F32 && a.d % 8 == 0 && (a.d <= 64 || a.d > 96) && 64 % a.g == 0 &&
+  return dtype != BTR_F32 && a.d % 8 == 0 && a.g <= 128 &&
          aligned(a.q, a.q_sb, a.q_sl, a.q_sh) && a.q_sl >= 0 && a.q_sh >= 0 &&
          a.q_sh <= (1 << 22) && ((uintptr_t)dout & 15) == 0 && (long long)a.h * a.d <= (1 << 22);
 }
@@ -1287,15 +1317,15 @@ Shares key_shares(const XaArgs &a) {                  // dk, dv: over the rows
 template <typename T, int DP>
 void launch_fwd(const XaArgs &a, bool dma, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
-  if constexpr (sizeof(T) == 2 && DP != 96) {
-    constexpr int D = DP < 64 ? 64 : DP;
+  if constexpr (sizeof(T) == 2) {
+    constexpr int NT = DP / 32;
     if (dma) {
       if (few(a.rows))
-        hipLaunchKernelGGL((cross_attention_fwd_stream_kernel<T, D>), grid, dim3(256), 0, hs, a);
+        hipLaunchKernelGGL((cross_attention_fwd_stream_kernel<T, NT>), grid, dim3(256), 0, hs, a);
       else if (dma_rows_per(a) == 256)
-        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, D, 8>), grid, dim3(512), 0, hs, a);
+        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, NT, 8>), grid, dim3(512), 0, hs, a);
       else
-        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, D, 4>), grid, dim3(256), 0, hs, a);
+        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, NT, 4>), grid, dim3(256), 0, hs, a);
       return;
     }
   }
@@ -1307,13 +1337,13 @@ void launch_fwd(const XaArgs &a, bool dma, hipStream_t hs) {
 template <typename T, int DP>
 void launch_bwd_q(const XaArgs &a, bool dma, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
-  if constexpr (sizeof(T) == 2 && DP != 96) {
-    constexpr int D = DP < 64 ? 64 : DP;
+  if constexpr (sizeof(T) == 2) {
+    constexpr int NT = DP / 32;
     if (dma && !few(a.rows)) {
       if (dma_rows_per(a) == 256)
-        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, D, 8>), grid, dim3(512), 0, hs, a);
+        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, NT, 8>), grid, dim3(512), 0, hs, a);
       else
-        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, D, 4>), grid, dim3(256), 0, hs, a);
+        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, NT, 4>), grid, dim3(256), 0, hs, a);
       return;
     }
   }
@@ -1325,10 +1355,10 @@ void launch_bwd_q(const XaArgs &a, bool dma, hipStream_t hs) {
 template <typename T, int DP>
 void launch_bwd_kv(const XaArgs &a, bool dma, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
-  if constexpr (sizeof(T) == 2 && DP != 96) {
+  if constexpr (sizeof(T) == 2) {
     if (dma) {
-      hipLaunchKernelGGL((cross_attention_bwd_kv_dma_kernel<T, DP < 64 ? 64 : DP, 4>), grid,
-                         dim3(256), 0, hs, a);
+      hipLaunchKernelGGL((cross_attention_bwd_kv_dma_kernel<T, DP / 32, 4>), grid, dim3(256), 0, hs,
+                         a);
       return;
     }
   }
@@ -1432,9 +1462,13 @@ extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out
   }
   hipStream_t hs = as_stream(stream);
   BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_fwd, a, dma, hs));
-  if (s.n > 1)
+  if (s.n > kFewShares)
     BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_join_kernel<T>),
                                                     dim3((unsigned)nrow), dim3(256), 0, hs, a));
+  else if (s.n > 1)
+    BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_join_few_kernel<T>),
+                                                    dim3((unsigned)((nrow + 7) / 8)), dim3(256), 0,
+                                                    hs, a));
   return check_launch("cross_attention_fwd");
 }
 
