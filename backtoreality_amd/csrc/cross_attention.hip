@@ -1292,10 +1292,12 @@ Shares shares(int tiles, long long bh, int length, int step, int least) {
   return {tiles, std::max(1, cdiv(length, chunk)), chunk};
 }
 bool few(int rows) { return rows <= kFewRows; }
-// rows of a workgroup of the DMA kernels: 256 where those still give every CU two workgroups (the
-// keys are read half as often), else 128
+// Rows of a workgroup of the DMA kernels.  Wide heads, bound by the tiles' way to LDS: 256 where those
+// still give every CU two workgroups (the keys are read half as often).  Heads of up to 64 columns,
+// bound by the VALU: 128, of which three fit a CU instead of one of 256 (ragged batch: 163 -> 133 us
+// forward, 192 -> 157 us dq).
 int dma_rows_per(const XaArgs &a) {
-  return (long long)cdiv(a.rows, 256) * a.b * a.hk >= 512 ? 256 : 128;
+  return a.d > 64 && (long long)cdiv(a.rows, 256) * a.b * a.hk >= 512 ? 256 : 128;
 }
 Shares row_shares(const XaArgs &a, bool dma) {   // forward, dq: over the keys
   return shares(cdiv(a.rows, few(a.rows) ? 32 : dma ? dma_rows_per(a) : 128), (long long)a.b * a.hk,
