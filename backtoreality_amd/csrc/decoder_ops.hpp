@@ -38,6 +38,13 @@ struct Elem<_Float16> {
   typedef _Float16 VecU __attribute__((ext_vector_type(8), aligned(2)));
 };
 
+template <>
+struct Elem<unsigned short> {   // 16 bits as they are
+  static constexpr int kVec = 8;
+  typedef unsigned short Vec __attribute__((ext_vector_type(8)));
+  typedef unsigned short VecU __attribute__((ext_vector_type(8), aligned(2)));
+};
+
 // the elements [e0, e0 + kVec) of a row of n; beyond the row zero, and never read
 template <typename T>
 __device__ __forceinline__ typename Elem<T>::Vec load_row(const T *row, int e0, int n) {

@@ -18,10 +18,12 @@
 // Numbers: every product accumulates in f32 and the epilogue works on the f32 sums; y is rounded
 // once.  f32 operands are split into three bf16 terms (8 + 8 + 8 bits: exact up to the 24th) and
 // multiplied as the six products above 2^-24, the smallest first, as one reduction six times as
-// long, which the bf16 matrix pipe does 2.7 times faster than the f32 instructions do one; an infinite f32 element makes the sums it enters NaN.  What the
-// backward needs of the activation is its slope act'(z), taken from the f32 sum in the forward's
-// epilogue and kept in the type of x (half an ulp; 0 and 1 of ReLU are exact); dz is rounded to the
-// type of x as well before the two products that read it.
+// long, which the bf16 matrix pipe does 2.7 times faster than the f32 instructions do one; an
+// infinite f32 element makes the sums it enters NaN.  What the backward needs of the activation is
+// its slope act'(z), taken from the f32 sum in the forward's epilogue and kept in as many bits as x
+// has: for GELU's of 16 bits a fixed-point number (steps of 1 / 46 000 from -0.1875: 1e-5 at most,
+// against 2^-9 for a bf16 slope, which was a third of the gradients' error).  dz is rounded to the
+// type of x before the two products that read it.
 #include <algorithm>
 #include <cstdint>
 
@@ -43,7 +45,7 @@ struct GemmArgs {
   const void *bias, *res;
   long long ldres;
   int act;
-  void *c, *slope;           // contiguous (m, n); slope: act' of the sums, or NULL
+  void *c, *slope;           // contiguous (m, n); slope: act' of the sums (Slope), or NULL
   float *part;               // split reduction: (nsplit, m, n) partial sums
   int nsplit, chunk;         // shares of k, their length
   long long aplane, bplane;  // f32: elements from one bf16 plane of an operand to the next
@@ -169,6 +171,32 @@ __device__ __forceinline__ float activate(float z, int act, float &slope) {
   return z;
 }
 
+// The slope as the backward gets it: f32 itself, or 16 bits -- GELU's in fixed point (at most 1.13:
+// below 60 600; all ones stand for NaN; what pads a row reads as 0 and must give 0), ReLU's 1 or 0.
+template <typename T>
+struct Slope {
+  typedef unsigned short S;
+  __device__ static __forceinline__ S keep(float d, int act) {
+    if (act == kActRelu) return d > 0.f ? 1 : 0;
+    return (S)(d == d ? (unsigned)fmaf(d, 46000.f, 0.1875f * 46000.f + 0.5f) : 0xffffu);
+  }
+  // dy act': ReLU's may also be the result itself (its sign; NaN lets dy through)
+  __device__ static __forceinline__ T times(T dy, S v, int act) {
+    if (act == kActRelu) return (short)v > 0 ? dy : (T)0.f;   // (an infinite dy stays out of it)
+    return v != 0xffff ? (T)((float)dy * fmaf((float)v, 1.f / 46000.f, -0.1875f))
+                       : (T)__builtin_nanf("");
+  }
+};
+template <>
+struct Slope<float> {
+  typedef float S;
+  __device__ static __forceinline__ S keep(float d, int) { return d; }
+  __device__ static __forceinline__ float times(float dy, S v, int act) {
+    if (act == kActRelu) return v > 0.f || v != v ? dy : 0.f;
+    return dy * v;
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ typename Elem<T>::Vec bias_at(const GemmArgs &g, int col) {
   return g.bias ? load_row((const T *)g.bias, col, g.n) : typename Elem<T>::Vec{};
@@ -183,14 +211,15 @@ __device__ __forceinline__ void epilogue(const GemmArgs &g, long long row, int c
                                          const float (&s)[Elem<T>::kVec],
                                          typename Elem<T>::Vec bias, typename Elem<T>::Vec res) {
   constexpr int V = Elem<T>::kVec;
-  typename Elem<T>::Vec slope, y;
+  typename Elem<T>::Vec y;
+  typename Elem<typename Slope<T>::S>::Vec slope;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float d;
     y[j] = (T)(activate<sizeof(T) == 4>(s[j] + (float)bias[j], g.act, d) + (float)res[j]);
-    slope[j] = (T)d;
+    slope[j] = Slope<T>::keep(d, g.act);
   }
-  if (g.slope) store_row((T *)g.slope + row * g.n, col, g.n, slope);
+  if (g.slope) store_row((typename Slope<T>::S *)g.slope + row * g.n, col, g.n, slope);
   store_row((T *)g.c + row * g.n, col, g.n, y);
 }
 
@@ -683,7 +712,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(GemmArgs g) {
 // columns (8 each), 8 rows at a time.  dz NULL: the sums only.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, const T *dy,
-                                                        long long lddy, const T *slope, int act,
+                                                        long long lddy, const typename Slope<T>::S *slope,
+                                                        int act,
                                                         typename Matrix<T>::E *dz, int ldz,
                                                         long long plane, float *part) {
   constexpr int V = Elem<T>::kVec, H = 8 / V;
@@ -693,7 +723,8 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, cons
   float sum[8] = {};
   if (col < n)
     for (long long row = (long long)blockIdx.y * 8 + rl; row < m; row += (long long)gridDim.y * 8) {
-      Vec g[H], d[H];
+      Vec g[H];
+      typename Elem<typename Slope<T>::S>::Vec d[H];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         g[h] = load_row(dy + row * lddy, col + h * V, n);
@@ -703,10 +734,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, cons
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if (act == kActRelu)                     // (a select: an infinite dy stays out of it)
-            g[h][j] = (float)d[h][j] > 0.f ? g[h][j] : (T)0.f;
-          else if (act != kActNone)
-            g[h][j] = (T)((float)g[h][j] * (float)d[h][j]);
+          if (act != kActNone) g[h][j] = Slope<T>::times(g[h][j], d[h][j], act);
           sum[h * V + j] += (float)g[h][j];
         }
       if (dz) {
@@ -935,7 +963,8 @@ void backward(const btr_linear_t &p, const void *slope, const void *dy, long lon
     }
     if (out || dbias)
       hipLaunchKernelGGL((linear_dz_kernel<T>), dim3(cdiv(n, 256), blocks), dim3(256), 0, hs,
-                         (long long)m, n, (const T *)dy, lddy, (const T *)slope, p.act, out, up8(n),
+                         (long long)m, n, (const T *)dy, lddy,
+                         (const typename Slope<T>::S *)slope, p.act, out, up8(n),
                          dz.plane, dbias ? part : nullptr);
   }
   if (dbias)   // (no rows: zeros)

@@ -1133,8 +1133,9 @@ int btr_layer_norm_bwd(int dtype, long long rows, int width, const void *x, long
                        void *dbias, void *workspace, size_t workspace_bytes, btr_stream_t stream);
 
 /* z = x weight^T + bias, y = act(z) [+ residual]: x (m, k), weight (n, k), bias (n) or NULL, residual
- * (m, n) or NULL, y (m, n) contiguous.  act: BTR_ACT_*; GELU is the erf form.  slope (m, n) contiguous
- * in the type of x: receives act'(z), what the backward of an activation needs, or NULL.  1 <= n, k <= 2^22. */
+ * (m, n) or NULL, y (m, n) contiguous.  act: BTR_ACT_*; GELU is the erf form.  slope (m, n) contiguous,
+ * of as many bytes as y: receives what the backward of an activation needs (act'(z), in a form of its
+ * own), or NULL.  1 <= n, k <= 2^22. */
 #define BTR_ACT_NONE 0
 #define BTR_ACT_RELU 1
 #define BTR_ACT_GELU 2

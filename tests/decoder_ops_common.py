@@ -109,10 +109,10 @@ def linear(x, weight, bias, act, residual, dy=None):
     dz = g * slope
     if act == "relu":      # z within its error of zero may fall on either side
         edz = g.abs() * (z.abs() <= ez + tiny(dtype)).double()
-    elif act == "gelu":    # the kept slope: half a step; |gelu''| <= 0.8; 2^-20 for its own arithmetic
-        # (16 bits: the tail, at most a half, to 2^-14)
-        own = 2.0 ** -20 if f32 else 2.0 ** -15
-        edz = g.abs() * (u * slope.abs() + tiny(dtype) + 0.8 * ez + own) + u * dz.abs() + tiny(dtype)
+    elif act == "gelu":    # |gelu''| <= 0.8; the slope's own arithmetic 2^-20, and its rounding, f32's
+        # half step (16 bits: the tail, at most a half, to 2^-14, and half a fixed-point step, 2^-16)
+        own = 2.0 ** -20 + F * slope.abs() if f32 else 2.0 ** -15 + 2.0 ** -16
+        edz = g.abs() * (0.8 * ez + own) + u * dz.abs() + tiny(dtype)
     else:
         edz = torch.zeros_like(g)
     dx, dw, db = dz @ W, dz.t() @ X, dz.sum(0)
