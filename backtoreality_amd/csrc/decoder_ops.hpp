@@ -82,6 +82,31 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
   return v;
 }
 
+// Column c of the sum of `rows` partial rows of n floats, in a fixed order: 1 024 threads are 32 columns
+// x 32 groups of rows, four loads of a thread in flight (eight groups and one load at a time made
+// these launches 10 - 33 us).  Valid in threads of group 0 (threadIdx.x < 32).
+__device__ __forceinline__ float column_sum(const float *part, int rows, long long n, long long c) {
+  __shared__ float s[32][33];
+  const int cl = threadIdx.x & 31, rg = threadIdx.x >> 5;
+  float acc[4] = {};
+  if (c < n) {
+    int r = rg;
+    for (; r + 96 < rows; r += 128) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += part[(r + 32ll * i) * n + c];
+    }
+    for (; r < rows; r += 32) acc[0] += part[(long long)r * n + c];
+  }
+  s[rg][cl] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+  __syncthreads();
+  float t = 0.f;
+  if (rg == 0) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) t += s[k][cl];
+  }
+  return t;
+}
+
 }  // namespace btr
 
 // runs `CALL` (an expression that names the element type as T) for the type code `dtype`

@@ -216,22 +216,13 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void layer_norm_bwd_kernel(LnArg
   }
 }
 
-// column sums of part (blocks, 2 * width) -> dweight, dbias: 32 columns x 8 row groups a workgroup
+// column sums of part (blocks, 2 * width) -> dweight, dbias
 template <typename T>
-__global__ __launch_bounds__(256) void layer_norm_params_kernel(const float *part, int blocks,
-                                                                int width, T *dw, T *db) {
-  __shared__ float s[8][32];
-  const int cl = threadIdx.x & 31, rg = threadIdx.x >> 5;
-  const long long c = (long long)blockIdx.x * 32 + cl;
-  float acc = 0.f;
-  if (c < 2ll * width)
-    for (int r = rg; r < blocks; r += 8) acc += part[(long long)r * 2 * width + c];
-  s[rg][cl] = acc;
-  __syncthreads();
-  if (rg == 0 && c < 2ll * width) {
-    float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t += s[k][cl];
+__global__ __launch_bounds__(1024) void layer_norm_params_kernel(const float *part, int blocks,
+                                                                 int width, T *dw, T *db) {
+  const long long c = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
+  const float t = column_sum(part, blocks, 2ll * width, c);
+  if (threadIdx.x < 32 && c < 2ll * width) {
     if (c < width) {
       if (dw) dw[c] = (T)t;
     } else if (db) {
@@ -469,7 +460,7 @@ extern "C" int btr_layer_norm_bwd(int dtype, long long rows, int width, const vo
   }
   if (params)   // (no rows: zeros)
     BTR_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(
-        (layer_norm_params_kernel<T>), dim3(cdiv(2ll * width, 32)), dim3(256), 0, hs,
+        (layer_norm_params_kernel<T>), dim3(cdiv(2ll * width, 32)), dim3(1024), 0, hs,
         (const float *)workspace, blocks, width, (T *)dweight, (T *)dbias));
   return check_launch("layer_norm_bwd");
 }

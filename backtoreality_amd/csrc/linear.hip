@@ -756,23 +756,13 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, cons
   if (blockIdx.x * 256 + c < n) part[(long long)blockIdx.y * n + blockIdx.x * 256 + c] = t;
 }
 
-// dbias = sum of the workgroups' rows, in order: 32 columns x 8 row groups a workgroup
+// dbias = sum of the workgroups' rows, in order
 template <typename T>
-__global__ __launch_bounds__(256) void linear_dbias_kernel(const float *part, int blocks, int n,
-                                                           T *db) {
-  __shared__ float s[8][32];
-  const int cl = threadIdx.x & 31, rg = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-  float acc = 0.f;
-  if (c < n)
-    for (int r = rg; r < blocks; r += 8) acc += part[(long long)r * n + c];
-  s[rg][cl] = acc;
-  __syncthreads();
-  if (rg == 0 && c < n) {
-    float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t += s[k][cl];
-    db[c] = (T)t;
-  }
+__global__ __launch_bounds__(1024) void linear_dbias_kernel(const float *part, int blocks, int n,
+                                                            T *db) {
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31);
+  const float t = column_sum(part, blocks, n, c);
+  if (threadIdx.x < 32 && c < n) db[c] = (T)t;
 }
 
 // --------------------------------------------------------------------------------------- host
@@ -968,7 +958,7 @@ void backward(const btr_linear_t &p, const void *slope, const void *dy, long lon
                          dz.plane, dbias ? part : nullptr);
   }
   if (dbias)   // (no rows: zeros)
-    hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3(cdiv(n, 32)), dim3(256), 0, hs, part, blocks, n,
+    hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3(cdiv(n, 32)), dim3(1024), 0, hs, part, blocks, n,
                        (T *)dbias);
   Rows op[2] = {{p.weight, p.ldw, 0, n, k}, {p.x, p.ldx, 0, m, k}};
   if (m > 0 && (dx || dweight))
