@@ -40,11 +40,12 @@ namespace {
 
 constexpr int kMaxShares = 1024;    // of a row's keys
 constexpr int kFewShares = 8;
+__host__ __device__ inline int up8(int v) { return (v + 7) & ~7; }
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct XaArgs {
-  int b, lq, lk, h, hk, g, d, rows;              // rows = lq * g
-  const void *q, *k, *v, *dout;
+  int b, lq, lk, h, hk, g, d, gd, rows;          // rows = lq * g
+  const void *q, *k, *v, *dout, *dout_dma;       // dout_dma: rows of gd elements that a DMA may read
   long long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;   // element strides
   const int *lengths;                            // (b) or NULL
   const unsigned char *mask;                     // (b, lk), nonzero = padding, or NULL
@@ -95,7 +96,9 @@ __device__ __forceinline__ constexpr int acc_row(int v, int hh) {
   return (v & 3) + 8 * (v >> 2) + 4 * hh;
 }
 
-// first product: tile rows [row0, row0 + 32) x the register operand f (one row per lane & 31)
+// first product: tile rows [row0, row0 + 32) x the register operand f (one row per lane & 31).  (All
+// of the padded width: skipping the pieces beyond d -- 3 of 8 at d = 36 -- cost registers and time,
+// dk / dv 50 -> 58 us.)
 template <typename T, int DP>
 __device__ __forceinline__ f32x16_t tile_times_rows(const char *tile, int row0, int l31, int hh,
                                                     const typename Elem<T>::Vec *f) {
@@ -296,45 +299,47 @@ __device__ __forceinline__ void finish_row(const XaArgs &a, const Rows<T> &rows,
   }
 }
 
-// the same for 32 rows whose keys WK waves of the workgroup of 256 have shared: through LDS (om: WK
-// x 32 x (DP + 4) floats, the tiles' storage), added in wave order
-template <typename T, int DP, int WK>
+// the same for 32 WR rows whose keys WK waves each of the workgroup of four have shared: through LDS
+// (om: 4 x 32 x (DP + 4) floats, the tiles' storage), added in wave order
+template <typename T, int DP, int WR, int WK>
 __device__ __forceinline__ void merge_rows(const XaArgs &a, const Rows<T> &rows, int bh, int split,
-                                           int tile, int wk, int tid, float m, float l,
+                                           int tile, int wr, int wk, int tid, float m, float l,
                                            const f32x16_t (&o)[DP / 32], float *om, float *mx,
                                            float *sm) {
-  constexpr int LDO = DP + kMergePitch;
-  const int lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
+  constexpr int LDO = DP + kMergePitch, PER = 256 / (32 * WR);   // threads a row
+  const int lane = tid & 63, l31 = lane & 31, hh = lane >> 5, at = (wr * WK + wk) * 32 + l31;
   __syncthreads();                               // every wave is done with the tiles
 #pragma unroll
   for (int nt = 0; nt < DP / 32; ++nt)
 #pragma unroll
     for (int gq = 0; gq < 4; ++gq)
-      *reinterpret_cast<f32x4_t *>(om + (wk * 32 + l31) * LDO + 32 * nt + 8 * gq + 4 * hh) =
+      *reinterpret_cast<f32x4_t *>(om + at * LDO + 32 * nt + 8 * gq + 4 * hh) =
           f32x4_t{o[nt][4 * gq], o[nt][4 * gq + 1], o[nt][4 * gq + 2], o[nt][4 * gq + 3]};
   if (hh == 0) {
-    mx[wk * 32 + l31] = m * a.scale_log2;
-    sm[wk * 32 + l31] = l;
+    mx[at] = m * a.scale_log2;
+    sm[at] = l;
   }
   __syncthreads();
-  const int row = tid >> 3, sub = tid & 7, rr = tile * 32 + row;
+  const int row = tid / PER, sub = tid % PER, rr = tile * 32 * WR + row;
   if (rr >= a.rows) return;
+  const int first = (row >> 5) * WK * 32 + (row & 31);           // of its WK partial rows
   const bool share = a.nsplit > 1;
   const long long prow = ((long long)split * a.b * a.hk + bh) * a.rows + rr;
   float M = -INFINITY, L = 0.f, f[WK];
 #pragma unroll
-  for (int k = 0; k < WK; ++k) M = fmaxf(M, mx[k * 32 + row]);
+  for (int k = 0; k < WK; ++k) M = fmaxf(M, mx[first + 32 * k]);
 #pragma unroll
   for (int k = 0; k < WK; ++k) {
-    f[k] = mx[k * 32 + row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[k * 32 + row] - M);
-    L = fmaf(sm[k * 32 + row], f[k], L);
+    const float mk = mx[first + 32 * k];
+    f[k] = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - M);
+    L = fmaf(sm[first + 32 * k], f[k], L);
   }
   const float inv = share ? 1.f : L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
-  for (int c = 4 * sub; c < a.d; c += 32) {
+  for (int c = 4 * sub; c < a.d; c += 4 * PER) {
     f32x4_t t = {};
 #pragma unroll
     for (int k = 0; k < WK; ++k)
-      t += *reinterpret_cast<const f32x4_t *>(om + (k * 32 + row) * LDO + c) * f[k];
+      t += *reinterpret_cast<const f32x4_t *>(om + (first + 32 * k) * LDO + c) * f[k];
     const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
     if (share)
       store4(a.part + prow * a.d, c, a.d, v4);
@@ -353,18 +358,17 @@ __device__ __forceinline__ void merge_rows(const XaArgs &a, const Rows<T> &rows,
 
 // -------------------------------------------------------------------------------- forward
 // WR waves along the rows (32 each) x WK along the keys, KT key subtiles of 32 per wave and tile.
-//   WR 4, WK 1: >= 33 rows; the four waves share every K / V tile.
-//   WR 1, WK 4: few rows (single queries): the waves take a quarter of every tile and merge.
-// NBUF 2: tiles double-buffered, one barrier a tile.
-template <typename T, int DP, int WR, int WK, int KT, int NBUF>
+//   WR 4, WK 1: many rows; the four waves share every K / V tile.
+//   WR 1, WK 4: few rows (single queries).
+template <typename T, int DP, int WR, int WK, int KT>
 __global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Vec Vec;
   constexpr int BKV = 32 * WK * KT, NT = DP / 32, TB = BKV * TL::PITCH;
-  constexpr int MERGE = WK > 1 ? WK * 32 * (DP + kMergePitch) * 4 : 0;
-  constexpr int BYTES = 2 * TB * NBUF > MERGE ? 2 * TB * NBUF : MERGE;
+  constexpr int MERGE = WK > 1 ? 4 * 32 * (DP + kMergePitch) * 4 : 0;
+  constexpr int BYTES = 2 * TB > MERGE ? 2 * TB : MERGE;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
-  __shared__ float mx[WK > 1 ? WK * 32 : 1], sm[WK > 1 ? WK * 32 : 1];
+  __shared__ float mx[WK > 1 ? 4 * 32 : 1], sm[WK > 1 ? 4 * 32 : 1];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
   const int wr = w % WR, wk = w / WR;
   int tile, bh, split;
@@ -395,12 +399,11 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
     sv.fetch(vrow, kbeg, kend, a.d, tid);
     lv.fetch(mask, kbeg, kend, lane);
   }
-  int buf = 0;
+  char *kt = smem, *vt = smem + TB;
   for (int k0 = kbeg; k0 < kend; k0 += BKV) {
-    char *kt = smem + buf * 2 * TB, *vt = kt + TB;
     unsigned long long live[Live<BKV>::W];
     lv.words(k0, kend, lane, live);
-    if (NBUF == 1) lds_barrier();                // the previous tile's reads are done
+    lds_barrier();                               // the previous tile's reads are done
     sk.store(kt, mask ? live : nullptr, tid);
     sv.store(vt, mask ? live : nullptr, tid);
     if (k0 + BKV < kend) {                       // next tile's loads fly under this one's math
@@ -409,7 +412,6 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
       lv.fetch(mask, k0 + BKV, kend, lane);
     }
     lds_barrier();
-    if (NBUF == 2) buf ^= 1;
     f32x16_t s[KT];
     float top = -INFINITY;
 #pragma unroll
@@ -452,7 +454,7 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
   if constexpr (WK == 1) {
     if (r < a.rows) finish_row<T, DP>(a, rows, bh, split, r, hh, m, l, o);
   } else {
-    merge_rows<T, DP, WK>(a, rows, bh, split, tile, wk, tid, m, l, o, (float *)smem, mx, sm);
+    merge_rows<T, DP, WR, WK>(a, rows, bh, split, tile, wr, wk, tid, m, l, o, (float *)smem, mx, sm);
   }
 }
 
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(256) void cross_attention_bwd_q_kernel(XaArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Vec Vec;
   constexpr int BKV = 32 * WK * KT, NT = DP / 32, TB = BKV * TL::PITCH;
-  constexpr int MERGE = WK > 1 ? WK * 32 * (DP + kMergePitch) * 4 : 0;
+  constexpr int MERGE = WK > 1 ? 4 * 32 * (DP + kMergePitch) * 4 : 0;
   constexpr int BYTES = 2 * TB > MERGE ? 2 * TB : MERGE;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l31 = lane & 31, hh = lane >> 5;
@@ -634,23 +636,25 @@ __global__ __launch_bounds__(256) void cross_attention_bwd_q_kernel(XaArgs a) {
           store4((T *)a.dq + rows.o(r), c, a.d, v4);
       }
   } else {
-    constexpr int LDO = DP + kMergePitch;
+    constexpr int LDO = DP + kMergePitch, PER = 256 / (32 * WR);
     float *om = reinterpret_cast<float *>(smem);
     __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq)
-        *reinterpret_cast<f32x4_t *>(om + (wk * 32 + l31) * LDO + 32 * nt + 8 * gq + 4 * hh) =
+        *reinterpret_cast<f32x4_t *>(om + ((wr * WK + wk) * 32 + l31) * LDO + 32 * nt + 8 * gq +
+                                     4 * hh) =
             f32x4_t{dq[nt][4 * gq], dq[nt][4 * gq + 1], dq[nt][4 * gq + 2], dq[nt][4 * gq + 3]};
     __syncthreads();
-    const int row = tid >> 3, sub = tid & 7, rr = tile * 32 + row;
+    const int row = tid / PER, sub = tid % PER, rr = tile * 32 * WR + row;
     if (rr >= a.rows) return;
-    for (int c = 4 * sub; c < a.d; c += 32) {
+    const int first = (row >> 5) * WK * 32 + (row & 31);
+    for (int c = 4 * sub; c < a.d; c += 4 * PER) {
       f32x4_t t = {};
 #pragma unroll
       for (int k = 0; k < WK; ++k)
-        t += *reinterpret_cast<const f32x4_t *>(om + (k * 32 + row) * LDO + c);
+        t += *reinterpret_cast<const f32x4_t *>(om + (first + 32 * k) * LDO + c);
       const float v4[4] = {t[0] * a.scale, t[1] * a.scale, t[2] * a.scale, t[3] * a.scale};
       if (a.nsplit > 1)
         store4(a.part + (prow + rr) * a.d, c, a.d, v4);
@@ -928,8 +932,8 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaA
   place(a, tile, bh, split);
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
-  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, a.d * 2};
-  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, a.d * 2};
+  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, up8(a.d) * 2};
+  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, up8(a.d) * 2};
   const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
   const Rows<T> rows{a, b, kh};
   const int r = (tile * WR + w) * 32 + l31;
@@ -937,8 +941,7 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaA
 #pragma unroll
   for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = Vec{};
-    if (r < a.rows && 16 * j + 8 * hh < a.d)
-      qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + 16 * j + 8 * hh);
+    if (r < a.rows) qf[j] = load_row(rows.q(r), 16 * j + 8 * hh, a.d);
   }
   f32x16_t o[NT] = {};
   float m = -INFINITY, l = 0.f;
@@ -995,8 +998,8 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
   place(a, tile, bh, split);
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
-  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, a.d * 2};
-  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, a.d * 2};
+  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, up8(a.d) * 2};
+  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, up8(a.d) * 2};
   const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
   const Rows<T> rows{a, b, kh};
   const int r = tile * 32 + l31;
@@ -1004,8 +1007,7 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
 #pragma unroll
   for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = Vec{};
-    if (r < a.rows && 16 * j + 8 * hh < a.d)
-      qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + 16 * j + 8 * hh);
+    if (r < a.rows) qf[j] = load_row(rows.q(r), 16 * j + 8 * hh, a.d);
   }
   f32x16_t o[NT] = {};
   float m = -INFINITY, l = 0.f;
@@ -1050,7 +1052,7 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
     dma_t<T, NT, 1>(v, vt, tb, s, o);
   }
   l += other_half(l);
-  merge_rows<T, 32 * NT, 4>(a, rows, bh, split, tile, w, tid, m, l, o, (float *)smem, mx, sm);
+  merge_rows<T, 32 * NT, 1, 4>(a, rows, bh, split, tile, 0, w, tid, m, l, o, (float *)smem, mx, sm);
 }
 
 // dq: WR waves x 32 rows share tiles of 64 keys as in the forward
@@ -1064,8 +1066,8 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
   place(a, tile, bh, split);
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const int kbeg = split * a.chunk, kend = min(key_count(a, b), kbeg + a.chunk);
-  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, a.d * 2};
-  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, a.d * 2};
+  const DmaSrc ks{(const char *)((const T *)a.k + b * a.k_sb + kh * a.k_sh), a.k_sl * 2, up8(a.d) * 2};
+  const DmaSrc vs{(const char *)((const T *)a.v + b * a.v_sb + kh * a.v_sh), a.v_sl * 2, up8(a.d) * 2};
   const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
   const Rows<T> rows{a, b, kh};
   const int r = (tile * WR + w) * 32 + l31;
@@ -1074,12 +1076,11 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
 #pragma unroll
   for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = gf[j] = Vec{};
-    if (r < a.rows && 16 * j + 8 * hh < a.d) {
+    if (r < a.rows) {
       const int c = 16 * j + 8 * hh;
-      qf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>(rows.q(r) + c);
-      gf[j] = *reinterpret_cast<const typename Elem<T>::VecU *>((const T *)a.dout + rows.o(r) + c);
-      const Vec of =
-          *reinterpret_cast<const typename Elem<T>::VecU *>((const T *)a.out + rows.o(r) + c);
+      qf[j] = load_row(rows.q(r), c, a.d);
+      gf[j] = load_row((const T *)a.dout + rows.o(r), c, a.d);
+      const Vec of = load_row((const T *)a.out + rows.o(r), c, a.d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta = fmaf((float)gf[j][i], (float)of[i], delta);
     }
@@ -1189,7 +1190,8 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
   const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
 
   const char *qb = (const char *)((const T *)a.q + b * a.q_sb + (long long)kh * a.g * a.q_sh);
-  const char *gb = (const char *)((const T *)a.dout + ((long long)b * a.lq * a.h + kh * a.g) * a.d);
+  const char *gb = (const char *)((const T *)a.dout_dma +
+                                  ((long long)b * a.lq * a.h + kh * a.g) * a.gd);
   // row r0 + row of the tile is query l0 + l, head hd of the group; (rem + row) / g by a multiplication
   // (exact: below 64 + g <= 192, times a reciprocal rounded up by less than g / 65 536)
   const int inv_g = (65536 + a.g - 1) / a.g;
@@ -1197,7 +1199,7 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
     char *qt = smem + buf * 2 * TB, *gt = qt + TB;
     const int l0 = r0 / a.g, rem = r0 - l0 * a.g;
     const i32x4_t qr = dma_rsrc(qb + 2 * (l0 * a.q_sl), kFar);
-    const i32x4_t gr = dma_rsrc(gb + 2 * ((long long)l0 * a.h * a.d), kFar);
+    const i32x4_t gr = dma_rsrc(gb + 2 * ((long long)l0 * a.h * a.gd), kFar);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = i * THREADS + tid, row = e / Dma<D>::UNITS;
@@ -1206,7 +1208,7 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
       const bool in = r0 + row < rend && 8 * u < a.d;
       dma16(qr, in ? 2 * (l * (int)a.q_sl + hd * (int)a.q_sh + 8 * u) : kFar,
             qt + (i * THREADS + (tid & ~63)) * 16);
-      dma16(gr, in ? 2 * ((l * a.h + hd) * a.d + 8 * u) : kFar,
+      dma16(gr, in ? 2 * ((l * a.h + hd) * a.gd + 8 * u) : kFar,
             gt + (i * THREADS + (tid & ~63)) * 16);
     }
     if (w < 2) {                                 // lse, D of the rows
@@ -1273,6 +1275,32 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
     }
 }
 
+// (batch, length, head, d) rows that do not lie on 16-byte boundaries in whole units -> contiguous ones
+// that do, zeros behind them; up to four tensors (blockIdx.y)
+struct XaPack {
+  struct One {
+    const void *src;
+    void *dst;
+    long long sb, sl, sh;
+    int len, heads;
+  } op[4];
+  int b, d;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void cross_attention_pack_kernel(XaPack a) {
+  const XaPack::One o = a.op[blockIdx.y];
+  const int units = up8(a.d) / 8;
+  const long long total = (long long)a.b * o.len * o.heads * units;
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total;
+       e += (long long)gridDim.x * 256) {
+    const long long row = e / units, bl = row / o.heads;
+    const int c = (int)(e - row * units) * 8, h = (int)(row - bl * o.heads);
+    const long long b = bl / o.len, l = bl - b * o.len;
+    reinterpret_cast<typename Elem<T>::Vec *>(o.dst)[e] =
+        load_row((const T *)o.src + b * o.sb + l * o.sl + h * o.sh, c, a.d);
+  }
+}
+
 // ------------------------------------------------------------------------------------ host
 constexpr int kFewRows = 32;     // one tile of rows: the waves split the keys instead
 
@@ -1299,80 +1327,121 @@ bool few(int rows) { return rows <= kFewRows; }
 int dma_rows_per(const XaArgs &a) {
   return a.d > 64 && (long long)cdiv(a.rows, 256) * a.b * a.hk >= 512 ? 256 : 128;
 }
-Shares row_shares(const XaArgs &a, bool dma) {   // forward, dq: over the keys
-  return shares(cdiv(a.rows, few(a.rows) ? 32 : dma ? dma_rows_per(a) : 128), (long long)a.b * a.hk,
-                a.lk, 128, 256);
-}
-bool aligned(const void *p, long long sb, long long sl, long long sh) {
-  return ((uintptr_t)p & 15) == 0 && ((sb | sl | sh) & 7) == 0 && sl <= (1 << 22);
-}
-// Can tiles of K and V go through LDS DMA?  Whole 16-byte units on 16-byte boundaries, rows apart
-// by at least a row, a tile's offsets within 31 bits.
-bool dma_ok(const XaArgs &a, int dtype) {
-  return dtype != BTR_F32 && a.d % 8 == 0 &&
-         aligned(a.k, a.k_sb, a.k_sl, a.k_sh) && aligned(a.v, a.v_sb, a.v_sl, a.v_sh) &&
-         a.k_sl >= a.d && a.v_sl >= a.d;
-}
-// ... and tiles of query and dout rows?  The same of theirs, offsets within a tile of 64 rows below
-// 2^31, and groups of at most 128.
-bool dma_rows_ok(const XaArgs &a, int dtype, const void *dout) {
-  return dtype != BTR_F32 && a.d % 8 == 0 && a.g <= 128 &&
-         aligned(a.q, a.q_sb, a.q_sl, a.q_sh) && a.q_sl >= 0 && a.q_sh >= 0 &&
-         a.q_sh <= (1 << 22) && ((uintptr_t)dout & 15) == 0 && (long long)a.h * a.d <= (1 << 22);
+// shares of the keys; rows of a tile: few of 16 bits have a forward of their own
+Shares row_shares(const XaArgs &a, int dtype, bool fwd) {
+  const int per = few(a.rows) && (fwd || dtype == BTR_F32) ? 32 : dtype == BTR_F32 ? 128 : dma_rows_per(a);
+  return shares(cdiv(a.rows, per), (long long)a.b * a.hk, a.lk, 128, 256);
 }
 Shares key_shares(const XaArgs &a) {                  // dk, dv: over the rows
   return shares(cdiv(a.lk, 128), (long long)a.b * a.hk, a.rows, 64, 128);
 }
 
+// Rows a DMA may read where they are: whole 16-byte units on 16-byte boundaries, a tile's offsets
+// below 2^31, and (keys) rows apart by at least a row.
+bool aligned(int d, const void *p, long long sb, long long sl, long long sh) {
+  return d % 8 == 0 && ((uintptr_t)p & 15) == 0 && ((sb | sl | sh) & 7) == 0 && sl <= (1 << 22) &&
+         sh <= (1 << 22) && sl >= 0 && sh >= 0;
+}
+bool key_rows_ok(const XaArgs &a, const void *p, long long sb, long long sl, long long sh) {
+  return aligned(a.d, p, sb, sl, sh) && sl >= a.d;
+}
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+size_t packed_bytes(const XaArgs &a, long long len, int heads) {
+  return align256((size_t)a.b * len * heads * up8(a.d) * 2);
+}
+// What has to be packed before the DMA kernels run: K and V, for dk / dv also q and dout.  The
+// workspace is counted with the same rule.
+template <typename F>
+void for_unaligned(const XaArgs &a, bool bwd, F f) {
+  if (!key_rows_ok(a, a.k, a.k_sb, a.k_sl, a.k_sh)) f(0);
+  if (!key_rows_ok(a, a.v, a.v_sb, a.v_sl, a.v_sh)) f(1);
+  if (bwd && !aligned(a.d, a.q, a.q_sb, a.q_sl, a.q_sh)) f(2);
+  if (bwd && !aligned(a.d, a.dout, 0, (long long)a.h * a.d, a.d)) f(3);
+}
+size_t pack_bytes(const XaArgs &a, int dtype, bool bwd) {
+  size_t n = 0;
+  if (dtype != BTR_F32)
+    for_unaligned(a, bwd, [&](int i) {
+      n += packed_bytes(a, i < 2 ? a.lk : a.lq, i < 2 ? a.hk : a.h);
+    });
+  return n;
+}
+template <typename T>
+void pack(XaArgs &a, bool bwd, char *&ws, hipStream_t hs) {
+  if constexpr (sizeof(T) == 2) {
+    XaPack pk{};
+    pk.b = a.b;
+    pk.d = a.d;
+    int n = 0;
+    long long most = 0;
+    const XaArgs in = a;
+    for_unaligned(in, bwd, [&](int i) {
+      const int len = i < 2 ? a.lk : a.lq, heads = i < 2 ? a.hk : a.h;
+      const long long sl = (long long)heads * up8(a.d), sb = sl * len, sh = up8(a.d);
+      const long long hd = (long long)in.h * in.d;
+      if (i == 0) {
+        pk.op[n++] = {in.k, ws, in.k_sb, in.k_sl, in.k_sh, len, heads};
+        a.k = ws; a.k_sb = sb; a.k_sl = sl; a.k_sh = sh;
+      } else if (i == 1) {
+        pk.op[n++] = {in.v, ws, in.v_sb, in.v_sl, in.v_sh, len, heads};
+        a.v = ws; a.v_sb = sb; a.v_sl = sl; a.v_sh = sh;
+      } else if (i == 2) {
+        pk.op[n++] = {in.q, ws, in.q_sb, in.q_sl, in.q_sh, len, heads};
+        a.q = ws; a.q_sb = sb; a.q_sl = sl; a.q_sh = sh;
+      } else {
+        pk.op[n++] = {in.dout, ws, hd * in.lq, hd, in.d, len, heads};
+        a.dout_dma = ws; a.gd = up8(a.d);
+      }
+      most = std::max(most, sb / 8 * a.b);
+      ws += packed_bytes(a, len, heads);
+    });
+    if (n && most)
+      hipLaunchKernelGGL((cross_attention_pack_kernel<T>),
+                         dim3((unsigned)std::min<long long>(4096, (most + 255) / 256), n), dim3(256),
+                         0, hs, pk);
+  }
+}
+
 template <typename T, int DP>
-void launch_fwd(const XaArgs &a, bool dma, hipStream_t hs) {
+void launch_fwd(const XaArgs &a, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
   if constexpr (sizeof(T) == 2) {
     constexpr int NT = DP / 32;
-    if (dma) {
-      if (few(a.rows))
-        hipLaunchKernelGGL((cross_attention_fwd_stream_kernel<T, NT>), grid, dim3(256), 0, hs, a);
-      else if (dma_rows_per(a) == 256)
-        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, NT, 8>), grid, dim3(512), 0, hs, a);
-      else
-        hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, NT, 4>), grid, dim3(256), 0, hs, a);
-      return;
-    }
+    if (few(a.rows))
+      hipLaunchKernelGGL((cross_attention_fwd_stream_kernel<T, NT>), grid, dim3(256), 0, hs, a);
+    else if (dma_rows_per(a) == 256)
+      hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, NT, 8>), grid, dim3(512), 0, hs, a);
+    else
+      hipLaunchKernelGGL((cross_attention_fwd_dma_kernel<T, NT, 4>), grid, dim3(256), 0, hs, a);
+  } else {
+    if (few(a.rows))
+      hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 1, 4, 1>), grid, dim3(256), 0, hs, a);
+    else
+      hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 4, 1, 2>), grid, dim3(256), 0, hs, a);
   }
-  if (few(a.rows))
-    hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 1, 4, 1, 1>), grid, dim3(256), 0, hs, a);
-  else
-    hipLaunchKernelGGL((cross_attention_fwd_kernel<T, DP, 4, 1, 2, 1>), grid, dim3(256), 0, hs, a);
 }
 template <typename T, int DP>
-void launch_bwd_q(const XaArgs &a, bool dma, hipStream_t hs) {
+void launch_bwd_q(const XaArgs &a, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
   if constexpr (sizeof(T) == 2) {
-    constexpr int NT = DP / 32;
-    if (dma && !few(a.rows)) {
-      if (dma_rows_per(a) == 256)
-        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, NT, 8>), grid, dim3(512), 0, hs, a);
-      else
-        hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, NT, 4>), grid, dim3(256), 0, hs, a);
-      return;
-    }
+    if (dma_rows_per(a) == 256)
+      hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, DP / 32, 8>), grid, dim3(512), 0, hs, a);
+    else
+      hipLaunchKernelGGL((cross_attention_bwd_q_dma_kernel<T, DP / 32, 4>), grid, dim3(256), 0, hs, a);
+  } else {
+    if (few(a.rows))
+      hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 1, 4, 1>), grid, dim3(256), 0, hs, a);
+    else
+      hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 4, 1, 2>), grid, dim3(256), 0, hs, a);
   }
-  if (few(a.rows))
-    hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 1, 4, 1>), grid, dim3(256), 0, hs, a);
-  else
-    hipLaunchKernelGGL((cross_attention_bwd_q_kernel<T, DP, 4, 1, 2>), grid, dim3(256), 0, hs, a);
 }
 template <typename T, int DP>
-void launch_bwd_kv(const XaArgs &a, bool dma, hipStream_t hs) {
+void launch_bwd_kv(const XaArgs &a, hipStream_t hs) {
   const dim3 grid((unsigned)((long long)a.tiles * a.b * a.hk * a.nsplit));
-  if constexpr (sizeof(T) == 2) {
-    if (dma) {
-      hipLaunchKernelGGL((cross_attention_bwd_kv_dma_kernel<T, DP / 32, 4>), grid, dim3(256), 0, hs,
-                         a);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((cross_attention_bwd_kv_kernel<T, DP>), grid, dim3(256), 0, hs, a);
+  if constexpr (sizeof(T) == 2)
+    hipLaunchKernelGGL((cross_attention_bwd_kv_dma_kernel<T, DP / 32, 4>), grid, dim3(256), 0, hs, a);
+  else
+    hipLaunchKernelGGL((cross_attention_bwd_kv_kernel<T, DP>), grid, dim3(256), 0, hs, a);
 }
 
 #define BTR_XA_WIDTH(FN, ...)                  \
@@ -1383,8 +1452,6 @@ void launch_bwd_kv(const XaArgs &a, bool dma, hipStream_t hs) {
     else FN<T, 128>(__VA_ARGS__);              \
   } while (0)
 
-size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
-
 int check(const char *what, const btr_cross_attention_t *p, XaArgs &a) {
   BTR_REQUIRE(p, "%s: null description", what);
   BTR_REQUIRE(p->dtype >= BTR_F32 && p->dtype <= BTR_F16, "%s: unknown element type %d", what,
@@ -1394,6 +1461,8 @@ int check(const char *what, const btr_cross_attention_t *p, XaArgs &a) {
               "%s: batch %d, queries %d, keys %d, heads %d on %d key heads", what, p->b, p->lq,
               p->lk, p->h, p->hk);
   BTR_REQUIRE(p->d >= 1 && p->d <= 128, "%s: head width %d (1 .. 128)", what, p->d);
+  BTR_REQUIRE(p->h / p->hk <= 128 && (long long)p->h * up8(p->d) <= (1 << 22),
+              "%s: %d heads on %d key heads", what, p->h, p->hk);
   BTR_REQUIRE(p->scale > 0.f && p->scale < INFINITY, "%s: scale %g", what, p->scale);
   a = XaArgs{};
   a.b = p->b; a.lq = p->lq; a.lk = p->lk; a.h = p->h; a.hk = p->hk; a.g = p->h / p->hk; a.d = p->d;
@@ -1418,18 +1487,17 @@ int check(const char *what, const btr_cross_attention_t *p, XaArgs &a) {
 }
 
 size_t fwd_bytes(const XaArgs &a, int dtype) {
-  const Shares s = row_shares(a, dma_ok(a, dtype));
-  if (s.n == 1) return 0;
-  const size_t n = (size_t)s.n * a.b * a.hk * a.rows;
-  return align256(n * a.d * 4) + align256(n * 8);
+  const Shares s = row_shares(a, dtype, true);
+  const size_t n = s.n == 1 ? 0 : (size_t)s.n * a.b * a.hk * a.rows;
+  return pack_bytes(a, dtype, false) + align256(n * a.d * 4) + align256(n * 8);
 }
-size_t bwd_bytes(const XaArgs &a, int dtype) {   // D, then the shares of dq or of dk, dv
+size_t bwd_bytes(const XaArgs &a, int dtype) {   // D, what is packed, then the shares of dq or of dk, dv
   const size_t delta = align256((size_t)a.b * a.hk * a.rows * 4);
-  const Shares q = row_shares(a, dma_ok(a, dtype)), k = key_shares(a);
+  const Shares q = row_shares(a, dtype, false), k = key_shares(a);
   size_t nq = 0, nk = 0;
   if (q.n > 1) nq = align256((size_t)q.n * a.b * a.hk * a.rows * a.d * 4);
   if (k.n > 1) nk = 2 * align256((size_t)k.n * a.b * a.lk * a.hk * a.d * 4);
-  return delta + std::max(nq, nk);
+  return delta + pack_bytes(a, dtype, true) + std::max(nq, nk);
 }
 
 }  // namespace
@@ -1443,9 +1511,11 @@ extern "C" size_t btr_cross_attention_fwd_workspace_bytes(const btr_cross_attent
   return fwd_bytes(a, p->dtype);
 }
 
-extern "C" size_t btr_cross_attention_bwd_workspace_bytes(const btr_cross_attention_t *p) {
+extern "C" size_t btr_cross_attention_bwd_workspace_bytes(const btr_cross_attention_t *p,
+                                                          const void *dout) {
   XaArgs a;
   if (check("cross_attention", p, a) != BTR_OK) return 0;
+  a.dout = dout;
   return bwd_bytes(a, p->dtype);
 }
 
@@ -1462,16 +1532,17 @@ extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out
               "cross_attention_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.out = out;
   a.lse = lse;
-  const bool dma = dma_ok(a, p->dtype);
-  const Shares s = row_shares(a, dma);
+  hipStream_t hs = as_stream(stream);
+  char *ws = (char *)workspace;
+  BTR_DISPATCH_DTYPE(p->dtype, pack<T>(a, false, ws, hs));
+  const Shares s = row_shares(a, p->dtype, true);
   a.tiles = s.tiles; a.nsplit = s.n; a.chunk = s.chunk;
   const long long nrow = (long long)a.b * a.hk * a.rows;
   if (s.n > 1) {
-    a.part = (float *)workspace;
-    a.part2 = (float *)((char *)workspace + align256((size_t)s.n * nrow * a.d * 4));
+    a.part = (float *)ws;
+    a.part2 = (float *)(ws + align256((size_t)s.n * nrow * a.d * 4));
   }
-  hipStream_t hs = as_stream(stream);
-  BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_fwd, a, dma, hs));
+  BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_fwd, a, hs));
   if (s.n > kFewShares)
     BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_join_kernel<T>),
                                                     dim3((unsigned)nrow), dim3(256), 0, hs, a));
@@ -1492,22 +1563,24 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
   if (a.b == 0) return BTR_OK;
   BTR_REQUIRE((a.rows == 0 || (out && lse && dout && dq)) && (a.lk == 0 || (dk && dv)),
               "cross_attention_bwd: null pointer");
+  a.dout = a.dout_dma = dout;
+  a.gd = a.d;
   const size_t need = bwd_bytes(a, p->dtype);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "cross_attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.out = const_cast<void *>(out);
   a.lse = const_cast<float *>(lse);
-  a.dout = dout;
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.delta = (float *)workspace;
-  float *ws = (float *)((char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4));
+  char *at = (char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4);
   hipStream_t hs = as_stream(stream);
+  BTR_DISPATCH_DTYPE(p->dtype, pack<T>(a, true, at, hs));
+  float *ws = (float *)at;
   if (a.rows > 0) {
-    const bool dma = dma_ok(a, p->dtype);
-    const Shares s = row_shares(a, dma);
+    const Shares s = row_shares(a, p->dtype, false);
     XaArgs q = a;
     q.tiles = s.tiles; q.nsplit = s.n; q.chunk = s.chunk; q.part = ws;
-    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_q, q, dma, hs));
+    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_q, q, hs));
     if (s.n > 1) {
       const long long n = (long long)a.b * a.hk * a.rows * a.d;
       const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
@@ -1522,7 +1595,7 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
     const long long n = (long long)a.b * a.lk * a.hk * a.d;
     k.tiles = s.tiles; k.nsplit = s.n; k.chunk = s.chunk; k.part = ws;
     k.part2 = (float *)((char *)ws + align256((size_t)s.n * n * 4));
-    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_kv, k, dma_rows_ok(a, p->dtype, dout), hs));
+    BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_kv, k, hs));
     if (s.n > 1) {
       const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
       BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_sum_kernel<T, false>),

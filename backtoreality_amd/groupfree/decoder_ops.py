@@ -292,7 +292,7 @@ class _CrossAttention(Function):
         dk = torch.empty(k.shape, dtype=dtype, device=dev)
         dv = torch.empty(v.shape, dtype=dtype, device=dev)
         addr = _addressof(p)
-        nbytes = _lib.btr_cross_attention_bwd_workspace_bytes(addr)
+        nbytes = _lib.btr_cross_attention_bwd_workspace_bytes(addr, dout.data_ptr())
         ws = _workspace(nbytes, dev)
         _launch(q, _lib.btr_cross_attention_bwd, addr, out.data_ptr(), lse.data_ptr(),
                 dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), nbytes)
@@ -304,8 +304,8 @@ class _CrossAttention(Function):
 def cross_attention(query, key, value, key_lengths=None, key_padding_mask=None, scale=None):
     """softmax(scale query key^T) value per head.
 
-    query (B, Lq, H, D), key and value (B, Lk, Hk, D), H a multiple of Hk (query head i reads key
-    head i // (H // Hk)), D <= 128; result (B, Lq, H, D).  Of batch entry b the keys from
+    query (B, Lq, H, D), key and value (B, Lk, Hk, D), H a multiple of Hk, at most 128 times
+    it (query head i reads key head i // (H // Hk)), D <= 128; result (B, Lq, H, D).  Of batch entry b the keys from
     key_lengths[b] (int32 (B), on the device) on and those where key_padding_mask (bool (B, Lk)) is
     True take no part, whatever they hold; a query left without keys gets zeros, and gives none of
     its gradient to anybody.  scale: D ** -0.5 by default, positive."""
@@ -319,7 +319,7 @@ def cross_attention(query, key, value, key_lengths=None, key_padding_mask=None, 
     if key.shape != value.shape or kB != B or kD != D:
         _refuse("cross_attention: query %s, key %s, value %s", tuple(query.shape), tuple(key.shape),
                 tuple(value.shape))
-    if Hk < 1 or H < 1 or H % Hk:
+    if Hk < 1 or H < 1 or H % Hk or H // Hk > 128:
         _refuse("cross_attention: %d heads on %d key heads", H, Hk)
     if not 1 <= D <= 128:
         _refuse("cross_attention: head width %d (1 .. 128)", D)

@@ -142,7 +142,7 @@ _SIGNATURES = {
     "btr_linear_bwd": (_ci, [_vp] * 3 + [_ll] + [_vp] * 4 + [_sz, _vp]),
     "btr_cross_attention_fwd_workspace_bytes": (_sz, [_vp]),
     "btr_cross_attention_fwd": (_ci, [_vp] * 4 + [_sz, _vp]),
-    "btr_cross_attention_bwd_workspace_bytes": (_sz, [_vp]),
+    "btr_cross_attention_bwd_workspace_bytes": (_sz, [_vp, _vp]),
     "btr_cross_attention_bwd": (_ci, [_vp] * 8 + [_sz, _vp]),
     # whole-layer entry points (csrc/sa_layer.hip): description + plan by address
     "btr_sa_layer_plan": (_ci, [_vp, _vp]),

@@ -86,11 +86,11 @@ def test_cross_attention_entry_refuses():
     def fwd(p, out=PTR, ws=PTR, nbytes=1 << 30):
         return lib.btr_cross_attention_fwd(ctypes.addressof(p), out, None, ws, nbytes, None)
     for bad in (dict(dtype=7), dict(b=-1), dict(lq=-1), dict(lk=-1), dict(h=0), dict(hk=0), dict(hk=3),
-                dict(d=0), dict(d=129), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
+                dict(h=258, hk=2), dict(d=0), dict(d=129), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
                 dict(scale=float("nan")), dict(q=None), dict(k=None), dict(v=None), dict(lq=2 ** 30)):
         p = desc(**bad)
         assert fwd(p) == -1 and "cross_attention_fwd" in _error(), bad
-        assert lib.btr_cross_attention_bwd_workspace_bytes(ctypes.addressof(p)) == 0
+        assert lib.btr_cross_attention_bwd_workspace_bytes(ctypes.addressof(p), PTR) == 0
     assert lib.btr_cross_attention_fwd(None, PTR, None, PTR, 1 << 30, None) == -1
     assert fwd(desc(), out=None) == -1
     long = desc(lq=1, lk=100000)                         # split over the keys: needs a workspace
