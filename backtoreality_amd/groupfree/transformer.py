@@ -5,11 +5,24 @@ the position-augmented tensors as `value`).  `torch.nn.MultiheadAttention` is th
 reference vendors a copy of (models/multi_head_attention.py), same parameter names; on the
 GPU the whole layer is one library call (groupfree/fused_decoder.py -> csrc/decoder.hip); the
 op-by-op form below (attention core through groupfree/fused_attention.py) is the CPU path and
-what `BTR_FUSED_DECODER=0` selects."""
+what `BTR_FUSED_DECODER=0` selects.  Layers in bfloat16 / float16 and keys with padding
+(`key_padding_mask`) run on the operators of groupfree/decoder_ops.py."""
+import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import fused_attention, fused_decoder
+from . import decoder_ops, fused_attention, fused_decoder
+
+_ACTIVATIONS = {F.relu: "relu", F.gelu: "gelu"}
+
+
+def _mha_covered(mha, dtype):
+    """Packed projections of one width in the layer's type, nothing appended to the keys, and no
+    dropout on the attention weights in this call."""
+    return (isinstance(mha, nn.MultiheadAttention) and mha._qkv_same_embed_dim and
+            mha.bias_k is None and mha.bias_v is None and not mha.add_zero_attn and
+            not getattr(mha, "batch_first", False) and mha.head_dim <= 128 and
+            (mha.dropout == 0 or not mha.training) and mha.in_proj_weight.dtype == dtype)
 
 
 class TransformerDecoderLayer(nn.Module):
@@ -33,12 +46,60 @@ class TransformerDecoderLayer(nn.Module):
         self.self_posembed = self_posembed
         self.cross_posembed = cross_posembed
 
-    def forward(self, query, key, query_pos, key_pos):
-        """query (B,C,Pq), key (B,C,Pk), query_pos (B,Pq,3|6), key_pos (B,Pk,3) -> (B,C,Pq)."""
+    def _ops_covered(self, query, key, key_padding_mask):
+        """Does groupfree/decoder_ops.py run this call?  Padded keys and 16-bit layers; float32
+        without padding has the whole-layer call."""
+        return (query.is_cuda and query.dtype in (torch.float32, torch.bfloat16, torch.float16) and
+                (key_padding_mask is not None or query.dtype != torch.float32) and
+                key.dtype == query.dtype and self.activation in _ACTIVATIONS and
+                _mha_covered(self.self_attn, query.dtype) and
+                _mha_covered(self.multihead_attn, query.dtype))
+
+    def _forward_ops(self, query, key, q_pos, k_pos, key_padding_mask):
+        """The layer on (B, P, C) rows: every projection one kernel with its bias (and activation),
+        every residual addition inside its norm."""
+        def norm(n, branch, x):
+            return decoder_ops.layer_norm(branch, n.weight, n.bias, residual=x, eps=n.eps)
+
+        def attend(mha, rows_q, rows_k, mask=None):
+            heads, width = mha.num_heads, mha.head_dim
+            W, b = mha.in_proj_weight, mha.in_proj_bias
+            E = mha.embed_dim
+            if rows_k is None:
+                q, k, v = decoder_ops.linear(rows_q, W, b).unflatten(2, (3, heads, width)).unbind(2)
+            else:
+                q = decoder_ops.linear(rows_q, W[:E], None if b is None else b[:E])
+                q = q.unflatten(2, (heads, width))
+                k, v = decoder_ops.linear(rows_k, W[E:], None if b is None else b[E:]).unflatten(
+                    2, (2, heads, width)).unbind(2)
+            out = decoder_ops.cross_attention(q, k, v, key_padding_mask=mask)
+            return decoder_ops.linear(out.flatten(2), mha.out_proj.weight, mha.out_proj.bias)
+
+        x, memory = query.transpose(1, 2).contiguous(), key.transpose(1, 2)
+        pos = None if q_pos is None else q_pos.transpose(1, 2)
+        qp = x if pos is None else x + pos
+        x = norm(self.norm1, self.dropout1(attend(self.self_attn, qp, None)), x)
+        qp = x if pos is None else x + pos
+        kp = memory if k_pos is None else memory + k_pos.transpose(1, 2)
+        x = norm(self.norm2, self.dropout2(attend(self.multihead_attn, qp, kp, key_padding_mask)), x)
+        h = decoder_ops.linear(x, self.linear1.weight, self.linear1.bias,
+                               activation=_ACTIVATIONS[self.activation])
+        f = decoder_ops.linear(self.dropout(h), self.linear2.weight, self.linear2.bias)
+        return norm(self.norm3, self.dropout3(f), x).transpose(1, 2)
+
+    def forward(self, query, key, query_pos, key_pos, key_padding_mask=None):
+        """query (B,C,Pq), key (B,C,Pk), query_pos (B,Pq,3|6), key_pos (B,Pk,3) -> (B,C,Pq).
+        key_padding_mask (B,Pk) bool or None: True marks keys that take no part, as in
+        `nn.MultiheadAttention`; every scene needs a key that is not padding unless the layer runs on
+        the library's operators, where a scene without keys gets a cross-attention of zero."""
         q_pos = self.self_posembed(query_pos) if self.self_posembed is not None else None
         k_pos = self.cross_posembed(key_pos) if self.cross_posembed is not None else None
+        if self._ops_covered(query, key, key_padding_mask):
+            return self._forward_ops(query, key, q_pos, k_pos, key_padding_mask)
         # the whole layer as one library call (csrc/decoder.hip) when it covers the configuration
-        out = fused_decoder.layer_forward(self, query, key, q_pos, k_pos)
+        out = None
+        if key_padding_mask is None:
+            out = fused_decoder.layer_forward(self, query, key, q_pos, k_pos)
         if out is not None:
             return out
         q_pos = q_pos.permute(2, 0, 1) if q_pos is not None else None
@@ -56,9 +117,12 @@ class TransformerDecoderLayer(nn.Module):
 
         qp = query if q_pos is None else query + q_pos
         kp = key if k_pos is None else key + k_pos
-        att = fused_attention.mha_forward(self.multihead_attn, qp, kp)
+        att = None
+        if key_padding_mask is None:
+            att = fused_attention.mha_forward(self.multihead_attn, qp, kp)
         if att is None:
-            att = self.multihead_attn(query=qp, key=kp, value=kp)[0]
+            att = self.multihead_attn(query=qp, key=kp, value=kp,
+                                      key_padding_mask=key_padding_mask)[0]
         query = self.norm2(query + self.dropout2(att))
 
         ffn = self.linear2(self.dropout(self.activation(self.linear1(query))))

@@ -103,3 +103,18 @@ def test_cross_attention_entry_refuses():
                                        1 << 30, None) == -1
     assert lib.btr_cross_attention_bwd(ctypes.addressof(p), PTR, PTR, PTR, PTR, PTR, PTR, PTR, 0,
                                        None) == -1 and "workspace" in _error()
+
+
+def test_decoder_layer_masks_padded_keys_on_the_cpu():
+    """key_padding_mask on the op-by-op path: the same as leaving the padded keys out."""
+    from backtoreality_amd.groupfree.transformer import TransformerDecoderLayer
+    torch.manual_seed(0)
+    layer = TransformerDecoderLayer(32, 4, 64, 0.0).double()
+    query, key = torch.randn(1, 32, 5).double(), torch.randn(1, 32, 9).double()
+    mask = torch.zeros(1, 9, dtype=torch.bool)
+    mask[0, [2, 6, 7]] = True
+    a = layer(query, key, None, None, key_padding_mask=mask)
+    b = layer(query, key[:, :, ~mask[0]], None, None)
+    assert torch.allclose(a, b, rtol=0, atol=1e-12)
+    assert torch.equal(layer(query, key, None, None),
+                       layer(query, key, None, None, key_padding_mask=torch.zeros_like(mask)))

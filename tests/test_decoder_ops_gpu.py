@@ -435,3 +435,101 @@ def test_double_backward_is_refused(cuda):
     (g,) = torch.autograd.grad(ops.layer_norm(x).pow(2).sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+# ------------------------------------------------------------------------ the decoder layer on them
+def _layer(cuda, dtype, activation="relu", E=96, heads=4, posembed=True):
+    import torch.nn as nn
+    from backtoreality_amd.groupfree.transformer import TransformerDecoderLayer
+    torch.manual_seed(3)
+
+    class Position(nn.Module):        # (B, P, 3) -> (B, E, P)
+        def __init__(self):
+            super().__init__()
+            self.map = nn.Linear(3, E)
+
+        def forward(self, xyz):
+            return self.map(xyz).transpose(1, 2)
+    layer = TransformerDecoderLayer(E, heads, 4 * E, 0.0, activation,
+                                    self_posembed=Position() if posembed else None,
+                                    cross_posembed=Position() if posembed else None)
+    with torch.no_grad():
+        for p in layer.parameters():
+            if p.dim() == 1:
+                p.add_(torch.randn(p.shape) * 0.1)
+    return layer.to(cuda).to(dtype)
+
+
+def _layer_inputs(cuda, dtype, E=96):
+    gen = _gen(21)
+    B, Pq, Pk = 3, 70, 260
+    mask = torch.rand((B, Pk), generator=gen, device=cuda) < 0.3
+    mask[1, 100:] = True
+    return (_randn(gen, (B, E, Pq), dtype), _randn(gen, (B, E, Pk), dtype),
+            _randn(gen, (B, Pq, 3), dtype), _randn(gen, (B, Pk, 3), dtype), mask,
+            _randn(gen, (B, E, Pq), dtype))
+
+
+@pytest.mark.parametrize("activation", ["relu", "gelu"])
+@pytest.mark.parametrize("masked", [True, False])
+@pytest.mark.parametrize("dtype", ref.DTYPES, ids=str)
+def test_decoder_layer_on_the_operators(cuda, dtype, masked, activation, monkeypatch):
+    """TransformerDecoderLayer in every type, with and without padded keys, against the stock modules
+    in float64 on the CPU: output, input gradients and parameter gradients, root mean square.  Eight
+    roundings forward and as many back reach each result, amplified a few times: 60 half steps
+    (ReLU's switches next to zero included), as in the run of the three above."""
+    import copy
+    from backtoreality_amd.groupfree import decoder_ops
+    layer = _layer(cuda, dtype, activation)
+    q, k, qpos, kpos, mask, dy = _layer_inputs(cuda, dtype)
+    if not masked:
+        mask = None
+    calls = []
+    real = decoder_ops.cross_attention
+    monkeypatch.setattr(decoder_ops, "cross_attention",
+                        lambda *a, **kw: calls.append(1) or real(*a, **kw))
+    q, k = _leaf(q), _leaf(k)
+    out = layer(q, k, qpos, kpos, key_padding_mask=mask)
+    # (unpadded float32 has the whole-layer call)
+    assert len(calls) == (0 if dtype == torch.float32 and not masked else 2)
+    params = list(layer.parameters())
+    grads = torch.autograd.grad(out, [q, k] + params, dy)
+    cpu = copy.deepcopy(layer).cpu().double()
+    q64, k64 = (t.detach().cpu().double().requires_grad_(True) for t in (q, k))
+    want = cpu(q64, k64, qpos.cpu().double(), kpos.cpu().double(),
+               key_padding_mask=None if mask is None else mask.cpu())
+    grads64 = torch.autograd.grad(want, [q64, k64] + list(cpu.parameters()), dy.cpu().double())
+    names = ["out", "query", "key"] + [n for n, _ in layer.named_parameters()]
+    step = max(ref.half_step(dtype), 2.0 ** -22)
+    for name, a, b in zip(names, [out] + list(grads), [want] + list(grads64)):
+        err = float((a.detach().cpu().double() - b.detach()).pow(2).mean().sqrt())
+        assert err <= 60 * step * float(b.detach().pow(2).mean().sqrt()) + 1e-9, (name, err)
+
+
+def test_decoder_layer_ignores_what_padding_holds(cuda):
+    layer = _layer(cuda, torch.bfloat16)
+    q, k, qpos, kpos, mask, _ = _layer_inputs(cuda, torch.bfloat16)
+    mask[2] = True                                            # a scene without keys
+    with torch.no_grad():
+        a = layer(q, k, qpos, kpos, key_padding_mask=mask)
+        b = layer(q, k.masked_fill(mask[:, None], float("nan")), qpos, kpos, key_padding_mask=mask)
+    assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+def test_decoder_layer_with_attention_dropout_keeps_the_stock_core(cuda, monkeypatch):
+    """Dropout on the attention weights is not the operator's: a padded training call goes through
+    nn.MultiheadAttention, the same layer in eval mode through the operators."""
+    from backtoreality_amd.groupfree import decoder_ops
+    layer = _layer(cuda, torch.float32)
+    layer.self_attn.dropout = layer.multihead_attn.dropout = 0.1
+    q, k, qpos, kpos, mask, _ = _layer_inputs(cuda, torch.float32)
+    calls = []
+    real = decoder_ops.cross_attention
+    monkeypatch.setattr(decoder_ops, "cross_attention",
+                        lambda *a, **kw: calls.append(1) or real(*a, **kw))
+    layer.train()
+    layer(q, k, qpos, kpos, key_padding_mask=mask)
+    assert not calls
+    layer.eval()
+    layer(q, k, qpos, kpos, key_padding_mask=mask)
+    assert len(calls) == 2
