@@ -533,3 +533,109 @@ def test_decoder_layer_with_attention_dropout_keeps_the_stock_core(cuda, monkeyp
     layer.eval()
     layer(q, k, qpos, kpos, key_padding_mask=mask)
     assert len(calls) == 2
+
+
+# ------------------------------------------------------------------------------------- the edges
+def test_refusals(cuda):
+    """Wrong types, shapes and devices: RuntimeError, nothing launched."""
+    f = lambda *s, dtype=torch.float32: torch.zeros(s, device=cuda, dtype=dtype)
+    x, w = f(4, 8), f(3, 8)
+    q, k = f(2, 3, 4, 16), f(2, 5, 2, 16)
+    bad = [
+        lambda: ops.layer_norm(x.double()), lambda: ops.layer_norm(x, f(7)),
+        lambda: ops.layer_norm(x, f(8, dtype=torch.bfloat16)), lambda: ops.layer_norm(x, f(8).cpu()),
+        lambda: ops.layer_norm(x, residual=f(4, 7)), lambda: ops.layer_norm(x, eps=-1.0),
+        lambda: ops.layer_norm(f(4, 0)), lambda: ops.layer_norm(f()), lambda: ops.layer_norm(x, f(1, 8)),
+        lambda: ops.linear(x, f(3, 7)), lambda: ops.linear(x, f(8)), lambda: ops.linear(x, w.half()),
+        lambda: ops.linear(x, w, f(4)), lambda: ops.linear(x, w, activation="glu"),
+        lambda: ops.linear(x, w, residual=f(3, 4)), lambda: ops.linear(x, w, residual=f(4, 3).cpu()),
+        lambda: ops.linear(x, f(0, 8)), lambda: ops.linear(x.long(), w),
+        lambda: ops.cross_attention(q, k, f(2, 6, 2, 16)), lambda: ops.cross_attention(q[0], k, k),
+        lambda: ops.cross_attention(q, f(2, 5, 3, 16), f(2, 5, 3, 16)),
+        lambda: ops.cross_attention(q, f(1, 5, 2, 16), f(1, 5, 2, 16)),
+        lambda: ops.cross_attention(f(1, 1, 1, 129), f(1, 1, 1, 129), f(1, 1, 1, 129)),
+        lambda: ops.cross_attention(f(1, 1, 258, 8), f(1, 1, 2, 8), f(1, 1, 2, 8)),
+        lambda: ops.cross_attention(q, k.half(), k.half()),
+        lambda: ops.cross_attention(q, k, k, key_lengths=torch.zeros(2, device=cuda, dtype=torch.int64)),
+        lambda: ops.cross_attention(q, k, k, key_lengths=torch.zeros(2, dtype=torch.int32)),
+        lambda: ops.cross_attention(q, k, k, key_lengths=torch.zeros(3, device=cuda, dtype=torch.int32)),
+        lambda: ops.cross_attention(q, k, k, key_padding_mask=f(2, 5)),
+        lambda: ops.cross_attention(q, k, k, key_padding_mask=f(2, 4).bool()),
+        lambda: ops.cross_attention(q, k, k, scale=0.0),
+        lambda: ops.cross_attention(q, k, k, scale=float("nan")),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail("call %d was not refused" % i)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_offsets_beyond_32_bits(cuda, dtype):
+    """Rows so far apart that the last ones start behind element 2^31: the same bits as from a compact
+    copy."""
+    apart, n, D = 1 << 16, 34000, 64
+    wide = torch.empty((n, apart), device=cuda, dtype=dtype)      # (only the columns below are touched)
+    gen = _gen(31)
+    kv = _randn(gen, (n, 2 * D), dtype)
+    wide[:, :2 * D] = kv
+    q, dy = _randn(gen, (1, 40, 1, D), dtype), _randn(gen, (1, 40, 1, D), dtype)
+    lengths = torch.tensor([n - 3], dtype=torch.int32, device=cuda)
+    res = []
+    for src in (wide[:, :2 * D], kv):
+        k, v = (_leaf(src[:, i * D:(i + 1) * D][None, :, None]) for i in (0, 1))
+        out = ops.cross_attention(q, k, v, key_lengths=lengths)
+        res.append([out] + list(torch.autograd.grad(out, [k, v], dy)))
+        one = ops.cross_attention(q[:, :1], k.detach(), v.detach(), key_lengths=lengths)
+        x, w = _leaf(src), _leaf(_randn(_gen(32), (24, 2 * D), dtype))
+        y = ops.linear(x, w, activation="relu")
+        res[-1] += [one, y] + list(torch.autograd.grad(y, [x, w], torch.ones_like(y)))
+        y = ops.layer_norm(x)
+        res[-1] += [y, torch.autograd.grad(y, [x], src)[0]]
+    for i, (a, b) in enumerate(zip(*res)):
+        assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES, ids=str)
+def test_one_tensor_in_several_places(cuda, dtype):
+    """The same leaf as input and residual, as query, key and value, as input and weight: gradients
+    add up."""
+    gen = _gen(33)
+    x = _leaf(_randn(gen, (24, 24), dtype))
+    dy = _randn(gen, (24, 24), dtype)
+    u = ref.half_step(dtype)
+    two = lambda want, i, j: (want[i][1] + want[j][1], want[i][2] + want[j][2] + 2 * u * (
+        want[i][1].abs() + want[j][1].abs()))                     # torch adds the rounded two
+    y = ops.layer_norm(x, residual=x)
+    (g,) = torch.autograd.grad(y, [x], dy)
+    ref.close("norm", g, *two(ref.layer_norm(x, None, None, x, 1e-5, dy), 1, 1))
+    y = ops.linear(x, x)
+    (g,) = torch.autograd.grad(y, [x], dy)
+    ref.close("linear", g, *two(ref.linear(x, x, None, None, None, dy), 1, 2))
+    s = _leaf(_randn(gen, (2, 40, 3, 16), dtype))
+    dy = _randn(gen, (2, 40, 3, 16), dtype)
+    out = ops.cross_attention(s, s, s)
+    (g,) = torch.autograd.grad(out, [s], dy)
+    want = ref.cross_attention(s, s, s, None, None, 0.25, dy)
+    total = sum(w[1] for w in want[1:])
+    ref.close("attention", g, total, sum(w[2] for w in want[1:]) + 4 * u * sum(w[1].abs() for w in want[1:]))
+
+
+def test_gradients_beside_a_living_graph_of_the_same_leaves(cuda):
+    """Two forwards of the same leaves alive at once, taken back in either order."""
+    t, run = _three(_gen(34), torch.bfloat16, cuda)
+    dy = _randn(_gen(35), (2, 50, 128), torch.bfloat16)
+    a, b = run(t), run(t)
+    gb = torch.autograd.grad(b, list(t.values()), dy)
+    ga = torch.autograd.grad(a, list(t.values()), dy)
+    for x, y in zip(ga, gb):
+        assert torch.equal(x, y)
+
+
+def test_a_result_changed_in_place_is_noticed(cuda):
+    """ReLU's backward reads the result: autograd refuses if it was overwritten."""
+    x, w = torch.randn((8, 8), device=cuda, requires_grad=True), torch.randn((8, 8), device=cuda)
+    y = ops.linear(x, w, activation="relu")
+    y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
