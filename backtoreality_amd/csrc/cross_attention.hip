@@ -1308,15 +1308,33 @@ struct Shares {
   int tiles, n, chunk;
 };
 
-// Shares of the long axis: one where the tiles alone give every CU two workgroups; else enough for
-// about four per CU, none shorter than `least`.
-Shares shares(int tiles, long long bh, int length, int step, int least) {
+// Shares of the long axis where the tiles alone do not fill the `slots` of resident workgroups, none
+// shorter than `least`: their partial sums are as large as the result each, so not more of them than
+// the rounds of workgroups call for -- the time of the rounds against 1 % of the whole per share (3
+// x 1 777 keys, 999 rows of 80 columns, f16: 7 shares dk / dv 73 us with their sum, 3 shares 53).
+// Not where the slots are full: 1 024 tiles on 768 in three shares cost 60 us of joins to save none.
+Shares shares(int tiles, long long bh, int length, int step, int least, int slots) {
   const long long base = std::max<long long>(1, tiles * bh);
-  long long n = 1;
-  if (base < 512) n = std::min<long long>((1024 + base - 1) / base, length / least);
-  n = std::max<long long>(1, n);
-  int chunk = cdiv(length, n);
-  chunk = std::max(step, cdiv(chunk, step) * step);
+  const long long most = base >= slots ? 1 : std::min<long long>(64, length / least);
+  long long best = 1;
+  double time = 1e30;
+  for (long long n = 1; n <= std::max<long long>(1, most); ++n) {
+    const double t = (double)((base * n + slots - 1) / slots) / n + 0.01 * n;
+    if (t < time) {
+      time = t;
+      best = n;
+    }
+  }
+  const int chunk = std::max(step, cdiv(cdiv(length, best), step) * step);
+  return {tiles, std::max(1, cdiv(length, chunk)), chunk};
+}
+// A few rows' forward streams the keys: about four workgroups per CU, which also evens out batch
+// entries of unequal length.
+Shares stream_shares(int tiles, long long bh, int length) {
+  const long long base = std::max<long long>(1, tiles * bh);
+  const long long n = std::max<long long>(
+      1, std::min<long long>(base < 512 ? (1024 + base - 1) / base : 1, length / 256));
+  const int chunk = std::max(128, cdiv(cdiv(length, n), 128) * 128);
   return {tiles, std::max(1, cdiv(length, chunk)), chunk};
 }
 bool few(int rows) { return rows <= kFewRows; }
@@ -1327,15 +1345,18 @@ bool few(int rows) { return rows <= kFewRows; }
 int dma_rows_per(const XaArgs &a) {
   return a.d > 64 && (long long)cdiv(a.rows, 256) * a.b * a.hk >= 512 ? 256 : 128;
 }
-// shares of the keys; rows of a tile: few of 16 bits have a forward of their own
+// forward, dq: over the keys
 Shares row_shares(const XaArgs &a, int dtype, bool fwd) {
-  const int per = few(a.rows) && (fwd || dtype == BTR_F32) ? 32 : dtype == BTR_F32 ? 128 : dma_rows_per(a);
-  return shares(cdiv(a.rows, per), (long long)a.b * a.hk, a.lk, 128, 256);
+  const long long bh = (long long)a.b * a.hk;
+  if (few(a.rows) && (fwd || dtype == BTR_F32)) return stream_shares(1, bh, a.lk);
+  const int per = dtype == BTR_F32 ? 128 : dma_rows_per(a);
+  const int cu = dtype == BTR_F32 ? 1 : per == 256 ? 1 : a.d <= 64 ? 3 : 2;   // workgroups it holds
+  return shares(cdiv(a.rows, per), bh, a.lk, 128, 256, 256 * cu);
 }
-Shares key_shares(const XaArgs &a) {                  // dk, dv: over the rows
-  return shares(cdiv(a.lk, 128), (long long)a.b * a.hk, a.rows, 64, 128);
+// dk, dv: over the rows; two workgroups a CU for heads of up to 64 columns, one for wider ones
+Shares key_shares(const XaArgs &a) {
+  return shares(cdiv(a.lk, 128), (long long)a.b * a.hk, a.rows, 64, 128, a.d <= 64 ? 512 : 256);
 }
-
 // Rows a DMA may read where they are: whole 16-byte units on 16-byte boundaries, a tile's offsets
 // below 2^31, and (keys) rows apart by at least a row.
 bool aligned(int d, const void *p, long long sb, long long sl, long long sh) {
