@@ -25,8 +25,13 @@
 // transpose read (16-bit) or 4-byte reads (f32).
 //
 // Numbers: scores, maxima, sums, O, dq, dk, dv accumulate in f32.  For 16-bit inputs P and dS are
-// rounded to the input type where they enter the matrix instructions (relative error half an
-// ulp per term; P <= 1).  f32 runs on the f32 matrix instructions, nothing is rounded below 32 bits.
+// rounded to the input type where they enter the matrix instructions (relative error half an ulp
+// per term).  float16 has five bits of exponent, too few for a backward pass as it stands -- a P of
+// 16 384 even keys and a dS of small dout are subnormal or nothing, a dS of large dout infinite -- so
+// there P is rounded as 2^15 P, and dS times a power of two: for dq each row's, from its largest
+// |dout|, for dk / dv each key's, from the largest |dout| of the rows and its own largest |v|.  All
+// are taken out of the f32 sums again.  f32 runs on the f32 matrix instructions, nothing is rounded
+// below 32 bits.
 #include <algorithm>
 #include <cstdint>
 
@@ -51,8 +56,10 @@ struct XaArgs {
   const unsigned char *mask;                     // (b, lk), nonzero = padding, or NULL
   long long mask_sb;
   void *out;                                     // (b, lq, h, d)
-  float *lse;      // (b * hk, rows): log2 of the row's sum of exp2(scale_log2 * s); +inf: no key
+  float *lse;      // (b * hk, rows): log2 of the row's sum of exp2(scale_log2 * s); +inf: no key;
+                   // float16: less kPExp
   float *delta;    // (b * hk, rows): D
+  float *dout_max; // (b * hk, ceil(rows / 32)): the largest |dout| of 32 rows (float16)
   void *dq, *dk, *dv;                            // contiguous, shaped like q, k, v
   float scale, scale_log2;
   int tiles, nsplit, chunk;                      // workgroup tiles, shares of the long axis, its length
@@ -265,6 +272,23 @@ __device__ __forceinline__ void store4(T *row, int c, int d, const float (&v)[4]
   }
 }
 
+// The powers of two of float16's backward pass.  P rounds as 2^15 P <= 32 768.  With |dout| < 2^e and
+// |v| < 2^f, |dP| < d 2^(e + f) <= 2^(7 + e + f) and |dS| <= P (1 - P) 2 |dP| <= 2^(6 + e + f): dk / dv
+// know e and f, 2^(9 - e - f) dS stays below 65 504; dq knows its row's e only: 2^(5 - e) dS does up to
+// |v| = 32 in the worst case.
+template <typename T>
+constexpr bool kHalf = false;
+template <>
+constexpr bool kHalf<_Float16> = true;
+constexpr int kPExp = 15, kDqExp = 5, kDkExp = 9;
+__device__ __forceinline__ int exp_above(float x) {   // |x| < 2^exp_above(x); 0 for 0, inf, NaN
+  return __builtin_amdgcn_frexp_expf(x);
+}
+template <typename T>
+__device__ __forceinline__ float lse_of(float m, float l) {   // l > 0, or NaN
+  return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l) - (kHalf<T> ? kPExp : 0);
+}
+
 constexpr int kMergePitch = 4;   // floats between rows beyond DP: rows land on different banks
 
 // writes row r from the transposed accumulators (lane: row, 4 consecutive columns a register quad):
@@ -294,7 +318,7 @@ __device__ __forceinline__ void finish_row(const XaArgs &a, const Rows<T> &rows,
       a.part2[2 * row] = mb;
       a.part2[2 * row + 1] = l;
     } else if (a.lse) {
-      a.lse[(long long)bh * a.rows + r] = l == 0.f ? INFINITY : mb + __builtin_amdgcn_logf(l);
+      a.lse[(long long)bh * a.rows + r] = lse_of<T>(mb, l);
     }
   }
 }
@@ -351,7 +375,7 @@ __device__ __forceinline__ void merge_rows(const XaArgs &a, const Rows<T> &rows,
       a.part2[2 * prow] = M;
       a.part2[2 * prow + 1] = L;
     } else if (a.lse) {
-      a.lse[(long long)bh * a.rows + rr] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+      a.lse[(long long)bh * a.rows + rr] = lse_of<T>(M, L);
     }
   }
 }
@@ -488,7 +512,7 @@ __global__ __launch_bounds__(256) void cross_attention_join_few_kernel(XaArgs a)
   const Rows<T> rows{a, bh / a.hk, bh % a.hk};
   const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
   store4((T *)a.out + rows.o(r), c, a.d, v4);
-  if (c == 0 && a.lse) a.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+  if (c == 0 && a.lse) a.lse[row] = lse_of<T>(M, L);
 }
 // Many shares (of few rows): a workgroup a row, the weights once into LDS, then eight groups of 32
 // threads add every eighth share, and the groups' sums are added in order.
@@ -534,7 +558,7 @@ __global__ __launch_bounds__(256) void cross_attention_join_kernel(XaArgs a) {
   const Rows<T> rows{a, bh / a.hk, bh % a.hk};
   const float v4[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
   store4((T *)a.out + rows.o(r), c, a.d, v4);
-  if (tid == 0 && a.lse) a.lse[row] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+  if (tid == 0 && a.lse) a.lse[row] = lse_of<T>(M, L);
 }
 
 // -------------------------------------------------------------------------------- backward, dq
@@ -1072,7 +1096,7 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
   const Rows<T> rows{a, b, kh};
   const int r = (tile * WR + w) * 32 + l31;
   Vec qf[2 * NT], gf[2 * NT];
-  float delta = 0.f, lse = INFINITY;
+  float delta = 0.f, lse = INFINITY, big = 0.f;
 #pragma unroll
   for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = gf[j] = Vec{};
@@ -1082,13 +1106,27 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
       gf[j] = load_row((const T *)a.dout + rows.o(r), c, a.d);
       const Vec of = load_row((const T *)a.out + rows.o(r), c, a.d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) delta = fmaf((float)gf[j][i], (float)of[i], delta);
+      for (int i = 0; i < 8; ++i) {
+        delta = fmaf((float)gf[j][i], (float)of[i], delta);
+        if (kHalf<T>) big = fmaxf(big, fabsf((float)gf[j][i]));
+      }
     }
   }
   delta += other_half(delta);
   if (r < a.rows) {
     lse = a.lse[(long long)bh * a.rows + r];
     if (split == 0 && hh == 0) a.delta[(long long)bh * a.rows + r] = delta;
+  }
+  int up = 0;                                    // float16: dS is rounded as 2^up dS
+  if constexpr (kHalf<T>) {
+    big = fmaxf(big, other_half(big));
+    up = kDqExp - exp_above(big);
+    lse += kPExp - up;
+    if (split == 0) {
+      for (int i = 1; i < 32; i <<= 1) big = fmaxf(big, __shfl_xor(big, i));
+      const int at = tile * WR + w, count = (a.rows + 31) / 32;
+      if (lane == 0 && at < count) a.dout_max[(long long)bh * count + at] = big;
+    }
   }
   f32x16_t dq[NT] = {};
   const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
@@ -1140,6 +1178,11 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
   }
   if (r >= a.rows) return;
   const long long prow = ((long long)split * a.b * a.hk + bh) * a.rows + r;
+  if constexpr (kHalf<T>) {
+    const float down = __builtin_ldexpf(1.f, -up);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) dq[nt] *= down;
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1186,6 +1229,20 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
           (const T *)a.v + b * a.v_sb + kh * a.v_sh + key * a.v_sl + c);
     }
   }
+  int up = 0;                                    // float16: dS is rounded as 2^up dS, P as 2^kPExp P
+  if constexpr (kHalf<T>) {
+    float top = 0.f, big = 0.f;
+    const float *most = a.dout_max + (long long)bh * ((a.rows + 31) / 32);
+    for (int i = rbeg / 32 + lane; i < (rend + 31) / 32; i += 64) big = fmaxf(big, most[i]);
+    for (int i = 1; i < 64; i <<= 1) big = fmaxf(big, __shfl_xor(big, i));
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf((float)vf[j][i]));
+    top = fmaxf(top, other_half(top));
+    up = kDkExp - exp_above(big) - exp_above(top);
+  }
+  const float ds_up = __builtin_ldexpf(1.f, up - kPExp);
   f32x16_t dk[NT] = {}, dv[NT] = {};
   const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
 
@@ -1243,6 +1300,7 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
           const int v = 4 * gq + i;
           p[0][v] = __builtin_amdgcn_exp2f(fmaf(p[0][v], a.scale_log2, -l4[i]));
           ds[0][v] = p[0][v] * (ds[0][v] - d4[i]);
+          if (kHalf<T>) ds[0][v] *= ds_up;
         }
       }
       dma_t<T, NT, 1>(gx, g2, tb, p, dv);
@@ -1252,6 +1310,14 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
     }
   }
   if (key >= a.lk) return;
+  if constexpr (kHalf<T>) {
+    const float down = __builtin_ldexpf(1.f, -up), p_down = __builtin_ldexpf(1.f, -kPExp);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      dk[nt] *= down;
+      dv[nt] *= p_down;
+    }
+  }
   const long long krow = (((long long)b * a.lk + key) * a.hk + kh) * a.d;
   const long long ptotal = (long long)a.b * a.lk * a.hk * a.d;
 #pragma unroll
@@ -1512,13 +1578,17 @@ size_t fwd_bytes(const XaArgs &a, int dtype) {
   const size_t n = s.n == 1 ? 0 : (size_t)s.n * a.b * a.hk * a.rows;
   return pack_bytes(a, dtype, false) + align256(n * a.d * 4) + align256(n * 8);
 }
-size_t bwd_bytes(const XaArgs &a, int dtype) {   // D, what is packed, then the shares of dq or of dk, dv
-  const size_t delta = align256((size_t)a.b * a.hk * a.rows * 4);
+size_t stats_bytes(const XaArgs &a, int dtype) { // D; float16: the largest |dout|
+  const size_t bh = (size_t)a.b * a.hk;
+  return align256(bh * a.rows * 4) +
+         (dtype == BTR_F16 ? align256(bh * ((a.rows + 31) / 32) * 4) : 0);
+}
+size_t bwd_bytes(const XaArgs &a, int dtype) {   // these, what is packed, the shares of dq or of dk, dv
   const Shares q = row_shares(a, dtype, false), k = key_shares(a);
   size_t nq = 0, nk = 0;
   if (q.n > 1) nq = align256((size_t)q.n * a.b * a.hk * a.rows * a.d * 4);
   if (k.n > 1) nk = 2 * align256((size_t)k.n * a.b * a.lk * a.hk * a.d * 4);
-  return delta + pack_bytes(a, dtype, true) + std::max(nq, nk);
+  return stats_bytes(a, dtype) + pack_bytes(a, dtype, true) + std::max(nq, nk);
 }
 
 }  // namespace
@@ -1593,7 +1663,8 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
   a.lse = const_cast<float *>(lse);
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.delta = (float *)workspace;
-  char *at = (char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4);
+  a.dout_max = (float *)((char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4));
+  char *at = (char *)workspace + stats_bytes(a, p->dtype);
   hipStream_t hs = as_stream(stream);
   BTR_DISPATCH_DTYPE(p->dtype, pack<T>(a, true, at, hs));
   float *ws = (float *)at;

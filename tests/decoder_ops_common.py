@@ -167,8 +167,11 @@ def cross_attention(q, k, v, lengths, mask, scale, dy=None):
     ep = 2 * ((D / 2 + 8) * F * size + (Lk / 16 + 40) * F)
     # ... and absolutely: the exponential instruction returns 0 for results below 2^-126, and P <= 1
     # is e^(s - max) (forward) or e^(s - max) / sum (backward) with 1 <= sum, so what is lost of a P is
-    # below 2^-126; a 16-bit P loses half the type's smallest step instead
+    # below 2^-126; a 16-bit P loses half the type's smallest step instead (backward, float16: of
+    # 2^15 P)
+    half = dtype == torch.float16
     ea = max(2.0 ** -126, tiny(dtype) if u else 0.0) * (p > 0).double()
+    ea_back = ea * 2.0 ** -15 if half else ea
     back = lambda t: t.permute(0, 2, 1, 3)
     eo = (ep + u) * (p @ V.abs()) + uo * out.abs() + tiny(dtype) + ea @ V.abs()
     res = [("out", back(out), back(eo))]
@@ -180,18 +183,26 @@ def cross_attention(q, k, v, lengths, mask, scale, dy=None):
     e_dp = (D / 2 + 8) * F * (g.abs() @ V.abs().transpose(-1, -2))
     e_delta = (g.abs() * eo).sum(-1, keepdim=True) + D * F * (g.abs() * out.abs()).sum(-1, keepdim=True)
     ds = p * (dp - delta)
-    # (dS itself is rounded once more, in steps of its own that end at 2^-126 or the type's half step)
+    # (dS itself is rounded once more, in steps of its own that end at 2^-126 or the type's half step;
+    # float16: of dS times 2^(5 - e) for dq, 2^(9 - e' - f) for dk, where 2^e, 2^e' and 2^f are above
+    # the row's, all rows' and the key's largest |dout|, |dout| and |v|: |x| < 2^e <= 2 |x|)
     e_ds = p * (ep * (dp - delta).abs() + e_dp + e_delta) + (u + 2 * F) * ds.abs() + \
-        2.0 ** -126 * (p > 0) * (dp - delta).abs() + ea
+        2.0 ** -126 * (p > 0) * (dp - delta).abs()
+    ea_q = ea_k = ea
+    if half:
+        most, vmost = g.abs().amax(-1, keepdim=True), V.abs().amax(-1)[:, :, None]
+        none = lambda t: torch.where(t > 0, 2 * t, torch.ones_like(t))        # (0: 2^0)
+        ea_q = ea * none(most) * 2.0 ** -5
+        ea_k = ea * none(most.reshape(B, -1).amax(-1)[:, None, None, None]) * none(vmost) * 2.0 ** -9
     fold = lambda t: t.reshape(B, Hk, G, Lk, D).sum(2).permute(0, 2, 1, 3)
     acc = lambda length: (length / 2 + 40) * F                    # the sums of the last products
     dq = scale * (ds @ K)
-    e_dq = scale * ((e_ds + acc(Lk) * ds.abs()) @ K.abs()) + uo * dq.abs() + tiny(dtype)
-    st, et = ds.transpose(-1, -2), e_ds.transpose(-1, -2)
+    e_dq = scale * ((e_ds + ea_q + acc(Lk) * ds.abs()) @ K.abs()) + uo * dq.abs() + tiny(dtype)
+    st, et = ds.transpose(-1, -2), (e_ds + ea_k).transpose(-1, -2)
     dk = fold(scale * (st @ Q))
     e_dk = fold(scale * ((et + acc(Lq * G) * st.abs()) @ Q.abs())) + uo * dk.abs() + tiny(dtype)
     pt = p.transpose(-1, -2)
     dv = fold(pt @ g)
-    e_dv = fold(((u + ep.transpose(-1, -2) + acc(Lq * G)) * pt + ea.transpose(-1, -2)) @ g.abs())
+    e_dv = fold(((u + ep.transpose(-1, -2) + acc(Lq * G)) * pt + ea_back.transpose(-1, -2)) @ g.abs())
     e_dv = e_dv + uo * dv.abs() + tiny(dtype)
     return res + [("dq", back(dq), back(e_dq)), ("dk", dk, e_dk), ("dv", dv, e_dv)]

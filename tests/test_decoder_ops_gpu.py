@@ -216,6 +216,30 @@ def test_cross_attention_padding(cuda, Lq, H, Hk, D, pad, dtype):
     assert not dk[dead].any() and not dv[dead].any()
 
 
+@pytest.mark.parametrize("Lq,Lk,H,Hk,D", [(65, 4096, 2, 2, 64), (200, 9, 4, 2, 40), (7, 20000, 4, 1, 128)])
+@pytest.mark.parametrize("size,qs,ks", [(2.0 ** -12, 2.0 ** -6, 2.0 ** 6), (2.0 ** -12, 2.0 ** 6, 2.0 ** -6),
+                                        (1.0, 1.0, 1.0), (2.0 ** 12, 2.0 ** -12, 2.0 ** -12)])
+def test_cross_attention_float16_backward_uses_its_range(cuda, Lq, Lk, H, Hk, D, size, qs, ks):
+    """Even rows of many keys with a small gradient -- P and dS below float16's smallest normal value
+    -- and rows of few keys with a large one, dS beyond its largest; q and k of sizes that bring dq or
+    dk back into the type's range."""
+    gen = _gen(Lk)
+    q = _leaf(_randn(gen, (2, Lq, H, D), torch.float16, qs))
+    k = _leaf(_randn(gen, (2, Lk, Hk, D), torch.float16, ks))
+    v = _leaf(_randn(gen, (2, Lk, Hk, D), torch.float16, 8.0))
+    dy = _randn(gen, (2, Lq, H, D), torch.float16, size)
+    scale = 0.3 / D ** 0.5
+    out = ops.cross_attention(q, k, v, scale=scale)
+    grads = torch.autograd.grad(out, [q, k, v], dy)
+    want = ref.cross_attention(q, k, v, None, None, scale, dy)
+    _all_close([out] + list(grads), want)
+    # as a whole: what three roundings (P or dS, D of a rounded out, the result) leave, and the
+    # result's own smallest steps
+    for got, (name, value, _) in zip(grads, want[1:]):
+        far = (got.double() - value).norm() / (value.norm() + value.numel() ** 0.5 * 2.0 ** -14)
+        assert torch.isfinite(got).all() and far <= 3 * ref.half_step(torch.float16), (name, float(far))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
 def test_cross_attention_lengths_out_of_range_are_clamped(cuda, dtype):
     gen = _gen(3)
