@@ -14,7 +14,8 @@ All three take CUDA (HIP) tensors of one type on one device, enqueue on that dev
 without synchronising, and raise RuntimeError for anything else.  Rows are read where they are when
 the last axis is contiguous, whatever the other strides; otherwise the tensor is copied first.
 Workspaces come from torch's allocator per call, so calls may be captured into HIP graphs and made
-from several streams.  First derivatives only.
+from several streams.  (As for any operator here: torch's engine cannot capture a backward pass while
+an eager graph of the same leaves is alive.)  First derivatives only.
 """
 import ctypes
 
@@ -30,7 +31,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # BTR_F32, B
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}                      # BTR_ACT_*
 _MAX_ROWS = 2 ** 30
 # (the checks below are written out, without helpers that format or build tuples on the way: a call
-# of a decoder's size is bound by the host, 20 -> 1x us forward)
+# of a decoder's size is bound by the host: 17.4 -> 11.6 us without gradients, 20.6 -> 17.5 with)
 
 
 def _refuse(message, *args):
@@ -221,7 +222,8 @@ class _Linear(Function):
 def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x weight^T + bias) + residual: x (..., k), weight (n, k), bias (n) or None, activation
     None / "relu" / "gelu" (the erf form), residual (..., n) or None.  Sums, activation and residual
-    in float32, rounded once."""
+    in float32, rounded once.  (float32 rows run as sums of three bfloat16 terms, exact to the 24th
+    bit: an infinite element makes the sums it enters NaN.)"""
     _check_ref("linear", x)
     _check_one("linear", "weight", weight, x)
     act = _ACTIVATIONS.get(activation)
@@ -304,11 +306,11 @@ class _CrossAttention(Function):
 def cross_attention(query, key, value, key_lengths=None, key_padding_mask=None, scale=None):
     """softmax(scale query key^T) value per head.
 
-    query (B, Lq, H, D), key and value (B, Lk, Hk, D), H a multiple of Hk, at most 128 times
-    it (query head i reads key head i // (H // Hk)), D <= 128; result (B, Lq, H, D).  Of batch entry b the keys from
-    key_lengths[b] (int32 (B), on the device) on and those where key_padding_mask (bool (B, Lk)) is
-    True take no part, whatever they hold; a query left without keys gets zeros, and gives none of
-    its gradient to anybody.  scale: D ** -0.5 by default, positive."""
+    query (B, Lq, H, D), key and value (B, Lk, Hk, D), H a multiple of Hk, at most 128 times it
+    (query head i reads key head i // (H // Hk)), D <= 128; result (B, Lq, H, D).  Of batch entry b
+    the keys from key_lengths[b] (int32 (B), on the device) on and those where key_padding_mask (bool
+    (B, Lk)) is True take no part, whatever they hold; a query left without keys gets zeros, and gives
+    none of its gradient to anybody.  scale: D ** -0.5 by default, positive."""
     _check_ref("cross_attention", query)
     _check_one("cross_attention", "key", key, query)
     _check_one("cross_attention", "value", value, query)

@@ -47,13 +47,17 @@ class TransformerDecoderLayer(nn.Module):
         self.cross_posembed = cross_posembed
 
     def _ops_covered(self, query, key, key_padding_mask):
-        """Does groupfree/decoder_ops.py run this call?  Padded keys and 16-bit layers; float32
-        without padding has the whole-layer call."""
-        return (query.is_cuda and query.dtype in (torch.float32, torch.bfloat16, torch.float16) and
-                (key_padding_mask is not None or query.dtype != torch.float32) and
-                key.dtype == query.dtype and self.activation in _ACTIVATIONS and
-                _mha_covered(self.self_attn, query.dtype) and
-                _mha_covered(self.multihead_attn, query.dtype))
+        """Does groupfree/decoder_ops.py run this call?  Padded keys and 16-bit layers, of one type
+        throughout and without autocast, which chooses types module by module; float32 without
+        padding has the whole-layer call."""
+        dtype = query.dtype
+        return (query.is_cuda and not torch.is_autocast_enabled() and dtype in
+                (torch.float32, torch.bfloat16, torch.float16) and
+                (key_padding_mask is not None or dtype != torch.float32) and
+                key.dtype == dtype and self.activation in _ACTIVATIONS and
+                all(m.weight.dtype == dtype for m in (self.linear1, self.linear2, self.norm1,
+                                                      self.norm2, self.norm3)) and
+                _mha_covered(self.self_attn, dtype) and _mha_covered(self.multihead_attn, dtype))
 
     def _forward_ops(self, query, key, q_pos, k_pos, key_padding_mask):
         """The layer on (B, P, C) rows: every projection one kernel with its bias (and activation),
