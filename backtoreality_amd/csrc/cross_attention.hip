@@ -66,18 +66,16 @@ struct XaArgs {
   float *part, *part2;                           // partial results of the shares
 };
 
-// ------------------------------------------------------------------------------- tiles in LDS
-// Row-major [row][DP]; PITCH bytes a row.  16-bit: 64 mod 128 bytes and the 16-byte units of a row
-// XOR-ed with (row / 4) % 4, so that both ways of reading -- sixteen rows at one column, and 4 x 16
-// blocks for the transpose read -- touch every bank once.  f32: one 16-byte unit of padding.
+// ------------------------------------------------------------------------------- f32 tiles in LDS
+// Row-major [row][DP]; PITCH bytes a row, one 16-byte unit of padding.  (The 16-bit tiles: lds_dma.hpp.)
 template <typename T, int DP>
 struct Tile {
+  static_assert(sizeof(T) == 4, "f32");
   static constexpr int V = Elem<T>::kVec;
-  static constexpr bool F32 = sizeof(T) == 4;
-  static constexpr int PITCH = F32 ? DP * 4 + 16 : (DP * 2) % 128 == 64 ? DP * 2 : DP * 2 + 64;
+  static constexpr int PITCH = DP * 4 + 16;
   static constexpr int UNITS = DP / V;           // 16-byte units of a row
   __device__ static __forceinline__ int unit_off(int row, int unit) {
-    return row * PITCH + (F32 ? unit : unit ^ ((row >> 2) & 3)) * 16;
+    return row * PITCH + unit * 16;
   }
 };
 
@@ -128,39 +126,12 @@ __device__ __forceinline__ void tile_t_times(const char *tile, int row0, int lan
   typedef Tile<T, DP> TL;
   const int l31 = lane & 31, hh = lane >> 5;
   const char *t = tile + row0 * TL::PITCH;
-  if constexpr (TL::F32) {
 #pragma unroll
-    for (int s = 0; s < 16; ++s) {
-      const float *row = reinterpret_cast<const float *>(t + acc_row(s, hh) * TL::PITCH);
+  for (int s = 0; s < 16; ++s) {
+    const float *row = reinterpret_cast<const float *>(t + acc_row(s, hh) * TL::PITCH);
 #pragma unroll
-      for (int nt = 0; nt < DP / 32; ++nt)
-        acc[nt] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * nt + l31], w[s], acc[nt], 0, 0, 0);
-    }
-  } else {
-    // lane p of a group of 16 addresses row p / 4, columns 4 (p % 4) .. + 3 of a [4][16] block and
-    // receives column p, rows 0 .. 3
-    const int p = lane & 15, half = (lane >> 4) & 1;
-    const int unit = 2 * half + ((p & 3) >> 1), sub = (p & 1) * 8;
-    const char *lo = t + (4 * hh + (p >> 2)) * TL::PITCH + (unit ^ hh) * 16 + sub;
-    const char *hi = t + (8 + 4 * hh + (p >> 2)) * TL::PITCH + (unit ^ (hh + 2)) * 16 + sub;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      typename Elem<T>::Vec bv;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) bv[j] = (T)w[8 * s + j];
-#pragma unroll
-      for (int nt = 0; nt < DP / 32; ++nt) {
-        union {
-          s16x4_t s4[2];
-          typename Elem<T>::Vec v;
-        } u;
-        u.s4[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4)(lo + 16 * s * TL::PITCH + 64 * nt));
-        u.s4[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4)(hi + 16 * s * TL::PITCH + 64 * nt));
-        acc[nt] = mma<T>(u.v, bv, acc[nt]);
-      }
-    }
+    for (int nt = 0; nt < DP / 32; ++nt)
+      acc[nt] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * nt + l31], w[s], acc[nt], 0, 0, 0);
   }
 }
 
@@ -384,6 +355,9 @@ __device__ __forceinline__ void merge_rows(const XaArgs &a, const Rows<T> &rows,
 // WR waves along the rows (32 each) x WK along the keys, KT key subtiles of 32 per wave and tile.
 //   WR 4, WK 1: many rows; the four waves share every K / V tile.
 //   WR 1, WK 4: few rows (single queries).
+// Bound by the f32 matrix instructions (64 columns wide for 33 .. 64) and, at a workgroup per CU, by
+// their latency: 4 x 8 heads of 36, 256 queries, 1 024 keys 34 us and 6 for the join, 16 at the matrix
+// pipe's rate.
 template <typename T, int DP, int WR, int WK, int KT>
 __global__ __launch_bounds__(256) void cross_attention_fwd_kernel(XaArgs a) {
   typedef Tile<T, DP> TL;
@@ -563,7 +537,8 @@ __global__ __launch_bounds__(256) void cross_attention_join_kernel(XaArgs a) {
 
 // -------------------------------------------------------------------------------- backward, dq
 // As the forward: per tile S^T = K Q^T, dP^T = V dO^T, dS^T in place, dq^T += K^T dS^T.  D = rowsum
-// (dO * O) comes first, from the same fragments, and is left for the dk / dv kernel.
+// (dO * O) comes first, from the same fragments, and is left for the dk / dv kernel.  (The sizes of
+// the forward: 44 us and 5 for the shares' sum; 24 at the matrix pipe's rate.)
 template <typename T, int DP, int WR, int WK, int KT>
 __global__ __launch_bounds__(256) void cross_attention_bwd_q_kernel(XaArgs a) {
   typedef Tile<T, DP> TL;
@@ -690,7 +665,7 @@ __global__ __launch_bounds__(256) void cross_attention_bwd_q_kernel(XaArgs a) {
 
 // ----------------------------------------------------------------------------- backward, dk, dv
 // Four waves x 32 keys; the rows pass by in tiles of 32.  S = Q K^T, dP = dO V^T with K and V rows
-// in registers, then dv^T += dO^T P and dk^T += Q^T dS.
+// in registers, then dv^T += dO^T P and dk^T += Q^T dS.  (The same sizes: 51 us and 8; 32.)
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void cross_attention_bwd_kv_kernel(XaArgs a) {
   typedef Tile<T, DP> TL;
@@ -784,16 +759,26 @@ __global__ __launch_bounds__(256) void cross_attention_bwd_kv_kernel(XaArgs a) {
 }
 
 // out[i] = sum over the shares, in order; blockIdx.y picks one of two tensors.  ROWS: the share is
-// laid out (batch, key head, row, d), the tensor (batch, query, head, d)
-template <typename T, bool ROWS>
+// laid out (batch, key head, row, d), the tensor (batch, query, head, d).  V elements at a time: 4
+// where d is a multiple of 4, else 1.
+template <typename T, bool ROWS, int V>
 __global__ __launch_bounds__(256) void cross_attention_sum_kernel(XaArgs a, long long n, T *out0,
                                                                   T *out1) {
+  typedef float F __attribute__((ext_vector_type(V), aligned(4)));
   const float *p = blockIdx.y ? a.part2 : a.part;
   T *out = blockIdx.y ? out1 : out0;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
-       i += (long long)gridDim.x * 256) {
-    float t = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) t += p[s * n + i];
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V; i < n;
+       i += (long long)gridDim.x * 256 * V) {
+    F t = 0.f;
+    int s = 0;
+    for (; s + 4 <= a.nsplit; s += 4) {            // (four loads in flight)
+      F x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const F *>(p + (s + u) * n + i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) t += x[u];
+    }
+    for (; s < a.nsplit; ++s) t += *reinterpret_cast<const F *>(p + s * n + i);
     long long dst = i;
     if (ROWS) {
       const long long row = i / a.d;
@@ -801,16 +786,30 @@ __global__ __launch_bounds__(256) void cross_attention_sum_kernel(XaArgs a, long
       const Rows<T> rows{a, bh / a.hk, bh % a.hk};
       dst = rows.o(r) + (i - row * a.d);
     }
-    out[dst] = (T)t;
+    typedef T O __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    O o;
+#pragma unroll
+    for (int u = 0; u < V; ++u) o[u] = (T)t[u];
+    *reinterpret_cast<O *>(out + dst) = o;
   }
+}
+template <typename T, bool ROWS>
+void launch_sum(const XaArgs &a, long long n, T *out0, T *out1, hipStream_t hs) {
+  const int v = a.d % 4 ? 1 : 4;
+  const dim3 grid((unsigned)std::min<long long>(4096, (n / v + 255) / 256), out1 ? 2 : 1);
+  if (v == 4)
+    hipLaunchKernelGGL((cross_attention_sum_kernel<T, ROWS, 4>), grid, dim3(256), 0, hs, a, n, out0, out1);
+  else
+    hipLaunchKernelGGL((cross_attention_sum_kernel<T, ROWS, 1>), grid, dim3(256), 0, hs, a, n, out0, out1);
 }
 
 // =========================================================== 16-bit, aligned: tiles by LDS DMA
-// Head widths of whole 16-byte units, rows on 16-byte boundaries: the tiles go from memory to LDS by
-// DMA (lds_dma.hpp; rows of 64 or 128 columns, of which the products take 32 NT), a tile ahead of their use, which frees the 32 staging
-// registers a lane (two waves per SIMD fit: 332 -> 218 registers at D = 128) and the LDS write
-// instructions.  Rows past the last key, masked keys and columns past d are loaded from beyond the
-// buffer's bound, which reads as zero.
+// Head widths of whole 16-byte units, rows on 16-byte boundaries (cross_attention_pack_kernel makes
+// them so): the tiles go from memory to LDS by DMA (lds_dma.hpp; rows of 64 or 128 columns, of which
+// the products take 32 NT), a tile ahead of their use, which frees the 32 staging registers a lane
+// (two waves per SIMD fit: 332 -> 218 registers at D = 128) and the LDS write instructions.  Rows past
+// the last key, masked keys and columns past d are loaded from beyond the buffer's bound, which reads
+// as zero.
 // rows x columns of a (row stride sl) matrix that a DMA may touch; anything else reads as zero
 struct DmaSrc {
   const char *base;
@@ -945,7 +944,12 @@ __device__ __forceinline__ void drop_dead(f32x16_t (&s)[KT], unsigned long long 
   }
 }
 
-// forward: WR waves x 32 rows share tiles of 64 keys, double-buffered, one barrier a tile
+// forward: WR waves x 32 rows share tiles of 64 keys, double-buffered, one barrier a tile.  Bound by
+// the matrix pipe and the VALU in turns: a wave's exponentials run beside another's products as far
+// as two or three waves a SIMD allow.  2 x 16 heads of 128 on 4 key heads, 4 096 queries, 16 384 keys,
+// bf16: 1.03 ms, 1.07 PFLOP/s of the 1.5 that a large product reaches; 4 x 16 heads of 64, 2 048
+// queries, 1 024 .. 4 096 keys: 125 - 140 us, 0.65 PFLOP/s (a score's VALU work is the same at half the
+// products).
 template <typename T, int NT, int WR>
 __global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
@@ -1009,8 +1013,9 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_fwd_dma_kernel(XaA
 }
 
 // few rows (32): every wave streams its own tiles of 32 keys -- wave w those of index w, w + 4, ..
-// -- through its own double buffer, without a barrier until the four merge.  Bound by HBM: 64 KB a
-// CU in flight.
+// -- through its own double buffer, without a barrier until the four merge.  Bound by HBM: 64 KB a CU
+// in flight.  (One query of 8 x 32 heads of 128 on 8 key heads, 8 192 .. 32 768 keys, bf16: 144 us,
+// 4.65 TB/s, and 5 us for joining the shares.)
 template <typename T, int NT>
 __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
@@ -1079,7 +1084,8 @@ __global__ __launch_bounds__(256) void cross_attention_fwd_stream_kernel(XaArgs 
   merge_rows<T, 32 * NT, 1, 4>(a, rows, bh, split, tile, 0, w, tid, m, l, o, (float *)smem, mx, sm);
 }
 
-// dq: WR waves x 32 rows share tiles of 64 keys as in the forward
+// dq: WR waves x 32 rows share tiles of 64 keys as in the forward (the ragged batch: 155 - 170 us, 0.8
+// PFLOP/s)
 template <typename T, int NT, int WR>
 __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
@@ -1199,7 +1205,8 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
 
 // dk, dv: WK waves x 32 keys, tiles of 64 rows.  A lane owns one key, its column of both results
 // depends on no other key: what a padded key's lane computes is dropped at the end, nothing is
-// selected on the way.  Rows past the end read as zeros (P = 1, but dout, dP - D and q are 0).
+// selected on the way.  Rows past the end read as zeros (P = 1, but dout, dP - D and q are 0).  (The
+// ragged batch: 210 - 235 us, 0.8 PFLOP/s.)
 template <typename T, int NT, int WK>
 __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_kv_dma_kernel(XaArgs a) {
   typedef typename Elem<T>::Vec Vec;
@@ -1675,10 +1682,7 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
     BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_q, q, hs));
     if (s.n > 1) {
       const long long n = (long long)a.b * a.hk * a.rows * a.d;
-      const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
-      BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_sum_kernel<T, true>),
-                                                      dim3(grid), dim3(256), 0, hs, q, n, (T *)dq,
-                                                      (T *)nullptr));
+      BTR_DISPATCH_DTYPE(p->dtype, launch_sum<T, true>(q, n, (T *)dq, (T *)nullptr, hs));
     }
   }
   if (a.lk > 0) {
@@ -1688,12 +1692,8 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
     k.tiles = s.tiles; k.nsplit = s.n; k.chunk = s.chunk; k.part = ws;
     k.part2 = (float *)((char *)ws + align256((size_t)s.n * n * 4));
     BTR_DISPATCH_DTYPE(p->dtype, BTR_XA_WIDTH(launch_bwd_kv, k, hs));
-    if (s.n > 1) {
-      const int grid = (int)std::min<long long>(4096, (n + 255) / 256);
-      BTR_DISPATCH_DTYPE(p->dtype, hipLaunchKernelGGL((cross_attention_sum_kernel<T, false>),
-                                                      dim3(grid, 2), dim3(256), 0, hs, k, n,
-                                                      (T *)dk, (T *)dv));
-    }
+    if (s.n > 1)
+      BTR_DISPATCH_DTYPE(p->dtype, launch_sum<T, false>(k, n, (T *)dk, (T *)dv, hs));
   }
   return check_launch("cross_attention_bwd");
 }

@@ -5,8 +5,8 @@
 // per lane, from the lanes' own addresses, so the rows of a tile cannot be padded apart.  Instead
 // unit u of row r lies at u ^ swz(r), chosen so that neither way of reading meets a bank twice in a
 // cycle (256 bytes): 16 rows at one unit fall on 16 different units of the 64 banks, and so do the
-// four rows x 64 bytes that 32 lanes of a transpose read touch.  An offset of kFar is beyond the descriptor's bound: that lane's unit
-// is filled with zeros.
+// four rows x 64 bytes that 32 lanes of a transpose read touch.  An offset of kFar is beyond the
+// descriptor's bound: that lane's unit is filled with zeros.
 #pragma once
 #include "decoder_ops.hpp"
 

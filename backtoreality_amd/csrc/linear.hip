@@ -470,6 +470,7 @@ __global__ __launch_bounds__(64 * GM * GN, OCC) void linear_dma_kernel(GemmArgs 
 // cut into 32 x 32 per wave (one product between two LDS round trips and a barrier) a step took 0.45
 // us, here a wave's step is eight products behind one round trip and four run at once.  (Rings of
 // four fit a CU once: 1 024 x 2 048 outputs, 128 / 1 024 steps 9.9 / 14.6 us against 6.9 / 12.1.)
+// 1 999 x 1 301 x 775 f16: 20.6 us, 195 TFLOP/s, 2.6 rounds of workgroups of 13 steps.
 template <typename T, bool TA, bool TB>
 __global__ __launch_bounds__(256) void linear_stream_kernel(GemmArgs g) {
   typedef typename Matrix<T>::E E;
@@ -591,7 +592,8 @@ __global__ __launch_bounds__(256) void linear_stream_kernel(GemmArgs g) {
 
 // Few rows of x (up to 16 MT): a workgroup's eight waves share 16 rows of W and split the reduction
 // (wave w: the steps of 32 numbered w, w + 8, ..), W goes from memory into the matrix instructions,
-// the eight sums meet in LDS.  Bound by the bytes of W: eight loads of 1 KB in flight a wave.
+// the eight sums meet in LDS.  Bound by the bytes of W: eight loads of 1 KB in flight a wave (1 row x
+// 4 096 x 4 096 bf16: 9.4 us; its bytes are 6.8 at a large copy's rate).
 template <typename T, int MT>
 __global__ __launch_bounds__(512) void linear_rows_kernel(GemmArgs g) {
   constexpr int P = Op<T>::P, U = sizeof(T) == 4 ? 4 : 8;
@@ -683,7 +685,8 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
   }
 }
 
-// adds the shares of the reduction in order, then the epilogue
+// adds the shares of the reduction in order, then the epilogue (bound by memory: four shares of 4 096
+// x 1 024 sums 13.5 us, 5.6 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void linear_join_kernel(GemmArgs g) {
   constexpr int V = Elem<T>::kVec;
@@ -709,7 +712,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(GemmArgs g) {
 
 // dz = dy slope (ReLU: dy where slope > 0) into rows of ldz elements, zeros behind them (f32: into
 // its three planes), and the column sums of dz over this workgroup's rows: 32 threads along the
-// columns (8 each), 8 rows at a time.  dz NULL: the sums only.
+// columns (8 each), 8 rows at a time.  dz NULL: the sums only.  (Bound by memory: 16 384 x 4 096 bf16
+// 74 us, 5.4 TB/s.  In the products' own staging it would be recomputed per tile, 4 to 64 times.)
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, const T *dy,
                                                         long long lddy, const typename Slope<T>::S *slope,
