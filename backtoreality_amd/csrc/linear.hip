@@ -12,8 +12,8 @@
 // has them and the second is read out of LDS with gfx950's transpose read, so nothing is ever
 // transposed in memory.  Operands go to LDS by DMA (linear_dma_kernel); 16-bit rows that do not lie
 // on 16-byte boundaries in whole 16-byte units are first copied to rows that do, in the workspace,
-// f32 ones are split into three bf16 planes there.  Few rows (single tokens) read W once, straight
-// into the matrix instructions (linear_rows_kernel).
+// f32 ones are split into three bf16 planes there.  Few rows (single tokens) or few outputs read the
+// long operand once, straight into the matrix instructions (linear_rows_kernel).
 //
 // Numbers: every product accumulates in f32 and the epilogue works on the f32 sums; y is rounded
 // once.  f32 operands are split into three bf16 terms (8 + 8 + 8 bits: exact up to the 24th) and
@@ -594,17 +594,22 @@ __global__ __launch_bounds__(256) void linear_stream_kernel(GemmArgs g) {
 // (wave w: the steps of 32 numbered w, w + 8, ..), W goes from memory into the matrix instructions,
 // the eight sums meet in LDS.  Bound by the bytes of W: eight loads of 1 KB in flight a wave (1 row x
 // 4 096 x 4 096 bf16: 9.4 us; its bytes are 6.8 at a large copy's rate).
-template <typename T, int MT>
+// COLS: the roles the other way round -- few outputs (up to 16 MT), 16 rows of x a workgroup, x read
+// once where it is.
+template <typename T, int MT, bool COLS>
 __global__ __launch_bounds__(512) void linear_rows_kernel(GemmArgs g) {
   constexpr int P = Op<T>::P, U = sizeof(T) == 4 ? 4 : 8;
   __shared__ float part[8][MT][16][20];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l15 = lane & 15, q = lane >> 4;
   const int n0 = blockIdx.x * 16;
   f32x4_t acc[MT] = {};
-  const T *wrow = (const T *)g.b + min(n0 + l15, g.n - 1) * g.ldb;
+  const int many = COLS ? g.m : g.n, few = COLS ? g.n : g.m;
+  const long long ldm = COLS ? g.lda : g.ldb, ldf = COLS ? g.ldb : g.lda;
+  const T *wrow = (const T *)(COLS ? g.a : g.b) + min(n0 + l15, many - 1) * ldm;
   const T *xrow[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) xrow[t] = (const T *)g.a + min(16 * t + l15, g.m - 1) * g.lda;
+  for (int t = 0; t < MT; ++t)
+    xrow[t] = (const T *)(COLS ? g.b : g.a) + min(16 * t + l15, few - 1) * ldf;
   // U steps of 32 at a time, their loads together
   for (int s0 = w * U * 32; s0 < g.k; s0 += 8 * U * 32) {
     typename Elem<T>::Vec wv[U][sizeof(T) / 2];
@@ -636,11 +641,26 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(GemmArgs g) {
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t)                     // [row of x][row of W]
+  for (int t = 0; t < MT; ++t)                     // [of the few][of the 16]
     *reinterpret_cast<f32x4_t *>(&part[w][t][l15][4 * q]) = acc[t];
   __syncthreads();
   // 16 outputs of a row in pieces of V columns
-  constexpr int V = Elem<T>::kVec, PR = 16 / V;
+  constexpr int V = Elem<T>::kVec;
+  if constexpr (COLS) {
+    constexpr int PC = MT * 16 / V;
+    for (int e = tid; e < 16 * PC; e += 512) {
+      const int row = e / PC, col = (e % PC) * V;
+      if (n0 + row >= g.m || col >= g.n) continue;
+      float s[V] = {};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int u = 0; u < V; ++u) s[u] += part[k][col >> 4][(col & 15) + u][row];
+      epilogue<T>(g, n0 + row, col, s, bias_at<T>(g, col), res_at<T>(g, n0 + row, col));
+    }
+    return;
+  }
+  constexpr int PR = 16 / V;
   for (int e = tid; e < MT * 16 * PR; e += 512) {
     const int row = e / PR, col = (e % PR) * V;
     if (row >= g.m || n0 + col >= g.n) continue;
@@ -824,7 +844,7 @@ size_t packed_bytes(int dtype, long long rows, int len) {
 size_t pack_bytes(int dtype, const void *p, long long ld, long long rows, int len) {
   return dma_rows(dtype, p, ld, len) ? 0 : packed_bytes(dtype, rows, len);
 }
-constexpr int kFewRows = 16;       // linear_rows_kernel up to here
+constexpr int kFewRows = 16;       // linear_rows_kernel up to here, whatever the rest
 // workgroups along the rows of the dz / dbias pass
 int dz_blocks(long long m, int n) {
   const long long cols = cdiv(n, 256);
@@ -902,8 +922,32 @@ int check(const char *what, const btr_linear_t *p) {
   return BTR_OK;
 }
 
+// Does linear_rows_kernel take a forward product with `few` rows (or outputs) against `many` outputs
+// (or rows)?  f32: up to 64, where the tiled kernels would first write three planes of the long operand
+// (rows x reduction x outputs, 32 x 4 096 x 4 096: 64 -> 31 us, 64 x 4 096 x 4 096: 68 -> 48, 30 000 x
+// 2 048 x 64: 274 -> 157; of what was timed only 30 000 x 128 x 64 loses, 28 -> 33).  16 bits: up to 32
+// while a round of workgroups covers the long side and the reduction is short (4 096 x 2 048 x 32 bf16:
+// 10.6 -> 9.5, 1 024 x 288 x 23 off 16-byte boundaries 9.2 -> 6.1; beyond: 30 000 x 128 x 23 8 -> 33,
+// 2 048 x 4 096 x 32 12 -> 15).
+bool few_of(int dtype, int few, int many, int k) {
+  return dtype == BTR_F32 ? few <= 64 : few <= 32 && many <= 4096 && k <= 2048;
+}
+bool few_rows(const btr_linear_t &p) { return p.m <= kFewRows || few_of(p.dtype, p.m, p.n, p.k); }
+bool few_columns(const btr_linear_t &p) { return few_of(p.dtype, p.n, p.m, p.k); }
+template <typename T, bool COLS>
+void launch_rows(const GemmArgs &g, int few, int many, hipStream_t hs) {
+  const dim3 grid(cdiv(many, 16));
+  if (few <= 16) {
+    hipLaunchKernelGGL((linear_rows_kernel<T, 1, COLS>), grid, dim3(512), 0, hs, g);
+  } else if (few <= 32) {
+    hipLaunchKernelGGL((linear_rows_kernel<T, 2, COLS>), grid, dim3(512), 0, hs, g);
+  } else {
+    if constexpr (sizeof(T) == 4)
+      hipLaunchKernelGGL((linear_rows_kernel<T, 4, COLS>), grid, dim3(512), 0, hs, g);
+  }
+}
 size_t fwd_bytes(const btr_linear_t &p) {
-  if (p.m <= kFewRows) return 0;
+  if (few_rows(p) || few_columns(p)) return 0;
   return pack_bytes(p.dtype, p.x, p.ldx, p.m, p.k) + pack_bytes(p.dtype, p.weight, p.ldw, p.n, p.k) +
          split_bytes(p.m, p.n, p.k, p.dtype);
 }
@@ -914,9 +958,12 @@ void forward(const btr_linear_t &p, void *y, void *slope, void *workspace, hipSt
   g.m = p.m; g.n = p.n; g.k = p.k;
   g.bias = p.bias; g.res = p.residual; g.ldres = p.ldr; g.act = p.act;
   g.c = y; g.slope = slope; g.nsplit = 1;
-  if (p.m <= kFewRows) {
+  if (few_rows(p) || few_columns(p)) {
     g.a = p.x; g.lda = p.ldx; g.b = p.weight; g.ldb = p.ldw;
-    hipLaunchKernelGGL((linear_rows_kernel<T, 1>), dim3(cdiv(p.n, 16)), dim3(512), 0, hs, g);
+    if (few_rows(p))
+      launch_rows<T, false>(g, p.m, p.n, hs);
+    else
+      launch_rows<T, true>(g, p.n, p.m, hs);
     return;
   }
   char *ws = (char *)workspace;

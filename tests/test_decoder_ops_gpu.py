@@ -80,7 +80,8 @@ def test_layer_norm_of_nothing(cuda):
 @pytest.mark.parametrize("m,k,n", [
     (1, 1, 1), (1, 288, 864), (3, 17, 5), (64, 64, 64), (65, 63, 129), (16, 1000, 40), (17, 2048, 288),
     (200, 36, 2048), (1024, 288, 288), (129, 775, 301), (48, 4096, 96), (2, 5000, 3), (700, 9, 700),
-    (2048, 512, 2304),
+    (2048, 512, 2304), (1000, 3375, 23), (333, 300, 16), (41, 1111, 64), (33, 600, 47), (64, 1030, 500),
+    (31, 2048, 129), (4097, 40, 32), (300, 2049, 31),
 ])
 @pytest.mark.parametrize("act,bias,residual", [(None, True, False), ("relu", True, True),
                                                ("relu", False, False), ("gelu", True, True)])
