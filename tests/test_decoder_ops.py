@@ -60,11 +60,11 @@ def test_linear_entry_refuses():
         assert lib.btr_linear_fwd_workspace_bytes(ctypes.addressof(desc(**bad))) == 0
     assert fwd(desc(), y=None) == -1
     assert lib.btr_linear_fwd(None, PTR, None, None, 0, None) == -1
-    long = desc(m=40, k=100000, ldx=100000, ldw=100000)       # shares of the reduction
+    long = desc(m=100, n=100, k=100000, ldx=100000, ldw=100000)       # shares of the reduction
     need = lib.btr_linear_fwd_workspace_bytes(ctypes.addressof(long))
     assert need > 0 and fwd(long, ws=PTR, nbytes=need - 1) == -1 and "workspace" in _error()
     assert fwd(long, ws=None, nbytes=need) == -1
-    odd = desc(dtype=1, k=15, ldx=15, ldw=15)                 # rows that are packed first
+    odd = desc(dtype=1, m=100, n=100, k=15, ldx=15, ldw=15)   # rows that are packed first
     assert lib.btr_linear_fwd_workspace_bytes(ctypes.addressof(odd)) > 0
     assert fwd(desc(m=0, x=None, weight=None), y=None) == 0
 
