@@ -29,8 +29,7 @@
 // per term).  float16 has five bits of exponent, too few for a backward pass as it stands -- a P of
 // 16 384 even keys and a dS of small dout are subnormal or nothing, a dS of large dout infinite -- so
 // there P is rounded as 2^15 P, and dS times a power of two: for dq each row's, from its largest
-// |dout|, for dk / dv each key's, from the largest |dout| of the rows and its own largest |v|.  All
-// are taken out of the f32 sums again.  f32 runs on the f32 matrix instructions, nothing is rounded
+// |dout|, for dk each key's, found on the way (fit_half).  All are taken out of the f32 sums again.  f32 runs on the f32 matrix instructions, nothing is rounded
 // below 32 bits.
 #include <algorithm>
 #include <cstdint>
@@ -59,7 +58,6 @@ struct XaArgs {
   float *lse;      // (b * hk, rows): log2 of the row's sum of exp2(scale_log2 * s); +inf: no key;
                    // float16: less kPExp
   float *delta;    // (b * hk, rows): D
-  float *dout_max; // (b * hk, ceil(rows / 32)): the largest |dout| of 32 rows (float16)
   void *dq, *dk, *dv;                            // contiguous, shaped like q, k, v
   float scale, scale_log2;
   int tiles, nsplit, chunk;                      // workgroup tiles, shares of the long axis, its length
@@ -244,16 +242,39 @@ __device__ __forceinline__ void store4(T *row, int c, int d, const float (&v)[4]
 }
 
 // The powers of two of float16's backward pass.  P rounds as 2^15 P <= 32 768.  With |dout| < 2^e and
-// |v| < 2^f, |dP| < d 2^(e + f) <= 2^(7 + e + f) and |dS| <= P (1 - P) 2 |dP| <= 2^(6 + e + f): dk / dv
-// know e and f, 2^(9 - e - f) dS stays below 65 504; dq knows its row's e only: 2^(5 - e) dS does up to
-// |v| = 32 in the worst case.
+// |v| < 2^f, |dP| < d 2^(e + f) <= 2^(7 + e + f) and |dS| <= P (1 - P) 2 |dP| <= 2^(6 + e + f): dq knows
+// its row's e only, 2^(5 - e) dS stays below 65 504 up to |v| = 32 in the worst case.  dk has no bound to
+// go by (dS holds the D of a row, which other keys' v make) and finds its power on the way, fit_half.
 template <typename T>
 constexpr bool kHalf = false;
 template <>
 constexpr bool kHalf<_Float16> = true;
-constexpr int kPExp = 15, kDqExp = 5, kDkExp = 9;
+constexpr int kPExp = 15, kDqExp = 5;
 __device__ __forceinline__ int exp_above(float x) {   // |x| < 2^exp_above(x); 0 for 0, inf, NaN
   return __builtin_amdgcn_frexp_expf(x);
+}
+// dS as float16 takes it: 2^up dS, up one number per lane pair (32 apart) that share the sums `acc`.  It
+// starts at kUpStart -- |dS| < 2^39, any of it fits float32 -- and goes down, for good, where a value
+// leaves float16's range, to the power that puts the largest into [2^14, 2^15); the sums follow.  So the
+// largest dS of a row or key decides, whatever the sizes of v and dout, and what it pushes below the
+// type's smallest steps is 2^-39 of it.  (A maximum per two scores; the rest is for the few tiles that
+// move it.)  Returns by how much.  `on`: a lane whose sums are dropped has no say.
+constexpr int kUpStart = 80;
+template <int N>
+__device__ __forceinline__ int fit_half(f32x16_t &ds, f32x16_t (&acc)[N], bool on) {
+  float top = 0.f;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) top = fmaxf(top, fabsf(ds[v]));
+  const bool over = on && top > 65504.f;
+  if (!__ballot(over)) return 0;
+  top = over ? top : 0.f;
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const int k = max(0, exp_above(top) - 15);     // (infinite: 0, nothing helps)
+  const float f = __builtin_ldexpf(1.f, -k);
+  ds *= f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) acc[n] *= f;
+  return k;
 }
 template <typename T>
 __device__ __forceinline__ float lse_of(float m, float l) {   // l > 0, or NaN
@@ -1128,11 +1149,6 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
     big = fmaxf(big, other_half(big));
     up = kDqExp - exp_above(big);
     lse += kPExp - up;
-    if (split == 0) {
-      for (int i = 1; i < 32; i <<= 1) big = fmaxf(big, __shfl_xor(big, i));
-      const int at = tile * WR + w, count = (a.rows + 31) / 32;
-      if (lane == 0 && at < count) a.dout_max[(long long)bh * count + at] = big;
-    }
   }
   f32x16_t dq[NT] = {};
   const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
@@ -1236,20 +1252,8 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
           (const T *)a.v + b * a.v_sb + kh * a.v_sh + key * a.v_sl + c);
     }
   }
-  int up = 0;                                    // float16: dS is rounded as 2^up dS, P as 2^kPExp P
-  if constexpr (kHalf<T>) {
-    float top = 0.f, big = 0.f;
-    const float *most = a.dout_max + (long long)bh * ((a.rows + 31) / 32);
-    for (int i = rbeg / 32 + lane; i < (rend + 31) / 32; i += 64) big = fmaxf(big, most[i]);
-    for (int i = 1; i < 64; i <<= 1) big = fmaxf(big, __shfl_xor(big, i));
-#pragma unroll
-    for (int j = 0; j < 2 * NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf((float)vf[j][i]));
-    top = fmaxf(top, other_half(top));
-    up = kDkExp - exp_above(big) - exp_above(top);
-  }
-  const float ds_up = __builtin_ldexpf(1.f, up - kPExp);
+  int up = kUpStart;                             // float16: dS is rounded as 2^up dS, P as 2^kPExp P
+  float ds_up = __builtin_ldexpf(1.f, up - kPExp);
   f32x16_t dk[NT] = {}, dv[NT] = {};
   const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
 
@@ -1309,6 +1313,10 @@ __global__ __launch_bounds__(64 * WK, NT <= 2 ? 2 : 1) void cross_attention_bwd_
           ds[0][v] = p[0][v] * (ds[0][v] - d4[i]);
           if (kHalf<T>) ds[0][v] *= ds_up;
         }
+      }
+      if constexpr (kHalf<T>) {
+        up -= fit_half(ds[0], dk, live);
+        ds_up = __builtin_ldexpf(1.f, up - kPExp);
       }
       dma_t<T, NT, 1>(gx, g2, tb, p, dv);
       DmaT<T, NT> qx;
@@ -1585,17 +1593,13 @@ size_t fwd_bytes(const XaArgs &a, int dtype) {
   const size_t n = s.n == 1 ? 0 : (size_t)s.n * a.b * a.hk * a.rows;
   return pack_bytes(a, dtype, false) + align256(n * a.d * 4) + align256(n * 8);
 }
-size_t stats_bytes(const XaArgs &a, int dtype) { // D; float16: the largest |dout|
-  const size_t bh = (size_t)a.b * a.hk;
-  return align256(bh * a.rows * 4) +
-         (dtype == BTR_F16 ? align256(bh * ((a.rows + 31) / 32) * 4) : 0);
-}
-size_t bwd_bytes(const XaArgs &a, int dtype) {   // these, what is packed, the shares of dq or of dk, dv
+size_t stats_bytes(const XaArgs &a) { return align256((size_t)a.b * a.hk * a.rows * 4); }   // D
+size_t bwd_bytes(const XaArgs &a, int dtype) {   // this, what is packed, the shares of dq or of dk, dv
   const Shares q = row_shares(a, dtype, false), k = key_shares(a);
   size_t nq = 0, nk = 0;
   if (q.n > 1) nq = align256((size_t)q.n * a.b * a.hk * a.rows * a.d * 4);
   if (k.n > 1) nk = 2 * align256((size_t)k.n * a.b * a.lk * a.hk * a.d * 4);
-  return stats_bytes(a, dtype) + pack_bytes(a, dtype, true) + std::max(nq, nk);
+  return stats_bytes(a) + pack_bytes(a, dtype, true) + std::max(nq, nk);
 }
 
 }  // namespace
@@ -1670,8 +1674,7 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
   a.lse = const_cast<float *>(lse);
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.delta = (float *)workspace;
-  a.dout_max = (float *)((char *)workspace + align256((size_t)a.b * a.hk * a.rows * 4));
-  char *at = (char *)workspace + stats_bytes(a, p->dtype);
+  char *at = (char *)workspace + stats_bytes(a);
   hipStream_t hs = as_stream(stream);
   BTR_DISPATCH_DTYPE(p->dtype, pack<T>(a, true, at, hs));
   float *ws = (float *)at;

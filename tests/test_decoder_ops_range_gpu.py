@@ -1,0 +1,56 @@
+"""groupfree/decoder_ops.py at the ends of its types' ranges, against float64: values of very different
+sizes in one call, tails, signs of zero, elements next to the type's largest (decoder_ops_common.py has
+the forms and their bounds)."""
+import pytest
+import torch
+
+import decoder_ops_common as ref
+from backtoreality_amd.groupfree import decoder_ops as ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(gen, shape, dtype, scale=1.0, shift=0.0):
+    return (torch.randn(shape, generator=gen, device="cuda") * scale + shift).to(dtype)
+
+
+def _leaf(t):
+    return None if t is None else t.detach().requires_grad_(True)
+
+
+def _attention_grads(q, k, v, dy, scale, lengths=None, mask=None):
+    leaves = [_leaf(q), _leaf(k), _leaf(v)]
+    out = ops.cross_attention(*leaves, key_lengths=lengths, key_padding_mask=mask, scale=scale)
+    return [out.detach()] + list(torch.autograd.grad(out, leaves, dy))
+
+
+# --------------------------------------------------------------------- float16 attention gradients
+@pytest.mark.parametrize("Lq,Lk,H,Hk,D", [(40, 16, 2, 1, 64), (3, 2, 1, 1, 64), (150, 300, 4, 2, 128),
+                                          (5, 5000, 2, 1, 40)])
+@pytest.mark.parametrize("pad", [False, True])
+def test_float16_key_gradients_with_values_of_different_sizes(cuda, Lq, Lk, H, Hk, D, pad):
+    """Keys whose values are 1, 2^-2 .. 2^-14 of the others' or nothing at all, dout along the result:
+    dS of a small value's key is as large as the others' (its D comes from them).  The bound of dk is
+    each term's rounding; a term that the type's smallest steps touch is 2^-39 of its key's largest
+    at most, far below that one's half step."""
+    gen = _gen(100 + Lk)
+    B = 2
+    q = _randn(gen, (B, Lq, H, D), torch.float16)
+    k = _randn(gen, (B, Lk, Hk, D), torch.float16, 0.2)
+    size = torch.pow(2.0, -2.0 * (torch.arange(Lk, device=cuda) % 9 - 1).clamp(min=0).float())
+    size[torch.arange(Lk, device=cuda) % 9 == 8] = 0.0
+    v = (_randn(gen, (B, Lk, Hk, D), torch.float32, 0.2, 1.0) * size[None, :, None, None]).half()
+    dy = _randn(gen, (B, Lq, H, D), torch.float16, 0.2, 1.0)
+    mask = None
+    if pad:                       # what is padded has values beyond all others, and takes no part
+        mask = torch.zeros((B, Lk), dtype=torch.bool, device=cuda)
+        mask[:, 1::7] = True
+        v = v.masked_fill(mask[:, :, None, None], 6e4)
+    got = _attention_grads(q, k, v, dy, D ** -0.5, mask=mask)
+    want = ref.cross_attention(q, k, v, None, mask, D ** -0.5, dy)
+    for t, (name, value, bound) in zip(got, want):
+        ref.close(name, t, value, bound)
