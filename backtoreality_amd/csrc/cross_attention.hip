@@ -28,8 +28,8 @@
 // rounded to the input type where they enter the matrix instructions (relative error half an ulp
 // per term).  float16 has five bits of exponent, too few for a backward pass as it stands -- a P of
 // 16 384 even keys and a dS of small dout are subnormal or nothing, a dS of large dout infinite -- so
-// there P is rounded as 2^15 P, and dS times a power of two: for dq each row's, from its largest
-// |dout|, for dk each key's, found on the way (fit_half).  All are taken out of the f32 sums again.  f32 runs on the f32 matrix instructions, nothing is rounded
+// there P is rounded as 2^15 P, and dS times a power of two, each row's for dq and each key's for dk,
+// found on the way (fit_half).  All are taken out of the f32 sums again.  f32 runs on the f32 matrix instructions, nothing is rounded
 // below 32 bits.
 #include <algorithm>
 #include <cstdint>
@@ -241,15 +241,12 @@ __device__ __forceinline__ void store4(T *row, int c, int d, const float (&v)[4]
   }
 }
 
-// The powers of two of float16's backward pass.  P rounds as 2^15 P <= 32 768.  With |dout| < 2^e and
-// |v| < 2^f, |dP| < d 2^(e + f) <= 2^(7 + e + f) and |dS| <= P (1 - P) 2 |dP| <= 2^(6 + e + f): dq knows
-// its row's e only, 2^(5 - e) dS stays below 65 504 up to |v| = 32 in the worst case.  dk has no bound to
-// go by (dS holds the D of a row, which other keys' v make) and finds its power on the way, fit_half.
+// float16's backward pass rounds P as 2^15 P <= 32 768 and dS as 2^up dS (fit_half).
 template <typename T>
 constexpr bool kHalf = false;
 template <>
 constexpr bool kHalf<_Float16> = true;
-constexpr int kPExp = 15, kDqExp = 5;
+constexpr int kPExp = 15;
 __device__ __forceinline__ int exp_above(float x) {   // |x| < 2^exp_above(x); 0 for 0, inf, NaN
   return __builtin_amdgcn_frexp_expf(x);
 }
@@ -1123,7 +1120,7 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
   const Rows<T> rows{a, b, kh};
   const int r = (tile * WR + w) * 32 + l31;
   Vec qf[2 * NT], gf[2 * NT];
-  float delta = 0.f, lse = INFINITY, big = 0.f;
+  float delta = 0.f, lse = INFINITY;
 #pragma unroll
   for (int j = 0; j < 2 * NT; ++j) {
     qf[j] = gf[j] = Vec{};
@@ -1133,10 +1130,7 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
       gf[j] = load_row((const T *)a.dout + rows.o(r), c, a.d);
       const Vec of = load_row((const T *)a.out + rows.o(r), c, a.d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        delta = fmaf((float)gf[j][i], (float)of[i], delta);
-        if (kHalf<T>) big = fmaxf(big, fabsf((float)gf[j][i]));
-      }
+      for (int i = 0; i < 8; ++i) delta = fmaf((float)gf[j][i], (float)of[i], delta);
     }
   }
   delta += other_half(delta);
@@ -1144,12 +1138,8 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
     lse = a.lse[(long long)bh * a.rows + r];
     if (split == 0 && hh == 0) a.delta[(long long)bh * a.rows + r] = delta;
   }
-  int up = 0;                                    // float16: dS is rounded as 2^up dS
-  if constexpr (kHalf<T>) {
-    big = fmaxf(big, other_half(big));
-    up = kDqExp - exp_above(big);
-    lse += kPExp - up;
-  }
+  int up = kUpStart;                             // float16: dS is rounded as 2^up dS
+  if (kHalf<T>) lse += kPExp - up;               // (P comes out as 2^up P)
   f32x16_t dq[NT] = {};
   const int rb = Dma<D>::row_base(l31, hh), tb = Dma<D>::tr_base(lane);
 
@@ -1194,6 +1184,11 @@ __global__ __launch_bounds__(64 * WR, 2) void cross_attention_bwd_q_dma_kernel(X
 #pragma unroll
         for (int v = 0; v < 16; ++v)
           s[0][v] = (bits >> (4 * hh)) & (1u << acc_row(v, 0)) ? s[0][v] : 0.f;
+      }
+      if constexpr (kHalf<T>) {
+        const int down = fit_half(s[0], dq, true);
+        up -= down;
+        lse += (float)down;
       }
       dma_t<T, NT, 1>(kx, kt2, tb, s, dq);
     }

@@ -54,3 +54,25 @@ def test_float16_key_gradients_with_values_of_different_sizes(cuda, Lq, Lk, H, H
     want = ref.cross_attention(q, k, v, None, mask, D ** -0.5, dy)
     for t, (name, value, bound) in zip(got, want):
         ref.close(name, t, value, bound)
+
+
+@pytest.mark.parametrize("Lq,Lk,H,Hk,D", [(40, 24, 2, 1, 64), (2, 2, 1, 1, 8), (200, 130, 4, 2, 128),
+                                          (7, 5000, 2, 1, 40)])
+@pytest.mark.parametrize("size,even", [(256.0, True), (2e3, True), (1e2, False), (1e4, False)])
+def test_float16_gradients_with_large_values(cuda, Lq, Lk, H, Hk, D, size, even):
+    """|v| of 10^2 to 10^4, a gradient that makes dq and dk fit: even -- a key's value is +-size in
+    every column, dout the same, so that no term of dP cancels -- or random."""
+    gen = _gen(200 + Lk)
+    B = 2
+    q = _randn(gen, (B, Lq, H, D), torch.float16, 2.0 ** -5)
+    k = _randn(gen, (B, Lk, Hk, D), torch.float16, 2.0 ** -5)
+    if even:
+        sign = (torch.rand((B, Lk, Hk, 1), generator=gen, device=cuda) < 0.5).float() * 2 - 1
+        v = (sign * size).expand(B, Lk, Hk, D).half().contiguous()
+        dy = torch.full((B, Lq, H, D), 0.01, device=cuda, dtype=torch.float16)
+    else:
+        v, dy = _randn(gen, (B, Lk, Hk, D), torch.float16, size), _randn(gen, (B, Lq, H, D), torch.float16, 0.01)
+    want = ref.cross_attention(q, k, v, None, None, D ** -0.5, dy)
+    assert all(float(value.abs().max()) < 3e4 for _, value, _ in want[1:])
+    for t, (name, value, bound) in zip(_attention_grads(q, k, v, dy, D ** -0.5), want):
+        ref.close(name, t, value, bound)
