@@ -12,7 +12,7 @@ parameters (same state-dict keys: in_proj_weight / in_proj_bias / out_proj.*):
 
 and its backward through btr_attention_bwd (dq / dk / dv written straight into the packed
 gradient of the projection output).  Returns None when the configuration is not covered
-(CPU tensors, masks, bias_k / add_zero_attn, separate q/k/v widths): the caller then runs the
+(CPU tensors, other types or autocast, masks, bias_k / add_zero_attn, separate q/k/v widths): the caller then runs the
 stock module.  `BTR_FUSED_ATTENTION=0` disables it.
 
 Dropout masks come from a counter-based hash of (a host seed unique per call, a device step
@@ -60,6 +60,8 @@ class _AttentionCore(Function):
     @staticmethod
     def forward(ctx, q_src, kv_src, nhead, dropout_p, seed):
         self_attn = kv_src is None
+        if q_src.dtype != torch.float32 or not (self_attn or kv_src.dtype == torch.float32):
+            raise RuntimeError("attention: projections should be float32")
         Lq, B, Wq = q_src.shape
         E = Wq // 3 if self_attn else Wq
         d = E // nhead
@@ -111,8 +113,12 @@ class _AttentionCore(Function):
 
 
 def _covered(mha, query, key):
+    # float32 throughout: the kernels read the projections' results as float32, and those are 16-bit
+    # (half the bytes) under autocast or with 16-bit weights
     return (enabled() and query.is_cuda and query.dtype == torch.float32 and query.dim() == 3 and
-            key.dim() == 3 and mha._qkv_same_embed_dim and mha.in_proj_bias is not None and
+            key.dtype == torch.float32 and key.dim() == 3 and not torch.is_autocast_enabled() and
+            mha._qkv_same_embed_dim and mha.in_proj_weight.dtype == torch.float32 and
+            mha.out_proj.weight.dtype == torch.float32 and mha.in_proj_bias is not None and
             mha.bias_k is None and mha.bias_v is None and not mha.add_zero_attn and
             not getattr(mha, "batch_first", False) and
             _lib.btr_attention_supported(mha.head_dim) and query.shape[2] == mha.embed_dim and

@@ -76,6 +76,8 @@ def covered(layer, query, key, q_pos, k_pos):
     if layer.linear1.bias is None or layer.linear2.bias is None or \
             layer.linear1.out_features % 4:
         return False
+    if any(t.dtype != torch.float32 for t in _params(layer)):   # (the kernels read them as float32)
+        return False
     for pos, P in ((q_pos, Pq), (k_pos, key.shape[2])):
         if pos is not None and (tuple(pos.shape) != (B, E, P) or pos.dtype != torch.float32):
             return False

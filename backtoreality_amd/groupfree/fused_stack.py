@@ -309,6 +309,9 @@ def _set_pointers(ent, det, specs, params, cat_at):
                                  bn.momentum]
     if ptrs == ent.ptrs:
         return
+    # (a detector converted after its checks were kept: other pointers, so it is seen here)
+    if any(t is not None and t.dtype != torch.float32 for t in params):
+        raise RuntimeError("decoder stack: parameters should be float32")
     d = ent.d
     at = 0
     for i in range(det.num_decoder_layers):
