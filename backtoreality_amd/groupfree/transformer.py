@@ -25,6 +25,26 @@ def _mha_covered(mha, dtype):
             (mha.dropout == 0 or not mha.training) and mha.in_proj_weight.dtype == dtype)
 
 
+def _stock_attention(mha, query, key, key_padding_mask=None):
+    """mha(query, key, value=key)[0].  Attention that torch would do in bfloat16 on the GPU -- the
+    layer's type, or autocast's -- is done in float32 and rounded once: torch multiplies its batches of
+    matrices by transposed views, and such a product of bfloat16 has faulted this GPU in the library's
+    kernel.  The module is called as it is (its own forward, hooks), on float32 copies of its
+    parameters."""
+    bf16 = torch.bfloat16
+    in_bf16 = query.is_cuda and (torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda")
+                                 else query.dtype) == bf16
+    if not in_bf16:
+        return mha(query, key, value=key, key_padding_mask=key_padding_mask)[0]
+    q = query.float()
+    k = q if key is query else key.float()
+    params = {name: p.float() for name, p in mha.named_parameters()}
+    with torch.autocast("cuda", enabled=False):
+        out = torch.func.functional_call(mha, params, (q, k), {
+            "value": k, "key_padding_mask": key_padding_mask})[0]
+    return out.to(bf16)
+
+
 class TransformerDecoderLayer(nn.Module):
     def __init__(self, d_model, nhead, dim_feedforward=2048, dropout=0.1, activation="relu",
                  self_posembed=None, cross_posembed=None):
@@ -116,7 +136,7 @@ class TransformerDecoderLayer(nn.Module):
         qp = query if q_pos is None else query + q_pos
         att = fused_attention.mha_forward(self.self_attn, qp, qp)
         if att is None:
-            att = self.self_attn(qp, qp, value=qp)[0]
+            att = _stock_attention(self.self_attn, qp, qp)
         query = self.norm1(query + self.dropout1(att))
 
         qp = query if q_pos is None else query + q_pos
@@ -125,8 +145,7 @@ class TransformerDecoderLayer(nn.Module):
         if key_padding_mask is None:
             att = fused_attention.mha_forward(self.multihead_attn, qp, kp)
         if att is None:
-            att = self.multihead_attn(query=qp, key=kp, value=kp,
-                                      key_padding_mask=key_padding_mask)[0]
+            att = _stock_attention(self.multihead_attn, qp, kp, key_padding_mask)
         query = self.norm2(query + self.dropout2(att))
 
         ffn = self.linear2(self.dropout(self.activation(self.linear1(query))))

@@ -64,3 +64,64 @@ def test_decoder_stack_refuses_a_converted_detector():
     det, ent = types.SimpleNamespace(num_decoder_layers=0), types.SimpleNamespace(ptrs=None, d=None)
     with pytest.raises(RuntimeError, match="float32"):
         fused_stack._set_pointers(ent, det, [], params, [])
+
+
+# ------------------------------------------------------- torch's attention in bfloat16 on the GPU
+class NoBfloat16Batches(torch.utils._python_dispatch.TorchDispatchMode):
+    """Batched products of bfloat16, by any name, are an error; counts the others."""
+
+    def __init__(self):
+        super().__init__()
+        self.batches = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if any(n in func.name() for n in ("bmm", "attention")):
+            self.batches += 1
+            assert not any(isinstance(a, torch.Tensor) and a.dtype == torch.bfloat16 for a in args), func
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("how", ["layer", "autocast"])
+def test_bfloat16_attention_of_the_modules_runs_in_float32(how, masked, autocast, monkeypatch):
+    """Dropout on the attention weights, autocast: the module's attention, forward and backward, without
+    a batched product of bfloat16."""
+    torch.manual_seed(0)
+    layer = TransformerDecoderLayer(32, 4, 64, 0.1).train()
+    dtype = torch.float32
+    if how == "layer":
+        layer, dtype = layer.bfloat16(), torch.bfloat16
+    query, key = (_on_gpu(2, 32, n, dtype=dtype).requires_grad_(True) for n in (5, 9))
+    mask = torch.zeros((2, 9), dtype=torch.bool)
+    mask[:, 6:] = True
+    autocast(how == "autocast")
+    monkeypatch.setenv("BTR_FUSED_DECODER", "0")     # (the whole-layer call takes float32 as it is)
+    with NoBfloat16Batches() as seen:
+        out = layer(query, key, None, None, key_padding_mask=mask if masked else None)
+        assert out.dtype == dtype
+        out.sum().backward()
+    assert seen.batches >= 8
+    assert all(p.grad is not None and p.grad.dtype == p.dtype for p in layer.parameters())
+    assert query.grad is not None and key.grad is not None
+
+
+def test_bfloat16_attention_keeps_the_module_and_its_result():
+    """The module's own forward and hooks; the float32 result rounded once."""
+    torch.manual_seed(1)
+    from backtoreality_amd.groupfree.transformer import _stock_attention
+    mha = torch.nn.MultiheadAttention(32, 4).bfloat16()
+    seen = []
+    mha.register_forward_hook(lambda m, args, out: seen.append(args[0].dtype))
+    q, k = _on_gpu(5, 2, 32, dtype=torch.bfloat16), _on_gpu(7, 2, 32, dtype=torch.bfloat16)
+    mask = torch.zeros((2, 7), dtype=torch.bool)
+    mask[1, 3:] = True
+    got = _stock_attention(mha, q, k, mask)
+    assert seen == [torch.float32] and got.dtype == torch.bfloat16
+    assert all(p.dtype == torch.bfloat16 for p in mha.parameters())
+    wide = torch.nn.MultiheadAttention(32, 4).double()
+    wide.load_state_dict(mha.state_dict())
+    q64, k64 = (t.as_subclass(torch.Tensor).double() for t in (q, k))
+    want = wide(q64, k64, k64, key_padding_mask=mask)[0]
+    # float32 sums of some 32 terms, then half a step of bfloat16
+    off = (got.as_subclass(torch.Tensor).double() - want).abs()
+    assert bool((off <= 2.0 ** -8 * want.abs() + 2.0 ** -18).all())
