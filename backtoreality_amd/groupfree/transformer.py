@@ -10,19 +10,36 @@ what `BTR_FUSED_DECODER=0` selects.  Layers in bfloat16 / float16 and keys with 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import decoder_ops, fused_attention, fused_decoder
 
 _ACTIVATIONS = {F.relu: "relu", F.gelu: "gelu"}
 
 
+def _own_call(m, kind, dtype):
+    """Is calling `m` what its class does with its parameters, and nothing else?  Exactly a `kind` (a
+    subclass, a wrapper or a parametrised module has a forward of its own) without hooks (weight_norm
+    and pruning make their weight in one), its parameters plain tensors of the layer's type."""
+    return (type(m) is kind and "forward" not in m.__dict__ and
+            not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or
+                 m._backward_pre_hooks) and
+            all(p is None or (p.dtype == dtype and type(p) is nn.Parameter)
+                for p in m._parameters.values()))
+
+
 def _mha_covered(mha, dtype):
-    """Packed projections of one width in the layer's type, nothing appended to the keys, and no
-    dropout on the attention weights in this call."""
-    return (isinstance(mha, nn.MultiheadAttention) and mha._qkv_same_embed_dim and
+    """Packed projections of one width, nothing appended to the keys, and no dropout on the attention
+    weights in this call.  (The output projection is read, never called, by the stock module too.)"""
+    return (_own_call(mha, nn.MultiheadAttention, dtype) and mha._qkv_same_embed_dim and
             mha.bias_k is None and mha.bias_v is None and not mha.add_zero_attn and
             not getattr(mha, "batch_first", False) and mha.head_dim <= 128 and
-            (mha.dropout == 0 or not mha.training) and mha.in_proj_weight.dtype == dtype)
+            (mha.dropout == 0 or not mha.training) and mha.out_proj.weight.dtype == dtype and
+            (mha.out_proj.bias is None or mha.out_proj.bias.dtype == dtype))
+
+
+def _norm_covered(n, width, dtype):
+    return _own_call(n, nn.LayerNorm, dtype) and tuple(n.normalized_shape) == (width,)
 
 
 def _stock_attention(mha, query, key, key_padding_mask=None):
@@ -68,15 +85,18 @@ class TransformerDecoderLayer(nn.Module):
 
     def _ops_covered(self, query, key, key_padding_mask):
         """Does groupfree/decoder_ops.py run this call?  Padded keys and 16-bit layers, of one type
-        throughout and without autocast, which chooses types module by module; float32 without
-        padding has the whole-layer call."""
+        throughout and without autocast, which chooses types module by module, and only modules that
+        are what they look like (_own_call); float32 without padding has the whole-layer call."""
         dtype = query.dtype
-        return (query.is_cuda and not torch.is_autocast_enabled() and dtype in
-                (torch.float32, torch.bfloat16, torch.float16) and
-                (key_padding_mask is not None or dtype != torch.float32) and
-                key.dtype == dtype and self.activation in _ACTIVATIONS and
-                all(m.weight.dtype == dtype for m in (self.linear1, self.linear2, self.norm1,
-                                                      self.norm2, self.norm3)) and
+        if not (query.is_cuda and dtype in (torch.float32, torch.bfloat16, torch.float16) and
+                (key_padding_mask is not None or dtype != torch.float32) and key.dtype == dtype and
+                self.activation in _ACTIVATIONS and not torch.is_autocast_enabled("cuda") and
+                not _has_any_global_hook()):
+            return False
+        width = query.shape[1]
+        return (all(_norm_covered(n, width, dtype) for n in (self.norm1, self.norm2, self.norm3)) and
+                _own_call(self.linear1, nn.Linear, dtype) and
+                _own_call(self.linear2, nn.Linear, dtype) and
                 _mha_covered(self.self_attn, dtype) and _mha_covered(self.multihead_attn, dtype))
 
     def _forward_ops(self, query, key, q_pos, k_pos, key_padding_mask):

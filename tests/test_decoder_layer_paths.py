@@ -125,3 +125,73 @@ def test_bfloat16_attention_keeps_the_module_and_its_result():
     # float32 sums of some 32 terms, then half a step of bfloat16
     off = (got.as_subclass(torch.Tensor).double() - want).abs()
     assert bool((off <= 2.0 ** -8 * want.abs() + 2.0 ** -18).all())
+
+
+# ----------------------------------------------- the operators replace nothing but the stock modules
+def _covered(layer, dtype=torch.bfloat16, mask=True):
+    mask = torch.zeros((2, 9), dtype=torch.bool) if mask else None
+    return layer._ops_covered(_on_gpu(2, 32, 5, dtype=dtype), _on_gpu(2, 32, 9, dtype=dtype), mask)
+
+
+def _plain_layer(dtype=torch.bfloat16):
+    return TransformerDecoderLayer(32, 4, 64, 0.0).to(dtype)
+
+
+class AddingLinear(torch.nn.Linear):
+    def forward(self, x):
+        return super().forward(x) + 100
+
+
+def test_operators_take_the_stock_modules():
+    for dtype in (torch.bfloat16, torch.float16):
+        assert _covered(_plain_layer(dtype), dtype) and _covered(_plain_layer(dtype), dtype, mask=False)
+    assert _covered(_plain_layer(torch.float32), torch.float32)
+    assert not _covered(_plain_layer(torch.float32), torch.float32, mask=False)
+    layer = _plain_layer()
+    layer.norm2 = torch.nn.LayerNorm(32, elementwise_affine=False)
+    layer.linear1 = torch.nn.Linear(32, 64, bias=False).bfloat16()
+    assert _covered(layer)
+
+
+def _hooked(register):
+    return lambda m: getattr(m, register)(lambda *a: None)
+
+
+@pytest.mark.parametrize("change", [
+    _hooked("register_forward_hook"), _hooked("register_forward_pre_hook"),
+    _hooked("register_full_backward_hook"), _hooked("register_full_backward_pre_hook"),
+    lambda m: setattr(m, "forward", lambda *a, **k: None),
+], ids=["hook", "pre", "backward", "backward_pre", "forward"])
+@pytest.mark.parametrize("name", ["linear1", "linear2", "norm1", "norm2", "norm3", "self_attn",
+                                  "multihead_attn"])
+def test_operators_leave_changed_modules_alone(name, change):
+    layer = _plain_layer()
+    change(getattr(layer, name))
+    assert not _covered(layer) and not _covered(layer, mask=False)
+
+
+@pytest.mark.parametrize("name,make", [
+    ("linear1", lambda: AddingLinear(32, 64)),
+    ("linear2", lambda: torch.nn.Sequential(torch.nn.Linear(64, 32))),
+    ("linear1", lambda: torch.nn.utils.parametrizations.weight_norm(torch.nn.Linear(32, 64))),
+    ("linear2", lambda: torch.nn.utils.prune.l1_unstructured(torch.nn.Linear(64, 32), "weight", 0.5)),
+    ("linear1", lambda: torch.nn.utils.spectral_norm(torch.nn.Linear(32, 64))),
+    ("norm1", torch.nn.Identity), ("norm3", lambda: torch.nn.RMSNorm(32)),
+    ("norm2", lambda: torch.nn.LayerNorm((5, 32))),
+    ("self_attn", lambda: type("Own", (torch.nn.MultiheadAttention,), {})(32, 4)),
+])
+def test_operators_leave_other_modules_alone(name, make):
+    import torch.nn.utils.prune  # noqa: F401
+    layer = _plain_layer()
+    setattr(layer, name, make().bfloat16())
+    assert not _covered(layer) and not _covered(layer, mask=False)
+
+
+def test_operators_stay_out_of_global_hooks():
+    layer = _plain_layer()
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+    try:
+        assert not _covered(layer)
+    finally:
+        handle.remove()
+    assert _covered(layer)
