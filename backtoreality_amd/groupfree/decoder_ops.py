@@ -15,12 +15,13 @@ without synchronising, and raise RuntimeError for anything else.  Rows are read 
 the last axis is contiguous, whatever the other strides; otherwise the tensor is copied first.
 Workspaces come from torch's allocator per call, so calls may be captured into HIP graphs and made
 from several streams.  (As for any operator here: torch's engine cannot capture a backward pass while
-an eager graph of the same leaves is alive.)  First derivatives only.
+an eager graph of the same leaves is alive.)  First derivatives in backward mode only: a second
+derivative, a forward-mode one and torch.func's transforms are refused.
 """
 import ctypes
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from ..pointnet2 import _ext
@@ -58,6 +59,16 @@ def _check_ref(name, t):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _ext._stream
 
 
+_tracing = torch._C._get_tracing_state
+
+
+def transformed():
+    """Is this call differentiated in forward mode, transformed (torch.func), traced or compiled?  The
+    operators refuse most of that; a caller that has elementary torch operations to offer takes those."""
+    return (forward_ad._current_level >= 0 or _tracing() is not None or
+            torch._C._functorch.peek_interpreter_stack() is not None or torch.compiler.is_compiling())
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -93,6 +104,12 @@ def _workspace(nbytes, device):
 
 
 def _wants_grad(*tensors):
+    # Without gradients the autograd node around the call is left out -- but not where the node is what
+    # refuses a forward-mode derivative (a dual tensor need not require a gradient; without the node its
+    # tangent would be lost without a word), or what torch.jit.trace records (it does not see the kernel
+    # write the result).
+    if forward_ad._current_level >= 0 or _tracing() is not None:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

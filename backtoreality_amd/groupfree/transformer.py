@@ -86,11 +86,14 @@ class TransformerDecoderLayer(nn.Module):
     def _ops_covered(self, query, key, key_padding_mask):
         """Does groupfree/decoder_ops.py run this call?  Padded keys and 16-bit layers, of one type
         throughout and without autocast, which chooses types module by module, and only modules that
-        are what they look like (_own_call); float32 without padding has the whole-layer call."""
+        are what they look like (_own_call), called as they are (not in forward mode, torch.func or a
+        trace); float32 without padding has the whole-layer call, and BTR_FUSED_DECODER=0 has the
+        modules (second derivatives need them)."""
         dtype = query.dtype
         if not (query.is_cuda and dtype in (torch.float32, torch.bfloat16, torch.float16) and
                 (key_padding_mask is not None or dtype != torch.float32) and key.dtype == dtype and
                 self.activation in _ACTIVATIONS and not torch.is_autocast_enabled("cuda") and
+                fused_decoder.enabled() and not decoder_ops.transformed() and
                 not _has_any_global_hook()):
             return False
         width = query.shape[1]

@@ -195,3 +195,62 @@ def test_operators_stay_out_of_global_hooks():
     finally:
         handle.remove()
     assert _covered(layer)
+
+
+# ------------------------------------------------------------------ what the operators cannot derive
+def test_operators_stay_out_of_transformed_calls(monkeypatch):
+    """Forward mode, torch.func, tracing: the modules, whose operations torch knows; and by the switch."""
+    import torch.autograd.forward_ad as forward_ad
+    layer = _plain_layer()
+    assert _covered(layer)
+    with forward_ad.dual_level():
+        assert not _covered(layer)
+    seen = []
+
+    def look(x):
+        seen.append(_covered(layer))
+        return x * 2
+    torch.func.vmap(look, randomness="same")(torch.ones(3))
+    torch.jit.trace(look, torch.ones(3), check_trace=False)
+    assert seen == [False, False] and _covered(layer)
+    monkeypatch.setenv("BTR_FUSED_DECODER", "0")
+    assert not _covered(layer)
+
+
+@pytest.fixture
+def calls_on_the_cpu(monkeypatch):
+    """The operators with their kernels left out: results of zeros."""
+    from backtoreality_amd.groupfree import decoder_ops
+    real = torch.empty
+    monkeypatch.setattr(decoder_ops, "_launch", lambda *a: None)
+    monkeypatch.setattr(decoder_ops, "_check_ref", lambda *a: None)
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: real(*a, **kw).zero_())
+    return {"layer_norm": lambda x: decoder_ops.layer_norm(x),
+            "linear": lambda x: decoder_ops.linear(x, torch.ones(3, 8)),
+            "cross_attention": lambda x: decoder_ops.cross_attention(*[x.view(1, 4, 1, 8)] * 3)}
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "linear", "cross_attention"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(calls_on_the_cpu, name, grad):
+    """A dual tensor without requires_grad: an error, not a result without its tangent."""
+    import torch.autograd.forward_ad as forward_ad
+    fn, x = calls_on_the_cpu[name], torch.randn(4, 8)
+    with torch.set_grad_enabled(grad):
+        assert not fn(x).requires_grad
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="jvp"):
+                fn(forward_ad.make_dual(x, torch.ones_like(x)))
+            assert not fn(x).any()               # no dual among its inputs: an ordinary call
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(fn, (x,), (x,))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "linear", "cross_attention"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_a_trace_records_the_call(calls_on_the_cpu, name, grad):
+    """... and not the allocation of its result as the result."""
+    with torch.set_grad_enabled(grad):
+        graph = torch.jit.trace(calls_on_the_cpu[name], torch.randn(4, 8), check_trace=False).graph
+    kinds = [n.kind() for n in graph.nodes()]
+    assert "prim::PythonOp" in kinds and "aten::empty" not in kinds, kinds

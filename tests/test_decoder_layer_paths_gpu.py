@@ -72,3 +72,16 @@ def test_bfloat16_layer_trains_with_dropout(cuda, masked):
     out = layer(q, k, None, None, key_padding_mask=mask)
     grads = torch.autograd.grad(out, [q, k] + list(layer.parameters()), dy)
     _near_float64(layer.eval(), q, k, mask, out, grads, dy, 2.0 ** -8)
+
+
+def test_a_trace_of_the_operators_runs(cuda):
+    """torch.jit.trace without gradients: the traced function computes, on other inputs too."""
+    from backtoreality_amd.groupfree import decoder_ops
+    w, b = torch.randn(24, 16, device=cuda), torch.randn(24, device=cuda)
+    x = torch.randn(5, 16, device=cuda)
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda t: decoder_ops.layer_norm(decoder_ops.linear(t, w, b, "relu")), x,
+                                 check_trace=False)
+        for _ in range(2):
+            assert torch.equal(traced(x), decoder_ops.layer_norm(decoder_ops.linear(x, w, b, "relu")))
+            x = torch.randn(5, 16, device=cuda)
