@@ -159,30 +159,34 @@ __device__ __forceinline__ float gelu(float z, float &slope) {
   slope = (bits >= 0 ? 1.f : 0.f) + __int_as_float(__float_as_int(u) ^ (bits & (int)0x80000000));
   return fmaf(-az, h, fmaxf(z, 0.f));
 }
-// act(z), and act'(z) into slope
-template <bool F32>
+// act(z), and act'(z) into slope.  ReLU: the result itself, in T -- a z that T rounds to zero is off, and
+// NaN is on, as where the rounded result is all that is kept.
+template <typename T>
 __device__ __forceinline__ float activate(float z, int act, float &slope) {
-  slope = 1.f;
+  if (act == kActGelu) return gelu<sizeof(T) == 4>(z, slope);
   if (act == kActRelu) {
-    slope = z > 0.f ? 1.f : 0.f;
-    return z > 0.f ? z : z != z ? z : 0.f;
+    const float a = z > 0.f ? z : z != z ? z : 0.f;
+    slope = (float)(T)a;
+    return a;
   }
-  if (act == kActGelu) return gelu<F32>(z, slope);
+  slope = 1.f;
   return z;
 }
 
 // The slope as the backward gets it: f32 itself, or 16 bits -- GELU's in fixed point (at most 1.13:
 // below 60 600; all ones stand for NaN; what pads a row reads as 0 and must give 0), ReLU's 1 or 0.
+// For ReLU the result may stand in its place: on where it is positive or NaN.
 template <typename T>
 struct Slope {
   typedef unsigned short S;
   __device__ static __forceinline__ S keep(float d, int act) {
-    if (act == kActRelu) return d > 0.f ? 1 : 0;
+    if (act == kActRelu) return d > 0.f || d != d ? 1 : 0;
     return (S)(d == d ? (unsigned)fmaf(d, 46000.f, 0.1875f * 46000.f + 0.5f) : 0xffffu);
   }
-  // dy act': ReLU's may also be the result itself (its sign; NaN lets dy through)
-  __device__ static __forceinline__ T times(T dy, S v, int act) {
-    if (act == kActRelu) return (short)v > 0 ? dy : (T)0.f;   // (an infinite dy stays out of it)
+  __device__ static __forceinline__ T times(T dy, S v, int act) {   // dy act'
+    constexpr int inf = __is_same(T, __bf16) ? 0x7f80 : 0x7c00;
+    if (act == kActRelu)                         // (an infinite dy stays out of it)
+      return (short)v > 0 || (v & 0x7fff) > inf ? dy : (T)0.f;
     return v != 0xffff ? (T)((float)dy * fmaf((float)v, 1.f / 46000.f, -0.1875f))
                        : (T)__builtin_nanf("");
   }
@@ -216,7 +220,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs &g, long long row, int c
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float d;
-    y[j] = (T)(activate<sizeof(T) == 4>(s[j] + (float)bias[j], g.act, d) + (float)res[j]);
+    y[j] = (T)(activate<T>(s[j] + (float)bias[j], g.act, d) + (float)res[j]);
     slope[j] = Slope<T>::keep(d, g.act);
   }
   if (g.slope) store_row((typename Slope<T>::S *)g.slope + row * g.n, col, g.n, slope);

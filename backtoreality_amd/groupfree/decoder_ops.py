@@ -194,7 +194,7 @@ def _linear_forward(x, weight, bias, residual, act, keep):
     kept, slope = None, None          # kept: what dz is made of in the backward
     if act and keep:
         if act == 1 and residual is None:
-            kept = y                                              # y > 0 exactly where z > 0
+            kept = y                    # on where y > 0 or NaN: a z that rounds to 0 is off
         else:
             kept = slope = torch.empty((m, n), dtype=x.dtype, device=dev)
     p = _ext.Linear(_DTYPES[x.dtype], m, n, k, act, xr.data_ptr(), wr.data_ptr(), _ptr(b), _ptr(rr),

@@ -76,3 +76,31 @@ def test_float16_gradients_with_large_values(cuda, Lq, Lk, H, Hk, D, size, even)
     assert all(float(value.abs().max()) < 3e4 for _, value, _ in want[1:])
     for t, (name, value, bound) in zip(_attention_grads(q, k, v, dy, D ** -0.5), want):
         ref.close(name, t, value, bound)
+
+
+# -------------------------------------------------------------------------------------- activations
+@pytest.mark.parametrize("dtype", ref.DTYPES, ids=str)
+@pytest.mark.parametrize("cols", [1, 70])        # straight from the long operand, and in tiles
+def test_relu_with_and_without_a_residual_agree_on_what_is_on(cuda, dtype, cols):
+    """NaN of either sign lets the gradient through, as torch's ReLU does; what counts as positive does
+    not depend on a residual: a z that the type rounds to zero is off."""
+    nan = torch.tensor([0x7fc0, 0xffc0 - 0x10000], dtype=torch.int16, device=cuda).view(torch.bfloat16)
+    far = float("inf") if dtype != torch.float32 else 2.0      # (infinite float32: NaN, as documented)
+    z = torch.cat([torch.tensor([1.0, -1.0, 0.0, -0.0, far, -far], device=cuda), nan.float()]).to(dtype)
+    on = torch.tensor([1, 0, 0, 0, 1, 0, 1, 1], device=cuda, dtype=dtype)
+    x = _leaf(z.repeat(40)[:, None])
+    w, b = torch.ones((cols, 1), device=cuda, dtype=dtype), _leaf(torch.zeros(cols, device=cuda, dtype=dtype))
+    small = 2.0 ** -13
+    grads = []
+    for residual in (None, torch.zeros((320, cols), device=cuda, dtype=dtype)):
+        y = ops.linear(x, w, b, activation="relu", residual=residual)
+        dx, db = torch.autograd.grad(y, [x, b], torch.ones_like(y))
+        assert torch.equal(dx[:, 0], on.repeat(40) * cols)
+        assert bool((db == 40 * on.sum()).all())
+        # two factors of 2^-13: 2^-26, which float16 rounds to zero and the others keep
+        t = _leaf(torch.full((320, 1), small, device=cuda, dtype=dtype))
+        y = ops.linear(t, torch.full((cols, 1), small, device=cuda, dtype=dtype), activation="relu",
+                       residual=residual)
+        grads.append(torch.autograd.grad(y, [t], torch.ones_like(y))[0])
+    assert torch.equal(grads[0], grads[1])
+    assert bool((grads[0] == 0).all()) == (dtype == torch.float16)
