@@ -21,9 +21,10 @@
 // long, which the bf16 matrix pipe does 2.7 times faster than the f32 instructions do one; an
 // infinite f32 element makes the sums it enters NaN.  What the backward needs of the activation is
 // its slope act'(z), taken from the f32 sum in the forward's epilogue and kept in as many bits as x
-// has: for GELU's of 16 bits a fixed-point number (steps of 1 / 46 000 from -0.1875: 1e-5 at most,
-// against 2^-9 for a bf16 slope, which was a third of the gradients' error).  dz is rounded to the
-// type of x before the two products that read it.
+// has: for GELU's of 16 bits a fixed-point number, off by 2^-16 at most (a bf16 slope, off by 2^-9 of
+// itself, was a third of the gradients' error), and a floating-point one for the small slopes of the
+// negative tail, off by 2^-10 of itself down to 2^-30, below which it is 0 (z < -6.6).  dz is rounded to
+// the type of x before the two products that read it.
 #include <algorithm>
 #include <cstdint>
 
@@ -173,22 +174,30 @@ __device__ __forceinline__ float activate(float z, int act, float &slope) {
   return z;
 }
 
-// The slope as the backward gets it: f32 itself, or 16 bits -- GELU's in fixed point (at most 1.13:
-// below 60 600; all ones stand for NaN; what pads a row reads as 0 and must give 0), ReLU's 1 or 0.
-// For ReLU the result may stand in its place: on where it is positive or NaN.
+// The slope as the backward gets it: f32 itself, or 16 bits.  GELU's:
+//   code 0 .. 12 799: -2^-5 < slope <= -2^-30, the float's bits from 2^-30 on, 9 of its mantissa
+//   up to 64 446:     slope * 40 960 + 18 200 for all others (-0.1291 .. 1.1291; 0 comes back as 0)
+//   65 535:           NaN
+// (What pads a row reads as 0, against a dy of 0.)  ReLU's: 1 or 0, and the result may stand in its place:
+// on where it is positive or NaN.
+constexpr unsigned kTailBits = 0x80000000u | (127u - 30u) << 23, kTailCodes = 25 * 512;   // of -2^-30
+constexpr float kSlopeUnit = 40960.f, kSlopeZero = 18200.f;
 template <typename T>
 struct Slope {
   typedef unsigned short S;
   __device__ static __forceinline__ S keep(float d, int act) {
     if (act == kActRelu) return d > 0.f || d != d ? 1 : 0;
-    return (S)(d == d ? (unsigned)fmaf(d, 46000.f, 0.1875f * 46000.f + 0.5f) : 0xffffu);
+    const unsigned tail = __float_as_uint(d) - kTailBits + (1u << 13);   // (others wrap to large ones)
+    const unsigned fixed = (unsigned)fminf(fmaf(d, kSlopeUnit, kSlopeZero + 0.5f), 65535.f);   // (NaN too)
+    return (S)(tail < kTailCodes << 14 ? tail >> 14 : fixed);
   }
   __device__ static __forceinline__ T times(T dy, S v, int act) {   // dy act'
     constexpr int inf = __is_same(T, __bf16) ? 0x7f80 : 0x7c00;
     if (act == kActRelu)                         // (an infinite dy stays out of it)
       return (short)v > 0 || (v & 0x7fff) > inf ? dy : (T)0.f;
-    return v != 0xffff ? (T)((float)dy * fmaf((float)v, 1.f / 46000.f, -0.1875f))
-                       : (T)__builtin_nanf("");
+    float d = ((float)v - kSlopeZero) * (1.f / kSlopeUnit);
+    if (v < kTailCodes) d = __uint_as_float(kTailBits + ((unsigned)v << 14));
+    return v != 0xffff ? (T)((float)dy * d) : (T)__builtin_nanf("");
   }
 };
 template <>

@@ -104,3 +104,27 @@ def test_relu_with_and_without_a_residual_agree_on_what_is_on(cuda, dtype, cols)
         grads.append(torch.autograd.grad(y, [t], torch.ones_like(y))[0])
     assert torch.equal(grads[0], grads[1])
     assert bool((grads[0] == 0).all()) == (dtype == torch.float16)
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES, ids=str)
+@pytest.mark.parametrize("cols", [1, 70])
+def test_gelu_gradient_in_the_tail(cuda, dtype, cols):
+    """z in [-6, -4], slopes from 7e-4 to 4e-8: relative to each.  One term per row (W one column's
+    unit): the slope's own arithmetic 2^-14 and, for 16 bits, its code's half step 2^-10, dz's rounding
+    and the result's."""
+    n = 1000
+    z = torch.linspace(-6.0, -4.0, n, device=cuda).to(dtype)
+    x = _leaf(z[:, None])
+    w = torch.zeros((cols, 1), device=cuda, dtype=dtype)
+    w[cols // 2] = 1
+    dy = torch.full((n, cols), 2.0 ** 14, device=cuda, dtype=dtype)
+    # (the other columns' z is 0: their slope of a half meets a weight of 0)
+    (dx,) = torch.autograd.grad(ops.linear(x, w, activation="gelu"), [x], dy)
+    want = ref.linear(x, w, None, "gelu", None, dy)[1][1]
+    u = ref.half_step(dtype)
+    rel = 2.0 ** -14 if dtype == torch.float32 else 2.0 ** -14 + 2.0 ** -10 + 2 * u
+    ref.close("dx", dx, want, rel * want.abs() + ref.tiny(dtype))
+    # beyond: exactly nothing
+    x = _leaf(torch.tensor([[-20.0], [-40.0], [-300.0]], device=cuda, dtype=dtype))
+    (dx,) = torch.autograd.grad(ops.linear(x, w, activation="gelu"), [x], dy[:3])
+    assert not dx.any()
