@@ -24,7 +24,9 @@
 // has: for GELU's of 16 bits a fixed-point number, off by 2^-16 at most (a bf16 slope, off by 2^-9 of
 // itself, was a third of the gradients' error), and a floating-point one for the small slopes of the
 // negative tail, off by 2^-10 of itself down to 2^-30, below which it is 0 (z < -6.6).  dz is rounded to
-// the type of x before the two products that read it.
+// the type of x before the two products that read it (dbias is summed from the f32 values); a float16
+// GELU's, which its slopes push towards the type's smallest numbers, as dz times the power of two that
+// fits the largest |dy|.
 #include <algorithm>
 #include <cstdint>
 
@@ -49,9 +51,15 @@ struct GemmArgs {
   void *c, *slope;           // contiguous (m, n); slope: act' of the sums (Slope), or NULL
   float *part;               // split reduction: (nsplit, m, n) partial sums
   int nsplit, chunk;         // shares of k, their length
+  const float *unscale;      // float16: factor of the sums, or NULL (1)
   long long aplane, bplane;  // f32: elements from one bf16 plane of an operand to the next
   int mt, nt;                // tiles
 };
+
+template <typename T>
+constexpr bool kHalf = false;
+template <>
+constexpr bool kHalf<_Float16> = true;
 
 // what the matrix instructions eat: T itself, or three bf16 planes of f32
 template <typename T>
@@ -191,13 +199,13 @@ struct Slope {
     const unsigned fixed = (unsigned)fminf(fmaf(d, kSlopeUnit, kSlopeZero + 0.5f), 65535.f);   // (NaN too)
     return (S)(tail < kTailCodes << 14 ? tail >> 14 : fixed);
   }
-  __device__ static __forceinline__ T times(T dy, S v, int act) {   // dy act'
-    constexpr int inf = __is_same(T, __bf16) ? 0x7f80 : 0x7c00;
+  __device__ static __forceinline__ float times(T dy, S v, int act) {   // dy act'
+    constexpr int inf = kHalf<T> ? 0x7c00 : 0x7f80;
     if (act == kActRelu)                         // (an infinite dy stays out of it)
-      return (short)v > 0 || (v & 0x7fff) > inf ? dy : (T)0.f;
+      return (short)v > 0 || (v & 0x7fff) > inf ? (float)dy : 0.f;
     float d = ((float)v - kSlopeZero) * (1.f / kSlopeUnit);
     if (v < kTailCodes) d = __uint_as_float(kTailBits + ((unsigned)v << 14));
-    return v != 0xffff ? (T)((float)dy * d) : (T)__builtin_nanf("");
+    return (float)dy * (v != 0xffff ? d : __builtin_nanf(""));
   }
 };
 template <>
@@ -226,10 +234,13 @@ __device__ __forceinline__ void epilogue(const GemmArgs &g, long long row, int c
   constexpr int V = Elem<T>::kVec;
   typename Elem<T>::Vec y;
   typename Elem<typename Slope<T>::S>::Vec slope;
+  float u = 1.f;
+  if (kHalf<T> && g.unscale) u = *g.unscale;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float d;
-    y[j] = (T)(activate<T>(s[j] + (float)bias[j], g.act, d) + (float)res[j]);
+    const float sum = kHalf<T> ? s[j] * u : s[j];
+    y[j] = (T)(activate<T>(sum + (float)bias[j], g.act, d) + (float)res[j]);
     slope[j] = Slope<T>::keep(d, g.act);
   }
   if (g.slope) store_row((typename Slope<T>::S *)g.slope + row * g.n, col, g.n, slope);
@@ -743,20 +754,75 @@ __global__ __launch_bounds__(256) void linear_join_kernel(GemmArgs g) {
   }
 }
 
-// dz = dy slope (ReLU: dy where slope > 0) into rows of ldz elements, zeros behind them (f32: into
+// the largest finite |dy| of each workgroup's rows (16 384 x 4 096: 38 us, 3.5 TB/s)
+constexpr int kMostBlocks = 1024;
+template <typename T>
+__global__ __launch_bounds__(256) void linear_most_kernel(long long m, int n, const T *dy,
+                                                          long long lddy, float *most) {
+  constexpr int V = Elem<T>::kVec;
+  __shared__ float red[4];
+  const int per_row = (n + V - 1) / V, at = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
+  const int rows = step / per_row, pieces = step - rows * per_row;   // from one piece to the next
+  long long row = at / per_row;
+  int piece = at - (int)row * per_row;
+  float big = 0.f;
+  while (row < m) {
+    typename Elem<T>::Vec g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                  // (four loads in flight; past the end: the last row)
+      g[i] = load_row(dy + min(row, m - 1) * lddy, piece * V, n);
+      row += rows;
+      piece += pieces;
+      if (piece >= per_row) {
+        piece -= per_row;
+        ++row;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = fabsf((float)g[i][j]);
+        big = a < INFINITY ? fmaxf(big, a) : big;
+      }
+  }
+  for (int i = 32; i > 0; i >>= 1) big = fmaxf(big, __shfl_xor(big, i));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) most[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// dz = dy slope (ReLU: dy where it is on) into rows of ldz elements, zeros behind them (f32: into
 // its three planes), and the column sums of dz over this workgroup's rows: 32 threads along the
 // columns (8 each), 8 rows at a time.  dz NULL: the sums only.  (Bound by memory: 16 384 x 4 096 bf16
 // 74 us, 5.4 TB/s.  In the products' own staging it would be recomputed per tile, 4 to 64 times.)
+// most (float16, `count` of them, then the place of the factor that undoes it, or NULL): dz is written
+// as 2^up dz, |dz| <= 1.13 |dy| < 2^(e + 1) as below 1.13 2^14.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, const T *dy,
                                                         long long lddy, const typename Slope<T>::S *slope,
                                                         int act,
                                                         typename Matrix<T>::E *dz, int ldz,
-                                                        long long plane, float *part) {
+                                                        long long plane, float *part, float *most,
+                                                        int count) {
   constexpr int V = Elem<T>::kVec, H = 8 / V;
   typedef typename Elem<T>::Vec Vec;
   __shared__ float red[8][32 * 8];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, col = (blockIdx.x * 32 + cl) * 8;
+  float up = 1.f;
+  if (kHalf<T> && most) {
+    float big = 0.f;
+    for (int i = threadIdx.x; i < count; i += 256) big = fmaxf(big, most[i]);
+    for (int i = 32; i > 0; i >>= 1) big = fmaxf(big, __shfl_xor(big, i));
+    if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = big;
+    __syncthreads();
+    big = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    __syncthreads();
+    const int e = 14 - __builtin_amdgcn_frexp_expf(big);
+    up = __builtin_ldexpf(1.f, e);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+      most[count] = __builtin_ldexpf(1.f, -e);
+  }
   float sum[8] = {};
   if (col < n)
     for (long long row = (long long)blockIdx.y * 8 + rl; row < m; row += (long long)gridDim.y * 8) {
@@ -771,8 +837,10 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long m, int n, cons
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if (act != kActNone) g[h][j] = Slope<T>::times(g[h][j], d[h][j], act);
-          sum[h * V + j] += (float)g[h][j];
+          float z = (float)g[h][j];
+          if (act != kActNone) z = Slope<T>::times(g[h][j], d[h][j], act);
+          sum[h * V + j] += z;
+          g[h][j] = (T)(kHalf<T> ? z * up : z);
         }
       if (dz) {
         typename Op<T>::Frag f[Op<T>::P];
@@ -989,10 +1057,15 @@ void forward(const btr_linear_t &p, void *y, void *slope, void *workspace, hipSt
 bool writes_dz(const btr_linear_t &p, const void *dy, long long lddy) {
   return p.act != BTR_ACT_NONE || !dma_rows(p.dtype, dy, lddy, p.n);
 }
+// float16 dz with slopes below 1: scaled.  The floats that takes: the workgroups' largest |dy|, the factor
+bool scales_dz(const btr_linear_t &p) { return p.dtype == BTR_F16 && p.act == BTR_ACT_GELU; }
+size_t most_bytes(const btr_linear_t &p) {
+  return scales_dz(p) ? align256((kMostBlocks + 1) * sizeof(float)) : 0;
+}
 size_t bwd_bytes(const btr_linear_t &p, const void *dy, long long lddy) {
   const int m = p.m, n = p.n, k = p.k;
   if (m == 0) return 0;
-  size_t v = align256((size_t)dz_blocks(m, n) * n * sizeof(float));
+  size_t v = align256((size_t)dz_blocks(m, n) * n * sizeof(float)) + most_bytes(p);
   if (writes_dz(p, dy, lddy)) v += packed_bytes(p.dtype, m, n);
   v += pack_bytes(p.dtype, p.x, p.ldx, m, k) + pack_bytes(p.dtype, p.weight, p.ldw, n, k);
   return v + std::max(split_bytes(m, k, n, p.dtype), split_bytes(n, k, m, p.dtype));
@@ -1007,8 +1080,17 @@ void backward(const btr_linear_t &p, const void *slope, const void *dy, long lon
   float *part = (float *)ws;
   const int blocks = m > 0 ? dz_blocks(m, n) : 0;
   Rows dz{dy, lddy, 0, m, n};                      // what the two products read
+  float *most = nullptr;
   if (m > 0) {
     ws += align256((size_t)blocks * n * sizeof(float));
+    if constexpr (kHalf<T>) {
+      if (scales_dz(p) && (dx || dweight)) {
+        most = (float *)ws;
+        hipLaunchKernelGGL((linear_most_kernel<T>), dim3(kMostBlocks), dim3(256), 0, hs, (long long)m,
+                           n, (const T *)dy, lddy, most);
+      }
+    }
+    ws += most_bytes(p);
     E *out = nullptr;
     if (writes_dz(p, dy, lddy) && (dx || dweight)) {
       out = (E *)ws;
@@ -1019,22 +1101,23 @@ void backward(const btr_linear_t &p, const void *slope, const void *dy, long lon
       hipLaunchKernelGGL((linear_dz_kernel<T>), dim3(cdiv(n, 256), blocks), dim3(256), 0, hs,
                          (long long)m, n, (const T *)dy, lddy,
                          (const typename Slope<T>::S *)slope, p.act, out, up8(n),
-                         dz.plane, dbias ? part : nullptr);
+                         dz.plane, dbias ? part : nullptr, most, kMostBlocks);
   }
   if (dbias)   // (no rows: zeros)
     hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3(cdiv(n, 32)), dim3(1024), 0, hs, part, blocks, n,
                        (T *)dbias);
+  const float *unscale = most ? most + kMostBlocks : nullptr;
   Rows op[2] = {{p.weight, p.ldw, 0, n, k}, {p.x, p.ldx, 0, m, k}};
   if (m > 0 && (dx || dweight))
     pack_rows<T>(op + (dx ? 0 : 1), (dx ? 1 : 0) + (dweight ? 1 : 0), ws, hs);
   if (dx && m > 0) {
     GemmArgs g{};
-    g.m = m; g.n = k; g.k = n; g.c = dx;
+    g.m = m; g.n = k; g.k = n; g.c = dx; g.unscale = unscale;
     launch_gemm<T, false, true>(g, dz, op[0], ws, hs);
   }
   if (dweight) {
     GemmArgs g{};
-    g.m = n; g.n = k; g.k = m; g.c = dweight;      // (no rows: an empty reduction writes zeros)
+    g.m = n; g.n = k; g.k = m; g.c = dweight; g.unscale = unscale;   // (no rows: writes zeros)
     launch_gemm<T, true, true>(g, dz, op[1], ws, hs);
   }
 }

@@ -128,3 +128,30 @@ def test_gelu_gradient_in_the_tail(cuda, dtype, cols):
     x = _leaf(torch.tensor([[-20.0], [-40.0], [-300.0]], device=cuda, dtype=dtype))
     (dx,) = torch.autograd.grad(ops.linear(x, w, activation="gelu"), [x], dy[:3])
     assert not dx.any()
+
+
+@pytest.mark.parametrize("m,k,n", [(100, 48, 96), (700, 130, 65), (5, 33, 7)])
+@pytest.mark.parametrize("size,ws,xs", [(2.0 ** -13, 2.0 ** 9, 2.0 ** 9), (2.0 ** -20, 2.0 ** 13, 2.0 ** 13)])
+def test_float16_gelu_gradients_use_their_range(cuda, m, k, n, size, ws, xs):
+    """A small dy on slopes of 2^-5 and less: dz below float16's smallest normal value, weights and
+    inputs that bring dx and dW back into the range.  Each term: the slope's relative error (2^-10 of its
+    code, 2^-12 of its arithmetic and of z's sum), dz's rounding; the sums in float32."""
+    gen = _gen(300 + m)
+    f16, u = torch.float16, ref.half_step(torch.float16)
+    # z is the bias: x's one column of inputs meets a column of zeros
+    x, w = torch.zeros((m, k), device=cuda, dtype=f16), _randn(gen, (n, k), f16, ws)
+    x[:, 0], w[:, 0] = _randn(gen, (m,), f16, xs), 0
+    bias = -(torch.rand((n,), generator=gen, device=cuda) * 1.5 + 2.5).half()
+    x, w, bias = _leaf(x), _leaf(w), _leaf(bias)
+    dy = _randn(gen, (m, n), f16, size)
+    y = ops.linear(x, w, bias, activation="gelu")
+    dx, dw, db = torch.autograd.grad(y, [x, w, bias], dy)
+    z = x.double() @ w.double().t() + bias.double()
+    cdf = torch.special.erfc(-z / 2 ** 0.5) / 2
+    dz = dy.double() * (cdf + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5)
+    rel = u + 2.0 ** -10 + 2.0 ** -11
+    e = rel * dz.abs()
+    for name, got, want, bound in (("dx", dx, dz @ w.double(), e @ w.double().abs()),
+                                   ("dw", dw, dz.t() @ x.double(), e.t() @ x.double().abs()),
+                                   ("db", db, dz.sum(0), e.sum(0))):
+        ref.close(name, got, want, 1.01 * bound + u * want.abs() + ref.tiny(f16))
