@@ -19,7 +19,8 @@
 // once.  f32 operands are split into three bf16 terms (8 + 8 + 8 bits: exact up to the 24th) and
 // multiplied as the six products above 2^-24, the smallest first, as one reduction six times as
 // long, which the bf16 matrix pipe does 2.7 times faster than the f32 instructions do one; an
-// infinite f32 element makes the sums it enters NaN.  What the backward needs of the activation is
+// infinite f32 element makes the sums it enters NaN, and one below 2^-108 has fewer bits (its last term
+// is below 2^-126, the second from 2^-117).  What the backward needs of the activation is
 // its slope act'(z), taken from the f32 sum in the forward's epilogue and kept in as many bits as x
 // has: for GELU's of 16 bits a fixed-point number, off by 2^-16 at most (a bf16 slope, off by 2^-9 of
 // itself, was a third of the gradients' error), and a floating-point one for the small slopes of the
@@ -89,11 +90,14 @@ __device__ __forceinline__ f32x16_t mfma(f16x8_t a, f16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// f = h + m + l; an h that left the range of bf16 keeps no rest
+// f = h + m + l.  Above bf16's largest value h is cut instead of rounded (rounded it would be infinite); an
+// infinite element keeps no rest.
 __device__ __forceinline__ void split3(f32x4_t f, bf16x4_t (&p)[3]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __bf16 h = (__bf16)f[i];
+    __bf16 h = (__bf16)f[i];
+    if (!(__builtin_fabsf((float)h) < INFINITY) && __builtin_fabsf(f[i]) < INFINITY)
+      h = __builtin_bit_cast(__bf16, (unsigned short)(__float_as_uint(f[i]) >> 16));
     float r = f[i] - (float)h;
     if (!(__builtin_fabsf((float)h) < INFINITY)) r = 0.f;
     const __bf16 m = (__bf16)r;

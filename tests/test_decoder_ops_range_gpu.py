@@ -155,3 +155,37 @@ def test_float16_gelu_gradients_use_their_range(cuda, m, k, n, size, ws, xs):
                                    ("dw", dw, dz.t() @ x.double(), e.t() @ x.double().abs()),
                                    ("db", db, dz.sum(0), e.sum(0))):
         ref.close(name, got, want, 1.01 * bound + u * want.abs() + ref.tiny(f16))
+
+
+# --------------------------------------------------------------------------- float32's largest elements
+@pytest.mark.parametrize("m,k,n", [(3, 40, 50), (200, 40, 200), (300, 700, 20), (130, 64, 70)])
+def test_float32_elements_above_the_largest_bfloat16(cuda, m, k, n):
+    """Finite operands between bfloat16's largest value and float32's, small ones against them: every
+    product finite and as exact as any other."""
+    gen = _gen(400 + m)
+    f32, top = torch.float32, torch.finfo(torch.float32).max
+    big = torch.tensor([top, -top, top * (1 - 2.0 ** -9 + 2.0 ** -12), -top * (1 - 2.0 ** -12)], device=cuda)
+
+    def sprinkle(t, every):
+        t = t.clone()
+        at = torch.arange(0, t.numel(), every, device=cuda)
+        t.view(-1)[at] = big[torch.arange(len(at), device=cuda) % 4]
+        return t
+    x = _leaf(sprinkle(_randn(gen, (m, k), f32), 7 * k + 1))       # one of a row at most
+    w = _leaf(_randn(gen, (n, k), f32, 2.0 ** -10))
+    dy = _randn(gen, (m, n), f32, 2.0 ** -20)
+    y = ops.linear(x, w)
+    want = ref.linear(x, w, None, None, None, dy)
+    for t, (name, value, bound) in zip([y] + list(torch.autograd.grad(y, [x, w], dy)), want):
+        ref.close(name, t.detach(), value, bound)
+    # ... in the weight
+    x, w = _leaf(_randn(gen, (m, k), f32, 2.0 ** -10)), _leaf(sprinkle(_randn(gen, (n, k), f32), 7 * k + 1))
+    y = ops.linear(x, w)
+    want = ref.linear(x, w, None, None, None, dy)
+    for t, (name, value, bound) in zip([y] + list(torch.autograd.grad(y, [x, w], dy)), want):
+        ref.close(name, t.detach(), value, bound)
+    # ... and in dy
+    w, dy = _leaf(_randn(gen, (n, k), f32, 2.0 ** -10)), sprinkle(_randn(gen, (m, n), f32), 7 * n + 1)
+    want = ref.linear(x, w, None, None, None, dy)[1:]
+    for t, (name, value, bound) in zip(torch.autograd.grad(ops.linear(x, w), [x, w], dy), want):
+        ref.close(name, t, value, bound)
