@@ -885,14 +885,15 @@ struct Plan {
 // full chip at 16 384 x 4 096 x 1 024 and 16 384 x 1 024 x 4 096, one workgroup or two per CU at 1 024 x
 // (32 .. 2 048) x 2 048.  f32 runs six passes over k.
 Plan plan_gemm(int m, int n, int k, int passes) {
-  static const struct { int bm, bn; double step, fixed, alone; } kTile[4] = {
-      {256, 256, 1.65, 11.0, 1.06}, {256, 128, 1.02, 6.7, 0.62}, {128, 128, 0.65, 5.5, 0.8},
-      {64, 64, 0.22, 2.0, 0.2}};
+  static const struct { int bm, bn, threads; double step, fixed, alone; } kTile[4] = {
+      {256, 256, 512, 1.65, 11.0, 1.06}, {256, 128, 512, 1.02, 6.7, 0.62},
+      {128, 128, 256, 0.65, 5.5, 0.8}, {64, 64, 256, 0.22, 2.0, 0.2}};
   Plan best{};
   double least = 1e30;
   for (const auto &t : kTile) {
     const int mt = cdiv(m, t.bm), nt = cdiv(n, t.bn);
     const long long tiles = (long long)mt * nt;
+    if (tiles * t.threads >= 1ll << 32) continue;  // (a grid's thread numbers; check(): not all tiles)
     for (int s = 1; s <= 32 && (s == 1 || (k / s * passes >= 128 && tiles * s <= 2048)); ++s) {
       const int chunk = std::max(64, cdiv(cdiv(k, s), 64) * 64), real = std::max(1, cdiv(k, chunk));
       if (real != s) continue;
@@ -997,9 +998,9 @@ int check(const char *what, const btr_linear_t *p) {
               p->act);
   const int m = p->m, n = p->n, k = p->k;
   BTR_REQUIRE(m >= 0 && n >= 1 && k >= 1 && m <= (1 << 30) && n <= (1 << 22) && k <= (1 << 22) &&
-                  ((long long)cdiv(m, 64) * cdiv(n, 64) <= (1 << 30)) &&
-                  ((long long)cdiv(m, 64) * cdiv(k, 64) <= (1 << 30)) &&
-                  ((long long)cdiv(n, 64) * cdiv(k, 64) <= (1 << 30)),
+                  ((long long)cdiv(m, 256) * cdiv(n, 256) <= (1 << 22)) &&
+                  ((long long)cdiv(m, 256) * cdiv(k, 256) <= (1 << 22)) &&
+                  ((long long)cdiv(n, 256) * cdiv(k, 256) <= (1 << 22)),
               "%s: (%d, %d) x (%d, %d)", what, m, k, n, k);
   BTR_REQUIRE(m == 0 || (p->x && p->weight && p->ldx >= k && p->ldw >= k &&
                          (!p->residual || p->ldr >= n)),
@@ -1031,6 +1032,21 @@ void launch_rows(const GemmArgs &g, int few, int many, hipStream_t hs) {
       hipLaunchKernelGGL((linear_rows_kernel<T, 4, COLS>), grid, dim3(512), 0, hs, g);
   }
 }
+// few outputs: as many rows a launch as a grid of 32-bit thread numbers has room for
+template <typename T>
+void launch_columns(GemmArgs g, hipStream_t hs) {
+  constexpr int kRows = 1 << 26;                   // 2^31 threads
+  const int m = g.m, n = g.n;
+  for (int row = 0; row < m; row += kRows) {       // (m <= 2^30: no overflow)
+    GemmArgs part = g;
+    part.m = std::min(kRows, m - row);
+    part.a = (const T *)g.a + row * g.lda;
+    part.c = (T *)g.c + (long long)row * n;
+    if (g.res) part.res = (const T *)g.res + row * g.ldres;
+    if (g.slope) part.slope = (typename Slope<T>::S *)g.slope + (long long)row * n;
+    launch_rows<T, true>(part, n, part.m, hs);
+  }
+}
 size_t fwd_bytes(const btr_linear_t &p) {
   if (few_rows(p) || few_columns(p)) return 0;
   return pack_bytes(p.dtype, p.x, p.ldx, p.m, p.k) + pack_bytes(p.dtype, p.weight, p.ldw, p.n, p.k) +
@@ -1048,7 +1064,7 @@ void forward(const btr_linear_t &p, void *y, void *slope, void *workspace, hipSt
     if (few_rows(p))
       launch_rows<T, false>(g, p.m, p.n, hs);
     else
-      launch_rows<T, true>(g, p.n, p.m, hs);
+      launch_columns<T>(g, hs);
     return;
   }
   char *ws = (char *)workspace;

@@ -1135,7 +1135,7 @@ int btr_layer_norm_bwd(int dtype, long long rows, int width, const void *x, long
 /* z = x weight^T + bias, y = act(z) [+ residual]: x (m, k), weight (n, k), bias (n) or NULL, residual
  * (m, n) or NULL, y (m, n) contiguous.  act: BTR_ACT_*; GELU is the erf form.  slope (m, n) contiguous,
  * of as many bytes as y: receives what the backward of an activation needs (act'(z), in a form of its
- * own), or NULL.  1 <= n, k <= 2^22. */
+ * own), or NULL.  1 <= n, k <= 2^22, m <= 2^30, no operand or result of more than 2^22 tiles of 256 x 256. */
 #define BTR_ACT_NONE 0
 #define BTR_ACT_RELU 1
 #define BTR_ACT_GELU 2

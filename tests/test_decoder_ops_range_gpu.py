@@ -189,3 +189,14 @@ def test_float32_elements_above_the_largest_bfloat16(cuda, m, k, n):
     want = ref.linear(x, w, None, None, None, dy)[1:]
     for t, (name, value, bound) in zip(torch.autograd.grad(ops.linear(x, w), [x, w], dy), want):
         ref.close(name, t, value, bound)
+
+
+# ------------------------------------------------------------------------- more than a grid has threads
+def test_linear_of_more_rows_than_one_launch_has_room_for(cuda):
+    """2^27 rows and a few, one input, one output: a power of two times each."""
+    m = 2 ** 27 + 5
+    x = torch.arange(m, device=cuda, dtype=torch.int32).remainder_(1021).float()[:, None]
+    w, b = torch.full((1, 1), 0.5, device=cuda), torch.full((1,), 3.0, device=cuda)
+    r = x.flip(0)
+    y = ops.linear(x, w, b, residual=r)
+    assert torch.equal(y, 0.5 * x + 3.0 + r)
