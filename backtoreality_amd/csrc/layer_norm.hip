@@ -223,14 +223,17 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void layer_norm_bwd_kernel(LnArg
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_params_kernel(const float *part, int blocks,
                                                                  int width, T *dw, T *db) {
-  const long long c = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
-  const float t = column_sum(part, blocks, 2ll * width, c);
-  if (threadIdx.x < 32 && c < 2ll * width) {
-    if (c < width) {
-      if (dw) dw[c] = (T)t;
-    } else if (db) {
-      db[c - width] = (T)t;
+  for (long long c0 = blockIdx.x * 32ll; c0 < 2ll * width; c0 += gridDim.x * 32ll) {
+    const long long c = c0 + (threadIdx.x & 31);
+    const float t = column_sum(part, blocks, 2ll * width, c);
+    if (threadIdx.x < 32 && c < 2ll * width) {
+      if (c < width) {
+        if (dw) dw[c] = (T)t;
+      } else if (db) {
+        db[c - width] = (T)t;
+      }
     }
+    __syncthreads();                             // (its LDS is used again)
   }
 }
 
@@ -463,7 +466,7 @@ extern "C" int btr_layer_norm_bwd(int dtype, long long rows, int width, const vo
   }
   if (params)   // (no rows: zeros)
     BTR_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(
-        (layer_norm_params_kernel<T>), dim3(cdiv(2ll * width, 32)), dim3(1024), 0, hs,
+        (layer_norm_params_kernel<T>), dim3(std::min(1 << 20, cdiv(2ll * width, 32))), dim3(1024), 0, hs,
         (const float *)workspace, blocks, width, (T *)dweight, (T *)dbias));
   return check_launch("layer_norm_bwd");
 }

@@ -200,3 +200,16 @@ def test_linear_of_more_rows_than_one_launch_has_room_for(cuda):
     r = x.flip(0)
     y = ops.linear(x, w, b, residual=r)
     assert torch.equal(y, 0.5 * x + 3.0 + r)
+
+
+def test_layer_norm_of_a_very_wide_row(cuda):
+    """2^26 columns: their parameter gradients are more than one grid of 32 columns a workgroup."""
+    n = 2 ** 26
+    x = (torch.arange(n, device=cuda, dtype=torch.int32).remainder_(5).float() - 2).half()[None]
+    w, b = _leaf(torch.ones(n, device=cuda, dtype=torch.float16)), _leaf(torch.zeros(n, device=cuda, dtype=torch.float16))
+    dy = x.flip(1).contiguous()
+    dw, db = torch.autograd.grad(ops.layer_norm(x, w, b), [w, b], dy)
+    assert torch.equal(db, dy[0])
+    xh = x.double() * (2.0 + 1e-5) ** -0.5       # (mean within 2^-24 of 0, mean square of 2)
+    off = (dw.double() - (dy.double() * xh)[0]).abs()
+    assert float(off.max()) <= 3 * 2.0 ** -11 + 1e-4
