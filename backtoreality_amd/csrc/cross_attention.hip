@@ -1564,7 +1564,7 @@ int check(const char *what, const btr_cross_attention_t *p, XaArgs &a) {
   a = XaArgs{};
   a.b = p->b; a.lq = p->lq; a.lk = p->lk; a.h = p->h; a.hk = p->hk; a.g = p->h / p->hk; a.d = p->d;
   const long long rows = (long long)p->lq * a.g;
-  // a workgroup list and a row index of 32 bits
+  // a workgroup list and a row index of 32 bits (check_grid: the launches)
   BTR_REQUIRE(rows <= (1 << 30) && p->lk <= (1 << 30) &&
                   (rows / 32 + p->lk / 128 + 2) * (long long)p->b * p->hk <= (1 << 30),
               "%s: too many rows (%lld) or keys (%d)", what, rows, p->lk);
@@ -1580,6 +1580,18 @@ int check(const char *what, const btr_cross_attention_t *p, XaArgs &a) {
   a.scale_log2 = p->scale * kLog2e;
   const bool some = p->b > 0 && p->lq > 0, keys = p->b > 0 && p->lk > 0;
   BTR_REQUIRE((!some || p->q) && (!keys || (p->k && p->v)), "%s: null pointer", what);
+  return BTR_OK;
+}
+
+// a launch's thread numbers have 32 bits
+int check_grid(const char *what, const XaArgs &a, int dtype, bool bwd) {
+  const long long bh = (long long)a.b * a.hk;
+  const auto threads = [&](const Shares &s, int per) { return s.tiles * bh * s.n * per; };
+  const bool wide = dtype != BTR_F32 && dma_rows_per(a) == 256 && (bwd || !few(a.rows));
+  long long most = threads(row_shares(a, dtype, !bwd), wide ? 512 : 256);
+  if (bwd) most = std::max(most, threads(key_shares(a), 256));
+  BTR_REQUIRE(most < 1ll << 32, "%s: batch %d, %d key heads, %d rows, %d keys: too many workgroups", what,
+              a.b, a.hk, a.rows, a.lk);
   return BTR_OK;
 }
 
@@ -1604,14 +1616,18 @@ using namespace btr;
 
 extern "C" size_t btr_cross_attention_fwd_workspace_bytes(const btr_cross_attention_t *p) {
   XaArgs a;
-  if (check("cross_attention", p, a) != BTR_OK) return 0;
+  if (check("cross_attention", p, a) != BTR_OK ||
+      check_grid("cross_attention", a, p->dtype, false) != BTR_OK)
+    return 0;
   return fwd_bytes(a, p->dtype);
 }
 
 extern "C" size_t btr_cross_attention_bwd_workspace_bytes(const btr_cross_attention_t *p,
                                                           const void *dout) {
   XaArgs a;
-  if (check("cross_attention", p, a) != BTR_OK) return 0;
+  if (check("cross_attention", p, a) != BTR_OK ||
+      check_grid("cross_attention", a, p->dtype, true) != BTR_OK)
+    return 0;
   a.dout = dout;
   return bwd_bytes(a, p->dtype);
 }
@@ -1620,7 +1636,8 @@ extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out
                                        void *workspace, size_t workspace_bytes,
                                        btr_stream_t stream) {
   XaArgs a;
-  const int rc = check("cross_attention_fwd", p, a);
+  int rc = check("cross_attention_fwd", p, a);
+  if (rc == BTR_OK) rc = check_grid("cross_attention_fwd", a, p->dtype, false);
   if (rc != BTR_OK) return rc;
   if (a.b == 0 || a.rows == 0) return BTR_OK;
   BTR_REQUIRE(out, "cross_attention_fwd: null pointer");
@@ -1655,7 +1672,8 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
                                        void *dv, void *workspace, size_t workspace_bytes,
                                        btr_stream_t stream) {
   XaArgs a;
-  const int rc = check("cross_attention_bwd", p, a);
+  int rc = check("cross_attention_bwd", p, a);
+  if (rc == BTR_OK) rc = check_grid("cross_attention_bwd", a, p->dtype, true);
   if (rc != BTR_OK) return rc;
   if (a.b == 0) return BTR_OK;
   BTR_REQUIRE((a.rows == 0 || (out && lse && dout && dq)) && (a.lk == 0 || (dk && dv)),

@@ -1158,7 +1158,8 @@ int btr_linear_bwd(const btr_linear_t *p, const void *slope, const void *dy, lon
 
 /* out = softmax(scale q k^T) v per head, q (b, lq, h, d), k / v (b, lk, hk, d) with strides
  * (batch, length, head); h % hk == 0, query head i reads key head i / (h / hk); d <= 128, h / hk
- * <= 128, scale > 0.
+ * <= 128, scale > 0; refused where a launch would have 2^32 threads or more
+ * (b * hk workgroups of 256 for every 128 rows lq * h / hk, in the backward also for every 128 keys).
  * Keys j >= lengths[b] (int32, or NULL: all lk; values outside [0, lk] are clamped) and keys with
  * mask[b * mask_sb + j] != 0 (one byte each, or NULL) take no part, whatever their rows hold; a
  * query without keys gets zeros.  out (b, lq, h, d) contiguous; lse: b * h * lq floats for the
