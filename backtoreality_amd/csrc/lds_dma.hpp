@@ -59,18 +59,21 @@ __device__ __forceinline__ unsigned lds_at(const char *lds) {
   return __builtin_amdgcn_readfirstlane(
       (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)lds);
 }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // (m0 is reserved: it warns, and honours it)
 __device__ __forceinline__ void dma16(i32x4_t rsrc, int off, const char *lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds_at(lds)), "v"(off), "s"(rsrc)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(i32x4_t rsrc, int off, const char *lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(lds_at(lds)), "v"(off), "s"(rsrc)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // The DMA instructions are the compiler's to count only through this: what it has loaded itself must
 // have arrived before the first of them, or it waits for everything in flight at the first use.
