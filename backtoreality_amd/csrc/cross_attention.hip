@@ -1644,6 +1644,7 @@ extern "C" int btr_cross_attention_fwd(const btr_cross_attention_t *p, void *out
   const size_t need = fwd_bytes(a, p->dtype);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "cross_attention_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  BTR_REQUIRE(aligned16(workspace), "cross_attention_fwd: workspace off a 16-byte boundary");
   a.out = out;
   a.lse = lse;
   hipStream_t hs = as_stream(stream);
@@ -1683,6 +1684,7 @@ extern "C" int btr_cross_attention_bwd(const btr_cross_attention_t *p, const voi
   const size_t need = bwd_bytes(a, p->dtype);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "cross_attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  BTR_REQUIRE(aligned16(workspace), "cross_attention_bwd: workspace off a 16-byte boundary");
   a.out = const_cast<void *>(out);
   a.lse = const_cast<float *>(lse);
   a.dq = dq; a.dk = dk; a.dv = dv;

@@ -74,6 +74,9 @@ __device__ __forceinline__ void store_row(T *row, int e0, int n, typename Elem<T
   }
 }
 
+// workspaces are written and read in 16-byte units (NULL where none is needed)
+inline bool aligned16(const void *p) { return ((unsigned long long)p & 15) == 0; }
+
 // sum over the 64 lanes, in every lane
 __device__ __forceinline__ float wave_sum_f32(float v) {
   v = row16_sum_f32(v);

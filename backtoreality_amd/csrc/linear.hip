@@ -1160,6 +1160,7 @@ extern "C" int btr_linear_fwd(const btr_linear_t *p, void *y, void *slope, void 
   const size_t need = fwd_bytes(*p);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "linear_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  BTR_REQUIRE(aligned16(workspace), "linear_fwd: workspace off a 16-byte boundary");
   BTR_DISPATCH_DTYPE(p->dtype, forward<T>(*p, y, slope, workspace, as_stream(stream)));
   return check_launch("linear_fwd");
 }
@@ -1179,6 +1180,7 @@ extern "C" int btr_linear_bwd(const btr_linear_t *p, const void *slope, const vo
   const size_t need = bwd_bytes(*p, dy, lddy);
   BTR_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
               "linear_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  BTR_REQUIRE(aligned16(workspace), "linear_bwd: workspace off a 16-byte boundary");
   BTR_DISPATCH_DTYPE(p->dtype, backward<T>(*p, slope, dy, lddy, dx, dweight, dbias, workspace,
                                            as_stream(stream)));
   return check_launch("linear_bwd");

@@ -1113,7 +1113,7 @@ int btr_grad_norm_final(int chunks, const float *partial, float clip, float *out
  * float32 whole-layer entry points above do not cover: 16-bit types, padded keys, key / value heads
  * shared by several query heads, any width, odd strides.  Strides are in elements, the last axis is
  * contiguous, rows may start at any element (16-byte alignment is not needed).  Workspaces are the
- * caller's: nothing is kept between calls, nothing is allocated, every call may be captured. */
+ * caller's, on 16-byte boundaries: nothing is kept between calls, nothing is allocated, every call may be captured. */
 #define BTR_F32 0
 #define BTR_BF16 1
 #define BTR_F16 2

@@ -45,3 +45,20 @@ def test_linear_grids_beyond_32_bits_are_refused():
         p = _ext.Linear(dtype=1, act=0, x=PTR, weight=PTR, ldx=2 ** 10, ldw=2 ** 10, **sizes)
         assert lib.btr_linear_fwd(ctypes.addressof(p), PTR, None, PTR, 1 << 60, None) == -1
         assert "linear_fwd" in _error()
+
+
+def test_workspaces_off_a_16_byte_boundary_are_refused():
+    odd = PTR + 8
+    p = _attention(lq=1, lk=100000)
+    need = lib.btr_cross_attention_fwd_workspace_bytes(ctypes.addressof(p))
+    assert need > 0
+    assert lib.btr_cross_attention_fwd(ctypes.addressof(p), PTR, None, odd, need, None) == -1
+    assert "16-byte" in _error()
+    assert lib.btr_cross_attention_bwd(ctypes.addressof(p), PTR, PTR, PTR, PTR, PTR, PTR, odd, 1 << 40,
+                                       None) == -1 and "16-byte" in _error()
+    p = _ext.Linear(dtype=1, m=100, n=100, k=15, act=0, x=PTR, weight=PTR, ldx=15, ldw=15)
+    need = lib.btr_linear_fwd_workspace_bytes(ctypes.addressof(p))
+    assert lib.btr_linear_fwd(ctypes.addressof(p), PTR, None, odd, need, None) == -1
+    assert "16-byte" in _error()
+    assert lib.btr_linear_bwd(ctypes.addressof(p), None, PTR, 100, PTR, PTR, PTR, odd, 1 << 40,
+                              None) == -1 and "16-byte" in _error()
