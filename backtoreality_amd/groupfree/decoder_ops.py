@@ -343,14 +343,15 @@ def cross_attention(query, key, value, key_lengths=None, key_padding_mask=None, 
     if not 1 <= D <= 128:
         _refuse("cross_attention: head width %d (1 .. 128)", D)
     if key_lengths is not None:
-        if key_lengths.dtype != torch.int32 or tuple(key_lengths.shape) != (B,) or \
-                key_lengths.device != query.device:
+        if not isinstance(key_lengths, torch.Tensor) or key_lengths.dtype != torch.int32 or \
+                tuple(key_lengths.shape) != (B,) or key_lengths.device != query.device:
             _refuse("cross_attention: key_lengths should be int32 of shape (%d,) on %s", B,
                     query.device)
         key_lengths = key_lengths.contiguous()
     if key_padding_mask is not None:
-        if key_padding_mask.dtype != torch.bool or tuple(key_padding_mask.shape) != (B, Lk) or \
-                key_padding_mask.device != query.device:
+        if not isinstance(key_padding_mask, torch.Tensor) or \
+                key_padding_mask.dtype != torch.bool or \
+                tuple(key_padding_mask.shape) != (B, Lk) or key_padding_mask.device != query.device:
             _refuse("cross_attention: key_padding_mask should be bool of shape (%d, %d) on %s", B, Lk,
                     query.device)
         key_padding_mask = _last_contiguous(key_padding_mask)

@@ -254,3 +254,11 @@ def test_a_trace_records_the_call(calls_on_the_cpu, name, grad):
         graph = torch.jit.trace(calls_on_the_cpu[name], torch.randn(4, 8), check_trace=False).graph
     kinds = [n.kind() for n in graph.nodes()]
     assert "prim::PythonOp" in kinds and "aten::empty" not in kinds, kinds
+
+
+def test_lengths_and_masks_that_are_no_tensors_are_refused(calls_on_the_cpu):
+    from backtoreality_amd.groupfree import decoder_ops
+    x = torch.randn(1, 4, 1, 8)
+    for kw in (dict(key_lengths=[4]), dict(key_padding_mask=[[False] * 4])):
+        with pytest.raises(RuntimeError, match="should be"):
+            decoder_ops.cross_attention(x, x, x, **kw)
