@@ -239,8 +239,13 @@ class _Linear(Function):
 def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x weight^T + bias) + residual: x (..., k), weight (n, k), bias (n) or None, activation
     None / "relu" / "gelu" (the erf form), residual (..., n) or None.  Sums, activation and residual
-    in float32, rounded once.  (float32 rows run as sums of three bfloat16 terms, exact to the 24th
-    bit: an infinite element makes the sums it enters NaN.)"""
+    in float32, rounded once.
+
+    Gradients: the gradient of the sum, dy act', enters the two products in the type of x; bfloat16 and
+    float16 layers keep GELU's slope in 16 bits (2^-16, small ones of the negative tail 2^-10 of
+    themselves, 0 below 2^-30).  ReLU is on where its rounded result is positive or NaN.  float32 rows
+    run as sums of three bfloat16 terms, exact to the 24th bit (elements below 2^-108 keep fewer), without
+    the three smallest of their nine products; an infinite element makes the sums it enters NaN."""
     _check_ref("linear", x)
     _check_one("linear", "weight", weight, x)
     act = _ACTIVATIONS.get(activation)
@@ -327,7 +332,11 @@ def cross_attention(query, key, value, key_lengths=None, key_padding_mask=None, 
     (query head i reads key head i // (H // Hk)), D <= 128; result (B, Lq, H, D).  Of batch entry b
     the keys from key_lengths[b] (int32 (B), on the device) on and those where key_padding_mask (bool
     (B, Lk)) is True take no part, whatever they hold; a query left without keys gets zeros, and gives
-    none of its gradient to anybody.  scale: D ** -0.5 by default, positive."""
+    none of its gradient to anybody.  scale: D ** -0.5 by default, positive.
+
+    Scores, softmax statistics and sums in float32.  For bfloat16 and float16 the probabilities (and in
+    the backward the scores' gradients) enter the products in 16 bits, half a step off each, and the
+    backward's rowsum(dout out) takes the rounded result."""
     _check_ref("cross_attention", query)
     _check_one("cross_attention", "key", key, query)
     _check_one("cross_attention", "value", value, query)

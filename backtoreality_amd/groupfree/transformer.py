@@ -6,7 +6,8 @@ reference vendors a copy of (models/multi_head_attention.py), same parameter nam
 GPU the whole layer is one library call (groupfree/fused_decoder.py -> csrc/decoder.hip); the
 op-by-op form below (attention core through groupfree/fused_attention.py) is the CPU path and
 what `BTR_FUSED_DECODER=0` selects.  Layers in bfloat16 / float16 and keys with padding
-(`key_padding_mask`) run on the operators of groupfree/decoder_ops.py."""
+(`key_padding_mask`) run on the operators of groupfree/decoder_ops.py where those do what the modules
+would (`_ops_covered`)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
