@@ -12,8 +12,8 @@ parameters (same state-dict keys: in_proj_weight / in_proj_bias / out_proj.*):
 
 and its backward through btr_attention_bwd (dq / dk / dv written straight into the packed
 gradient of the projection output).  Returns None when the configuration is not covered
-(CPU tensors, other types or autocast, masks, bias_k / add_zero_attn, separate q/k/v widths): the caller then runs the
-stock module.  `BTR_FUSED_ATTENTION=0` disables it.
+(CPU tensors, other types or autocast, masks, bias_k / add_zero_attn, separate q/k/v widths):
+the caller then runs the stock module.  `BTR_FUSED_ATTENTION=0` disables it.
 
 Dropout masks come from a counter-based hash of (a host seed unique per call, a device step
 counter, the element index): `bump_step()` once per training step makes a replayed HIP graph
