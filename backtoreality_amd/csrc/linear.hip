@@ -90,16 +90,19 @@ __device__ __forceinline__ f32x16_t mfma(f16x8_t a, f16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// f = h + m + l.  Above bf16's largest value h is cut instead of rounded (rounded it would be infinite); an
-// infinite element keeps no rest.
+constexpr float kBf16End = 0x1.ffp127f;   // from here on bf16 rounds to infinity
+// f = h + m + l.  FAR, where an element is above bf16's largest value: its h is cut instead of rounded
+// (rounded it would be infinite), and an infinite element keeps no rest.
+template <bool FAR>
 __device__ __forceinline__ void split3(f32x4_t f, bf16x4_t (&p)[3]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const float size = __builtin_fabsf(f[i]);
     __bf16 h = (__bf16)f[i];
-    if (!(__builtin_fabsf((float)h) < INFINITY) && __builtin_fabsf(f[i]) < INFINITY)
+    if (FAR && size >= kBf16End && size < INFINITY)
       h = __builtin_bit_cast(__bf16, (unsigned short)(__float_as_uint(f[i]) >> 16));
     float r = f[i] - (float)h;
-    if (!(__builtin_fabsf((float)h) < INFINITY)) r = 0.f;
+    if (FAR && size == INFINITY) r = 0.f;
     const __bf16 m = (__bf16)r;
     p[0][i] = h;
     p[1][i] = m;
@@ -118,8 +121,17 @@ template <typename V>
 __device__ __forceinline__ void pack(const V (&v)[1], V (&f)[1]) { f[0] = v[0]; }
 __device__ __forceinline__ void pack(const f32x4_t (&v)[2], bf16x8_t (&f)[3]) {
   bf16x4_t a[3], b[3];
-  split3(v[0], a);
-  split3(v[1], b);
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    top = fmaxf(fmaxf(top, __builtin_fabsf(v[0][i])), __builtin_fabsf(v[1][i]));
+  if (__builtin_expect(__ballot(top >= kBf16End) != 0, 0)) {   // (per element: 33 -> 39 us at 32 x 4 096
+    split3<true>(v[0], a);                                      // x 4 096)
+    split3<true>(v[1], b);
+  } else {
+    split3<false>(v[0], a);
+    split3<false>(v[1], b);
+  }
 #pragma unroll
   for (int p = 0; p < 3; ++p)
     f[p] = __builtin_shufflevector(a[p], b[p], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -1010,8 +1022,8 @@ int check(const char *what, const btr_linear_t *p) {
 
 // Does linear_rows_kernel take a forward product with `few` rows (or outputs) against `many` outputs
 // (or rows)?  f32: up to 64, where the tiled kernels would first write three planes of the long operand
-// (rows x reduction x outputs, 32 x 4 096 x 4 096: 64 -> 31 us, 64 x 4 096 x 4 096: 68 -> 48, 30 000 x
-// 2 048 x 64: 274 -> 157; of what was timed only 30 000 x 128 x 64 loses, 28 -> 33).  16 bits: up to 32
+// (rows x reduction x outputs, 32 x 4 096 x 4 096: 64 -> 33 us, 64 x 4 096 x 4 096: 68 -> 50, 30 000 x
+// 2 048 x 64: 274 -> 165; of what was timed only 30 000 x 128 x 64 loses, 28 -> 33).  16 bits: up to 32
 // while a round of workgroups covers the long side and the reduction is short (4 096 x 2 048 x 32 bf16:
 // 10.6 -> 9.5, 1 024 x 288 x 23 off 16-byte boundaries 9.2 -> 6.1; beyond: 30 000 x 128 x 23 8 -> 33,
 // 2 048 x 4 096 x 32 12 -> 15).
